@@ -371,6 +371,90 @@ int mvb_paged_decode_noalloc(const void* query, int64_t q_stride_seq, int64_t q_
                              float scale, int32_t dtype, int32_t variant, int32_t partition_tokens,
                              int32_t* error_flags, void* stream);
 
+/* ---- the 8-bit KV cache ---------------------------------------------------
+ * No reference counterpart (its pool has 16 or 32 bits).  key_cache and
+ * value_cache hold float8 e4m3 codes (no infinities) in the pool's layout
+ * [num_blocks][num_kv_heads][block_size][head_dim]; kv_scale, float32
+ * [num_blocks][num_kv_heads][2], holds the scale of the keys and the scale of
+ * the values of each (block, KV head).  An element stands for code * scale.
+ * Caches are 16-byte, kv_scale 8-byte aligned; block_size is a power of two
+ * from 16 to 1024, head_dim 64 or 128, dtype (of query, key, value and output)
+ * f16 or bf16.  Rows of query, key, value and outputs are 16-byte aligned
+ * (strides multiples of 8 elements). */
+
+/* Write of new key / value rows into the 8-bit cache, slots as in
+ * mvb_kv_cache_write.  For a block b that the call writes to, each KV head, and
+ * keys and values apart, with x the call's rows for it in float32:
+ *   base = 0 if the call writes slot 0 of b (the block starts anew) or b's scale
+ *          is not a positive finite number, else b's scale
+ *   s    = max(base, the smallest power of two s >= 2^-100 with max|x| <= 448 s)
+ *   codes of the block's other rows = round(code * (base / s)), where s > base > 0
+ *   codes of the rows               = round(x * (1 / s)),  kv_scale = s
+ * round is to the nearest e4m3 value, ties to even; max runs over the finite
+ * elements, infinities are stored as +-448 s, NaN as NaN.  A block is to be
+ * filled from slot 0 on.  Two tokens with one slot set MVB_DEV_DUP_SLOT (one of
+ * the two is written).  The call needs
+ * the bytes of workspace that mvb_kv_cache_write_fp8_workspace reports (0 for few tokens; 4-byte aligned, contents arbitrary before and
+ * after); calls that may overlap on the GPU need one each.  Calls that write
+ * to one block must be ordered. */
+int mvb_kv_cache_write_fp8(const void* key, int64_t k_stride_token, int64_t k_stride_head, const void* value,
+                           int64_t v_stride_token, int64_t v_stride_head, void* key_cache, void* value_cache,
+                           float* kv_scale, const int64_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t dtype, void* workspace,
+                           int64_t workspace_bytes, int32_t* error_flags, void* stream);
+int mvb_kv_cache_write_fp8_workspace(int32_t num_tokens, int32_t num_blocks, int32_t block_size, int64_t* bytes_out);
+
+/* Rotary embedding of the step's query and key rows fused with
+ * mvb_kv_cache_write_fp8 of the rotated keys and the values:
+ *   out = x * cos[pos] + rotate_half(x) * sin[pos]
+ * (mini_vllm/model/rotary.py:47-85) computed in float32 and rounded once: to
+ * dtype for query_out and key_out, to the cache's codes for the keys (the
+ * exact rotation rounded to float32 is what is coded).  The tables are
+ * contiguous [table_rows, head_dim] of `table_dtype`, which is dtype or
+ * MVB_DTYPE_F32.  query_out may equal query; key_out (optional) is contiguous
+ * [T, KH, D].  A position outside [0, table_rows) sets MVB_DEV_POSITION and
+ * leaves all of that token's rows unwritten; slot -1 rotates the query and
+ * writes nothing. */
+int mvb_rope_kv_cache_write_fp8(const void* query, int64_t q_stride_token, int64_t q_stride_head, void* query_out,
+                                int64_t qo_stride_token, int64_t qo_stride_head, const void* key,
+                                int64_t k_stride_token, int64_t k_stride_head, const void* value,
+                                int64_t v_stride_token, int64_t v_stride_head, const int64_t* positions,
+                                const void* cos_table, const void* sin_table, int64_t table_rows,
+                                int32_t table_dtype, void* key_cache, void* value_cache, float* kv_scale,
+                                const int64_t* slot_mapping, void* key_out, int32_t num_tokens, int32_t num_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks,
+                                int32_t dtype, void* workspace, int64_t workspace_bytes, int32_t* error_flags,
+                                void* stream);
+
+/* Paged decode attention over the 8-bit cache, one query token per sequence;
+ * arguments, zero rows and device errors as in mvb_paged_decode (at most 8192
+ * sequences).  `workspace` holds mvb_paged_decode_fp8_workspace bytes (same
+ * arguments; 256-byte aligned, contents arbitrary before and after); calls
+ * that may overlap on the GPU need one each. */
+int mvb_paged_decode_fp8(const void* query, int64_t q_stride_seq, int64_t q_stride_head, const void* key_cache,
+                         const void* value_cache, const float* kv_scale, const int64_t* block_table,
+                         int64_t block_table_stride, int32_t max_blocks_per_seq, const int32_t* kv_len, void* out,
+                         int64_t out_stride_seq, int64_t out_stride_head, int32_t num_seqs, int32_t num_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks, float scale,
+                         int32_t dtype, void* workspace, int64_t workspace_bytes, int32_t* error_flags,
+                         void* stream);
+int mvb_paged_decode_fp8_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                   int32_t block_size, int32_t num_blocks, int32_t max_blocks_per_seq, int32_t dtype,
+                                   int64_t* bytes_out);
+
+/* Causal paged prefill attention over the 8-bit cache: mvb_paged_prefill with
+ * every position, the chunk's own among them, read from the cache (written
+ * before the call).  A block id outside [0, num_blocks) sets MVB_DEV_BLOCK_ID
+ * and its tokens are left out. */
+int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, int64_t q_stride_head, const void* key_cache,
+                          const void* value_cache, const float* kv_scale, const int64_t* block_table,
+                          int64_t block_table_rows, int64_t block_table_stride, int32_t max_blocks_per_seq,
+                          const int64_t* seq_rows, const int64_t* cached_len, const int64_t* query_len,
+                          int32_t num_chunks, int32_t total_q, void* out, int64_t out_stride_tok,
+                          int64_t out_stride_head, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t block_size, int32_t num_blocks, float scale, int32_t dtype, int32_t* error_flags,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

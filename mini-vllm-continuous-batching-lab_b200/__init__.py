@@ -18,10 +18,14 @@ from .attention import (
     gather_paged_kv,
     gather_prefix_kv,
     paged_cache_write,
+    paged_cache_write_fp8,
     paged_decode_attention,
+    paged_decode_attention_fp8,
     paged_gather,
     paged_prefill_attention,
+    paged_prefill_attention_fp8,
     rope_cache_write,
+    rope_cache_write_fp8,
     rope_tables,
     triton_cache_write,
     triton_decode_attention,
@@ -52,10 +56,14 @@ __all__ = [
     "gather_paged_kv",
     "gather_prefix_kv",
     "paged_cache_write",
+    "paged_cache_write_fp8",
     "paged_decode_attention",
+    "paged_decode_attention_fp8",
     "paged_gather",
     "paged_prefill_attention",
+    "paged_prefill_attention_fp8",
     "rope_cache_write",
+    "rope_cache_write_fp8",
     "rope_tables",
     "triton_cache_write",
     "triton_decode_attention",

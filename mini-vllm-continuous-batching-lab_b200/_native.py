@@ -51,7 +51,7 @@ DECODE_SCHED = 4
 DECODE_AFTER_WRITE = 0x100
 DECODE_SCHEDULE_READY = 0x200
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 # Every symbol include/mini_vllm_b200.h declares, with (restype, argtypes).
 _i32, _i64, _u32, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_uint32, ctypes.c_float, ctypes.c_void_p
@@ -106,6 +106,28 @@ SIGNATURES = {
         _i32,
         [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64,
          _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _i32, _vp, _vp],
+    ),
+    "mvb_kv_cache_write_fp8": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+         _vp, _i64, _vp, _vp],
+    ),
+    "mvb_kv_cache_write_fp8_workspace": (_i32, [_i32, _i32, _i32, _p_i64]),
+    "mvb_rope_kv_cache_write_fp8": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i32,
+         _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _vp],
+    ),
+    "mvb_paged_decode_fp8": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64,
+         _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64, _vp, _vp],
+    ),
+    "mvb_paged_decode_fp8_workspace": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p_i64]),
+    "mvb_paged_prefill_fp8": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i64,
+         _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp],
     ),
 }
 

@@ -1021,6 +1021,11 @@ class AttentionBackendB200(AttentionBackend):
       kernel for bf16/f16, FMA kernel otherwise, split-K for long contexts);
     * ``prefill_attention`` → torch gather of the paged prefix by index
       tensors plus SDPA (no Triton; the reference's C3 path, :577-661).
+
+    With ``allocate_pool(..., dtype=torch.float8_e4m3fn)`` the pool is held in 8
+    bits with a scale per (block, KV head) and the methods run the functions of
+    ``paged_attention_fp8.py``; ``decode_variant``, ``partition_tokens`` and
+    ``overlap_after_write`` have no effect then.
     """
 
     def __init__(self, config: Any, *, strict: bool = True, decode_variant: str = "auto",
@@ -1066,6 +1071,8 @@ class AttentionBackendB200(AttentionBackend):
     def allocate_pool(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int,
                       head_dim: int, dtype: torch.dtype, device: torch.device) -> KVCachePool:
         validate_block_size(block_size)
+        if dtype == torch.float8_e4m3fn and not 16 <= block_size <= 1024:
+            raise RuntimeError(f"AttentionBackendB200: block_size={block_size} of an 8-bit pool must be 16 to 1024.")
         pool = KVCachePool.allocate(num_layers, num_blocks, block_size, num_kv_heads, head_dim,
                                     dtype, device)
         self._pool = pool
@@ -1077,6 +1084,12 @@ class AttentionBackendB200(AttentionBackend):
         pool = self._pool
         assert pool is not None, "allocate_pool must be called first"
         self._last_write = None
+        if getattr(pool, "kv_scales", None) is not None:
+            from .paged_attention_fp8 import paged_cache_write_fp8
+
+            paged_cache_write_fp8(key, value, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
+                                  pool.kv_scales[layer_idx], slot_mapping, pool.block_size, strict=self.strict)
+            return
         paged_cache_write(key, value, pool.key_caches[layer_idx], pool.value_caches[layer_idx],
                           slot_mapping, pool.block_size, strict=self.strict)
         if self.overlap_after_write and key.shape[0] > 0:
@@ -1100,6 +1113,12 @@ class AttentionBackendB200(AttentionBackend):
         after = last is not None and query.is_cuda and last == (layer_idx, _stream_handle(query.get_device()))
         kc, vc = pool.key_caches[layer_idx], pool.value_caches[layer_idx]
         bt, kvl = attn_metadata.decode_block_tables, group.kv_len_after
+        scales = getattr(pool, "kv_scales", None)
+        if scales is not None:
+            from .paged_attention_fp8 import paged_decode_attention_fp8
+
+            return paged_decode_attention_fp8(query, kc, vc, scales[layer_idx], bt, kvl, pool.block_size, out=out,
+                                              strict=self.strict)
         schedule = self._step_schedule(layer_idx, query, kc, bt, kvl, attn_metadata, pool.block_size, after)
         if schedule is not None and self._schedule_built_now:
             after = False  # the decode now follows the schedule launch, not the write
@@ -1169,12 +1188,18 @@ class AttentionBackendB200(AttentionBackend):
         groups = [g for g in attn_metadata.groups if g.attention_type in ("prefill_gpu", "prefill_ref")]
         if not groups:
             return query
-        if query.dtype not in (torch.bfloat16, torch.float16) or query.shape[2] not in (64, 128):
+        scales = getattr(pool, "kv_scales", None)
+        if scales is None and (query.dtype not in (torch.bfloat16, torch.float16) or query.shape[2] not in (64, 128)):
             return self._prefill_general(layer_idx, query, key, value, attn_metadata, pool)
         dev = query.device
         rows = torch.cat([torch.as_tensor(g.seq_indices, dtype=torch.int64).to(dev) for g in groups])
         cached = torch.cat([g.cached_len_before.to(device=dev, dtype=torch.int64).reshape(-1) for g in groups])
         qlen = torch.cat([g.query_len.to(device=dev, dtype=torch.int64).reshape(-1) for g in groups])
+        if scales is not None:  # the chunk is read back from the cache, as the decode steps after it will
+            from .paged_attention_fp8 import paged_prefill_attention_fp8
+
+            return paged_prefill_attention_fp8(query, kc, vc, scales[layer_idx], attn_metadata.prefill_block_tables,
+                                               rows, cached, qlen, pool.block_size, strict=self.strict)
         with_chunk = key is not None and value is not None
         return paged_prefill_attention(query, kc, vc, attn_metadata.prefill_block_tables, rows, cached, qlen,
                                        pool.block_size, key=key if with_chunk else None,

@@ -11,6 +11,11 @@ bf16 at block_size 16 / head_dim 64 — which is the unit the decode kernel's
 TMA tile loads move (16 token rows at a time).  Memory is not zeroed: readers
 never look past ``kv_len`` (the decode kernel masks and zeroes the tail of a
 partial last tile in shared memory instead).
+
+With ``dtype=torch.float8_e4m3fn`` (an extension) the caches hold codes and
+``kv_scales`` one float32 ``[num_blocks, num_kv_heads, 2]`` tensor per layer:
+the scale of the keys and of the values of each (block, KV head).  Scales start
+at zero, which the first write of a block replaces.
 """
 
 from __future__ import annotations
@@ -26,6 +31,12 @@ MIN_BLOCKS = 16
 _WORKSPACE_RESERVE = 256 * 1024 * 1024
 
 
+def _block_bytes(num_kv_heads: int, block_size: int, head_dim: int, dtype: torch.dtype) -> int:
+    """Bytes of one block of one layer, keys and values (and the scales of an 8-bit pool)."""
+    scales = 8 if dtype == torch.float8_e4m3fn else 0
+    return num_kv_heads * (2 * block_size * head_dim * dtype.itemsize + scales)
+
+
 @dataclass
 class KVCachePool:
     key_caches: List[torch.Tensor]
@@ -37,6 +48,7 @@ class KVCachePool:
     head_dim: int
     device: torch.device
     dtype: torch.dtype
+    kv_scales: Optional[List[torch.Tensor]] = None  # 8-bit pools only
 
     @staticmethod
     def allocate(
@@ -69,8 +81,11 @@ class KVCachePool:
         shape = (num_blocks, num_kv_heads, block_size, head_dim)
         keys = [torch.empty(shape, dtype=dtype, device=dev) for _ in range(num_layers)]
         values = [torch.empty(shape, dtype=dtype, device=dev) for _ in range(num_layers)]
+        scales = None
+        if dtype == torch.float8_e4m3fn:
+            scales = [torch.zeros((num_blocks, num_kv_heads, 2), device=dev) for _ in range(num_layers)]
         return KVCachePool(keys, values, num_blocks, block_size, num_layers, num_kv_heads,
-                           head_dim, dev, dtype)
+                           head_dim, dev, dtype, scales)
 
     def get_key_cache(self, layer_idx: int) -> torch.Tensor:
         return self.key_caches[layer_idx]
@@ -83,6 +98,8 @@ class KVCachePool:
         for k, v in zip(self.key_caches, self.value_caches):
             k.zero_()
             v.zero_()
+        for scale in self.kv_scales or []:
+            scale.zero_()
 
     @property
     def total_slots(self) -> int:
@@ -91,7 +108,7 @@ class KVCachePool:
 
     @property
     def bytes_per_block_per_layer(self) -> int:
-        return 2 * self.num_kv_heads * self.block_size * self.head_dim * self.dtype.itemsize
+        return _block_bytes(self.num_kv_heads, self.block_size, self.head_dim, self.dtype)
 
     @property
     def bytes_per_block_total(self) -> int:
@@ -143,5 +160,5 @@ def compute_num_gpu_blocks(
             f"peak={peak_runtime_estimate}, workspace={workspace_reserve}"
         )
     budget = int(post * gpu_memory_utilization)
-    per_block = num_layers * 2 * num_kv_heads * block_size * head_dim * dtype.itemsize
+    per_block = num_layers * _block_bytes(num_kv_heads, block_size, head_dim, dtype)
     return max(MIN_BLOCKS, budget // per_block)

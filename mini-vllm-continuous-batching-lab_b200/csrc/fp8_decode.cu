@@ -1,0 +1,722 @@
+// mvb_paged_decode_fp8: attention of one query token per sequence over an
+// 8-bit paged cache with a scale per (block, KV head):
+//   out[s, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - max),
+//   k_j = code * kv_scale[block(j), kvh, 0],  v_j = code * kv_scale[block(j), kvh, 1].
+//
+// Math of one 16-token tile (one warp).  The tile's tokens are the rows of the
+// tensor-core product and the KV head's query heads its 8 columns (a head
+// group; 16 heads are two column blocks), so 7 heads waste one column where
+// heads as rows would waste 9 of 16:
+//   S^T[16 tokens, 8 heads] = K_codes Q^T,   O^T[D, 8 heads] = V_codes^T P^T.
+// * Codes go to f16 (exact) in registers, straight from global memory: the sum
+//   over D may run in any order, so a lane's 16 contiguous bytes of a K row
+//   serve four k-steps, and its 8 (D = 64) or 16 contiguous bytes of four V rows
+//   are D/8 rows of O^T.  No shared memory lies between the cache and the tensor
+//   core.
+// * The query enters as f16, each head's row times a power of two that brings
+//   its largest element into [1, 2): exact for f16 queries and for bf16 ones but
+//   for elements below 2^-14 of the row's largest, which lose bits under 2^-24
+//   of it.
+// * All tokens of a tile lie in one block, so the key scale is one factor of the
+//   tile's logits and the value scale one factor of its O^T contribution; both
+//   multiply 32-bit results.
+// * p enters as f16 (11 bits; the output has 8 or 11).  The running maximum m is
+//   moved only when a logit exceeds it by 8 (in powers of two): p <= 2^8 then,
+//   and a tile needs no reduction across lanes, only a vote.
+//
+// Work split: the tiles of all (sequence, KV head, head group) units in order
+// are one stream, cut into equal ranges, one per warp of a grid of at most one
+// CTA per SM.  A unit inside a warp's range is written at once.  The pieces of
+// units cut between the warps of a CTA are merged in shared memory; only a unit
+// cut between two CTAs leaves partial states in global memory, which
+// fp8_decode_merge_kernel joins in CTA order.  The workspace holds nothing from
+// one call to the next and needs no initialisation.
+// Bound: memory (1 byte per element; 28 operations per byte at 7 heads).
+#include "fp8_common.cuh"
+
+namespace mvb {
+
+struct Fp8DecodeArgs {
+  const void* q;
+  int64_t q_s0, q_s1;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float2* scale;  // [num_blocks, KH] (key, value)
+  const int64_t* bt;
+  int64_t bt_s0;
+  int max_blocks;
+  const int* kv_len;
+  void* out;
+  int64_t o_s0, o_s1;
+  int num_seqs, num_heads, num_kv_heads, G, head_groups, block_shift, num_blocks;
+  float scale_log2;
+  float* part;  // [grid][2][16 * (D + 2)] partial states of units cut between CTAs: O, then (m, l)
+  int4* desc;   // [grid][2] {unit (-1: none), sequence, first head, heads}; slot 0: the unit began earlier
+  int* err;
+};
+
+namespace {
+
+constexpr int kFp8Tile = 16;
+constexpr int kFp8DecodeMaxSeqs = 8192;
+// A warp gets at least this many tiles where the batch has few.
+constexpr int kFp8MinTiles = 2;
+
+// Geometry by head_dim and column blocks: warps per CTA and tiles a warp loads ahead.
+template <int D, int NG> struct Fp8Geo;
+template <> struct Fp8Geo<64, 1> { static constexpr int NW = 16, DEPTH = 2; };
+template <> struct Fp8Geo<64, 2> { static constexpr int NW = 12, DEPTH = 2; };
+template <> struct Fp8Geo<128, 1> { static constexpr int NW = 12, DEPTH = 2; };
+template <> struct Fp8Geo<128, 2> { static constexpr int NW = 8, DEPTH = 2; };
+
+template <int D, int NG>
+int decode_smem(int num_seqs) {
+  constexpr int NW = Fp8Geo<D, NG>::NW, HR = 8 * NG;
+  return NW * 2 * HR * (D + 2) * 4 + NW * 2 * 16 + (2 * num_seqs + 1) * 4;
+}
+
+__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// One unit of the stream.
+struct Unit {
+  int start, end;  // its tiles [start, end) of the stream
+  int seq, k;      // sequence, unit of the sequence
+  int ctx;         // tokens
+};
+
+// Weighted sum of the pieces' states of one head row: lane i < n holds piece
+// i's (m, l) and calls `o(i, d)` for its sums.  Writes O to dst(d, value) with
+// the factor `norm ? 1 / L : 1` and returns (M, L).
+template <int D, typename LoadO, typename Store>
+__device__ __forceinline__ float2 merge_row(int n, float m, float l, bool norm, LoadO o, Store st) {
+  const int lane = threadIdx.x & 31;
+  float M = m;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  const float w = m == -INFINITY ? 0.f : fast_exp2(m - M);
+  float L = w * l;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
+  float acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int p = 0; p < n; ++p) {
+    const float wp = __shfl_sync(0xffffffffu, w, p);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(wp, o(p, lane + 32 * i), acc[i]);
+  }
+  const float f = !norm ? 1.f : L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) st(lane + 32 * i, acc[i] * f);
+  return make_float2(M, L);
+}
+
+template <typename T, int D, int NG>
+__global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(const Fp8DecodeArgs a) {
+  constexpr int NW = Fp8Geo<D, NG>::NW, DEPTH = Fp8Geo<D, NG>::DEPTH;
+  constexpr int HR = 8 * NG, MT = D / 16, KS = D / 16, KW = D / 64;
+  constexpr int PIECE = HR * (D + 2);  // floats of one partial state: O [HR][D], then (m, l) [HR]
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* parts = reinterpret_cast<float*>(smem);                       // [NW][2][PIECE]
+  int4* ids = reinterpret_cast<int4*>(smem + NW * 2 * PIECE * 4);      // [NW][2] {unit, seq, k, ends in this CTA}
+  int* pre = reinterpret_cast<int*>(ids + NW * 2);                     // [Nd + 1] tile prefix
+  int* ctxs = pre + a.num_seqs + 1;                                    // [Nd] tokens (0: left out)
+  __shared__ int sums[NW];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int Nd = a.num_seqs, KHG = a.num_kv_heads * a.head_groups;
+  T* const out = static_cast<T*>(a.out);
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  // ---- tiles of every sequence (all its units) and their exclusive prefix ----
+  {
+    constexpr int NT = NW * 32;
+    const int per = (Nd + NT - 1) / NT;
+    const int i0 = min(Nd, tid * per), i1 = min(Nd, i0 + per);
+    int mine = 0;
+    for (int i = i0; i < i1; ++i) {
+      const int c = __ldg(a.kv_len + i);
+      const int bad = c < 1 ? MVB_DEV_KV_LEN
+                      : ((int64_t)c + (1 << a.block_shift) - 1) >> a.block_shift > a.max_blocks ? MVB_DEV_TABLE_SHORT
+                                                                                               : 0;
+      const int n = bad ? 0 : ((c + kFp8Tile - 1) / kFp8Tile) * KHG;
+      ctxs[i] = bad ? 0 : c;
+      pre[i] = n;
+      mine += n;
+      if (bad && blockIdx.x == 0) atomicOr(a.err, bad);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) sums[warp] = incl;
+    if (tid < NW * 2) ids[tid] = make_int4(-1, 0, 0, 0);
+    __syncthreads();
+    int run = incl - mine, total = 0;
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) run += sums[w];
+      total += sums[w];
+    }
+    for (int i = i0; i < i1; ++i) {
+      const int n = pre[i];
+      pre[i] = run;
+      run += n;
+    }
+    if (tid == 0) pre[Nd] = total;
+    __syncthreads();
+  }
+  // rows of sequences that cannot be served: zeros
+  for (int i = blockIdx.x * NW + warp; i < Nd; i += gridDim.x * NW) {
+    if (ctxs[i] != 0) continue;
+    for (int e = lane; e < a.num_heads * D; e += 32)
+      out[(int64_t)i * a.o_s0 + (int64_t)(e / D) * a.o_s1 + e % D] = from_f32<T>(0.f);
+  }
+
+  const int T_all = pre[Nd];
+  const int ctas = min((int)gridDim.x, max(1, (T_all + NW * kFp8MinTiles - 1) / (NW * kFp8MinTiles)));
+  const int W = ctas * NW, wid = blockIdx.x * NW + warp;
+  auto bound = [&](int w) { return (int)((int64_t)min(w, W) * T_all / W); };
+  const int r0 = bound(wid), r1 = bound(wid + 1);
+  const int c0 = bound(blockIdx.x * NW), c1 = bound(blockIdx.x * NW + NW);
+
+  auto unit_at = [&](int tile) {
+    int lo = 0, hi = Nd;  // pre[lo] <= tile < pre[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= tile)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    Unit u;
+    u.seq = lo;
+    u.ctx = ctxs[lo];
+    const int n = (u.ctx + kFp8Tile - 1) / kFp8Tile;
+    u.k = (tile - pre[lo]) / n;
+    u.start = pre[lo] + u.k * n;
+    u.end = u.start + n;
+    return u;
+  };
+  const int BSm = (1 << a.block_shift) - 1;
+  // Lane-wise: where tile `tile` of the stream lies: (block, KV head) row and
+  // the tile's first token in the block; row -1 for a bad block id.
+  auto find_tile = [&](int tile, int& row, int& at) {
+    const Unit u = unit_at(tile);
+    const int tok = (tile - u.start) * kFp8Tile;
+    const int64_t b = __ldg(a.bt + (int64_t)u.seq * a.bt_s0 + (tok >> a.block_shift));
+    at = tok & BSm;
+    row = b >= 0 && b < a.num_blocks ? (int)b * a.num_kv_heads + u.k / a.head_groups : -1;
+    if (row < 0) atomicOr(a.err, MVB_DEV_BLOCK_ID);
+  };
+
+  if (r0 < r1) {
+    // 32 tiles' places and scales at a time, one per lane; the next 32 are fetched ahead
+    int row = -1, at = 0, row_n = -1, at_n = 0;
+    float2 sc = make_float2(0.f, 0.f);
+    if (r0 + lane < r1) find_tile(r0 + lane, row, at);
+    if (row >= 0) sc = __ldg(a.scale + row);
+    if (r0 + 32 + lane < r1) find_tile(r0 + 32 + lane, row_n, at_n);
+
+    uint4 kr[DEPTH][2 * KW];  // rows g and g + 8, 16 bytes per 64 columns
+    uint4 vr[DEPTH][KW == 1 ? 2 : 4];  // rows 2t, 2t+1, 2t+8, 2t+9: 8 (16) bytes each
+    auto tile_off = [&](int j) -> int64_t {  // byte offset of the tile `j` places into the current 32 (may be the next's)
+      const int rw = j < 32 ? __shfl_sync(0xffffffffu, row, j & 31) : __shfl_sync(0xffffffffu, row_n, j & 31);
+      const int ta = j < 32 ? __shfl_sync(0xffffffffu, at, j & 31) : __shfl_sync(0xffffffffu, at_n, j & 31);
+      return (((int64_t)max(rw, 0) << a.block_shift) + ta) * D;
+    };
+    auto load_k = [&](uint4 (&k)[2 * KW], int64_t off) {
+      const uint8_t* p = a.kc + off + 16 * t4;
+#pragma unroll
+      for (int c = 0; c < KW; ++c) {
+        k[2 * c] = ld_stream16(p + g * D + 64 * c);
+        k[2 * c + 1] = ld_stream16(p + (g + 8) * D + 64 * c);
+      }
+    };
+    auto load_v = [&](uint4 (&v)[KW == 1 ? 2 : 4], int64_t off) {
+      const uint8_t* p = a.vc + off + 2 * t4 * D + (D / 8) * g;
+      if constexpr (KW == 1) {
+        const uint2 x = ld_stream8(p), y = ld_stream8(p + D), z = ld_stream8(p + 8 * D), w = ld_stream8(p + 9 * D);
+        v[0] = make_uint4(x.x, x.y, y.x, y.y);
+        v[1] = make_uint4(z.x, z.y, w.x, w.y);
+      } else {
+        v[0] = ld_stream16(p);
+        v[1] = ld_stream16(p + D);
+        v[2] = ld_stream16(p + 8 * D);
+        v[3] = ld_stream16(p + 9 * D);
+      }
+    };
+#pragma unroll
+    for (int b = 0; b < DEPTH; ++b)
+      if (r0 + b < r1) {
+        const int64_t off = tile_off(b);
+        load_k(kr[b], off);
+        load_v(vr[b], off);
+      }
+
+    Unit u = unit_at(r0);
+    uint32_t qf[NG][KS][2];
+    float qs[NG][2];  // per column (heads 2t, 2t + 1): softmax scale, log2 e, the query row's power of two
+    float o[NG][MT][4], m[NG][2], l[NG][2];
+    int h0 = 0, nh = 0;
+    auto begin_unit = [&]() {
+      const int kvh = u.k / a.head_groups, hg = u.k - kvh * a.head_groups;
+      h0 = kvh * a.G + hg * HR;
+      nh = min(HR, a.G - hg * HR);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const int h = 8 * n + g;
+        const T* qp = static_cast<const T*>(a.q) + (int64_t)u.seq * a.q_s0 + (int64_t)(h0 + h) * a.q_s1;
+        float x[KW][16], amax = 0.f;
+#pragma unroll
+        for (int c = 0; c < KW; ++c) {
+          uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+          if (h < nh) {
+            raw[0] = __ldg(reinterpret_cast<const uint4*>(qp + 64 * c + 16 * t4));
+            raw[1] = __ldg(reinterpret_cast<const uint4*>(qp + 64 * c + 16 * t4) + 1);
+          }
+          const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[c][i] = to_f32<T>(e[i]);
+            const float y = fabsf(x[c][i]);
+            amax = fmaxf(amax, y < INFINITY ? y : 0.f);
+          }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // 2^-e with e = floor(log2 amax), kept where both 2^e and 2^-e are normal
+        const int e = min(max((int)(__float_as_uint(amax) >> 23), 2), 252);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+        for (int c = 0; c < KW; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            qf[n][4 * c + k][0] = pack_h2(x[c][4 * k] * down, x[c][4 * k + 1] * down);
+            qf[n][4 * c + k][1] = pack_h2(x[c][4 * k + 2] * down, x[c][4 * k + 3] * down);
+          }
+        // lane (g, t) holds head 8n + g's factor; its columns are heads 2t and 2t + 1
+        qs[n][0] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * t4) * 4);
+        qs[n][1] = a.scale_log2 * __shfl_sync(0xffffffffu, up, (2 * t4 + 1) * 4);
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      }
+    };
+    // The unit is finished in this range: written, or left as a piece.
+    auto end_unit = [&]() {
+      const bool whole = u.start >= r0 && u.end <= r1;
+      const int slot = u.start < r0 ? 0 : 1;
+      float* P = parts + (warp * 2 + slot) * PIECE;
+      if (!whole && lane == 0) ids[warp * 2 + slot] = make_int4(u.start, u.seq, u.k, u.end <= c1 ? 1 : 0);
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float s = l[n][c];
+          s += __shfl_xor_sync(0xffffffffu, s, 4);
+          s += __shfl_xor_sync(0xffffffffu, s, 8);
+          s += __shfl_xor_sync(0xffffffffu, s, 16);
+          const int h = 8 * n + 2 * t4 + c;
+          if (h >= nh) continue;
+          // this lane's D / 8 contiguous dims of head h: element 2i + half of o[i][c + 2 half]
+          if (whole) {
+            const float inv = s == 0.f ? 0.f : 1.f / s;
+            T* p = out + (int64_t)u.seq * a.o_s0 + (int64_t)(h0 + h) * a.o_s1 + (D / 8) * g;
+            uint32_t w[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              T e[2] = {from_f32<T>(o[n][i][c] * inv), from_f32<T>(o[n][i][c + 2] * inv)};
+              w[i] = *reinterpret_cast<uint32_t*>(e);
+            }
+#pragma unroll
+            for (int i = 0; i < MT / 4; ++i)
+              reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          } else {
+            float* p = P + h * D + (D / 8) * g;
+#pragma unroll
+            for (int i = 0; i < MT / 2; ++i)
+              *reinterpret_cast<float4*>(p + 4 * i) =
+                  make_float4(o[n][2 * i][c], o[n][2 * i][c + 2], o[n][2 * i + 1][c], o[n][2 * i + 1][c + 2]);
+            if (g == 0) *reinterpret_cast<float2*>(P + HR * D + 2 * h) = make_float2(m[n][c], s);
+          }
+        }
+    };
+    begin_unit();
+
+    int j = 0;  // the tile's place in the current 32
+    for (int tile = r0; tile < r1;) {
+#pragma unroll
+      for (int b = 0; b < DEPTH; ++b) {
+        if (tile < r1) {
+          if (tile == u.end) {
+            end_unit();
+            u = unit_at(tile);
+            begin_unit();
+          }
+          const int rw = __shfl_sync(0xffffffffu, row, j);
+          const float ks = __shfl_sync(0xffffffffu, sc.x, j), vs = __shfl_sync(0xffffffffu, sc.y, j);
+          int valid = rw < 0 ? 0 : u.ctx - (tile - u.start) * kFp8Tile;  // tokens of the tile that count
+          const bool more = tile + DEPTH < r1;
+          const int64_t next = more ? tile_off(j + DEPTH) : 0;
+          // S^T = K Q^T
+          float s[NG][4];
+#pragma unroll
+          for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+          for (int c = 0; c < KW; ++c) {
+            const uint32_t* x = reinterpret_cast<const uint32_t*>(&kr[b][2 * c]);
+            const uint32_t* y = reinterpret_cast<const uint32_t*>(&kr[b][2 * c + 1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16(x[k], a0, a2);
+              e4m3x4_to_f16(y[k], a1, a3);
+#pragma unroll
+              for (int n = 0; n < NG; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][4 * c + k][0], qf[n][4 * c + k][1]);
+            }
+          }
+          if (more) load_k(kr[b], next);
+          // logits (powers of two) above the running maximum; tokens g and g + 8
+          float y[NG][4];
+          bool jump = false;
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              y[n][i] = fmaf(s[n][i], qs[n][i & 1] * ks, -m[n][i & 1]);
+              if (g + (i >> 1) * 8 >= valid) y[n][i] = -INFINITY;
+              jump |= y[n][i] > 8.f;
+            }
+          }
+          if (__any_sync(0xffffffffu, jump)) {
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float f = qs[n][c] * ks;
+                float mx = m[n][c];
+                if (g < valid) mx = fmaxf(mx, s[n][c] * f);
+                if (g + 8 < valid) mx = fmaxf(mx, s[n][c + 2] * f);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float al = m[n][c] == mx ? 1.f : fast_exp2(m[n][c] - mx);
+                m[n][c] = mx;
+                l[n][c] *= al;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                  o[n][i][c] *= al;
+                  o[n][i][c + 2] *= al;
+                }
+                y[n][c] = g < valid ? fmaf(s[n][c], f, -mx) : -INFINITY;
+                y[n][c + 2] = g + 8 < valid ? fmaf(s[n][c + 2], f, -mx) : -INFINITY;
+              }
+          }
+          uint32_t pb[NG][2];
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              y[n][i] = fast_exp2(y[n][i]);
+              l[n][i & 1] += y[n][i];
+            }
+            pb[n][0] = movmatrix(pack_h2(y[n][0], y[n][1]));
+            pb[n][1] = movmatrix(pack_h2(y[n][2], y[n][3]));
+          }
+          // O^T += vs * (V^T P^T); rows past the last token may hold any bits
+          uint32_t* v = reinterpret_cast<uint32_t*>(&vr[b][0]);
+          constexpr int WR = D / 32;  // words of one V row in this lane
+          if (valid < kFp8Tile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (2 * t4 + (i & 1) + (i >> 1) * 8 >= valid)
+#pragma unroll
+                for (int w = 0; w < WR; ++w) v[i * WR + w] = 0u;
+          }
+#pragma unroll
+          for (int w = 0; w < WR; ++w) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7362 : 0x5140;  // bytes (A0 B0 A1 B1) or (A2 B2 A3 B3)
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16(__byte_perm(v[w], v[WR + w], sel), a0, a1);
+              e4m3x4_to_f16(__byte_perm(v[2 * WR + w], v[3 * WR + w], sel), a2, a3);
+              const int i = 2 * w + half;
+#pragma unroll
+              for (int n = 0; n < NG; ++n) {
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16(x, a0, a1, a2, a3, pb[n][0], pb[n][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][e] = fmaf(x[e], vs, o[n][i][e]);
+              }
+            }
+          }
+          if (more) load_v(vr[b], next);
+          ++tile;
+          if (++j == 32) {
+            j = 0;
+            row = row_n;
+            at = at_n;
+            sc = row >= 0 ? __ldg(a.scale + row) : make_float2(0.f, 0.f);
+            row_n = -1;
+            if (tile + 32 + lane < r1) find_tile(tile + 32 + lane, row_n, at_n);
+          }
+        }
+      }
+    }
+    end_unit();
+  }
+  __syncthreads();
+
+  // ---- units cut inside this CTA: candidates w < NW begin in warp w, candidate
+  // NW began in an earlier CTA; one head row per warp and step ----
+  if (tid < 2) a.desc[blockIdx.x * 2 + tid] = make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  for (int item = warp; item < (NW + 1) * HR; item += NW) {
+    const int cand = item / HR, h = item - cand * HR;
+    const int4 id = cand < NW ? ids[cand * 2 + 1] : ids[0];
+    if (id.x < 0) continue;
+    const int kvh = id.z / a.head_groups, hg = id.z - kvh * a.head_groups;
+    const int hb = kvh * a.G + hg * HR, n_h = min(HR, a.G - hg * HR);
+    if (h >= n_h) continue;
+    // pieces: the first warp's slot 1 (or warp 0's slot 0), then slot 0 of the warps after it
+    const int first = cand < NW ? cand : 0;
+    const int mine = first + lane;  // lane i: warp first + i
+    const bool has = mine < NW && (lane == 0 || ids[mine * 2].x == id.x);
+    const uint32_t mask = __ballot_sync(0xffffffffu, has);
+    const int n = 32 - __clz(mask);
+    auto piece = [&](int i) { return parts + ((first + i) * 2 + (i == 0 && cand < NW ? 1 : 0)) * PIECE; };
+    float pm = -INFINITY, pl = 0.f;
+    if (has) {
+      const float2 ml = *reinterpret_cast<const float2*>(piece(lane) + HR * D + 2 * h);
+      pm = ml.x;
+      pl = ml.y;
+    }
+    const bool whole = cand < NW && id.w != 0;
+    auto load_o = [&](int i, int d) { return (mask >> i) & 1 ? piece(i)[h * D + d] : 0.f; };
+    if (whole) {
+      T* p = out + (int64_t)id.y * a.o_s0 + (int64_t)(hb + h) * a.o_s1;
+      merge_row<D>(n, pm, pl, true, load_o, [&](int d, float x) { p[d] = from_f32<T>(x); });
+    } else {
+      const int slot = cand < NW ? 1 : 0;
+      float* p = a.part + ((int64_t)blockIdx.x * 2 + slot) * 16 * (D + 2);
+      const float2 ml = merge_row<D>(n, pm, pl, false, load_o, [&](int d, float x) { p[h * D + d] = x; });
+      if (lane == 0) {
+        *reinterpret_cast<float2*>(p + HR * D + 2 * h) = ml;
+        if (h == 0) a.desc[blockIdx.x * 2 + slot] = make_int4(id.x, id.y, hb, n_h);
+      }
+    }
+  }
+}
+
+// Joins the partial states of units cut between CTAs: CTA c takes the unit that
+// begins in stream CTA c and runs on; one head row per warp and step, pieces in
+// CTA order, 32 at a time.
+template <typename T, int D, int HR>
+__global__ void __launch_bounds__(256) fp8_decode_merge_kernel(const Fp8DecodeArgs a, int ctas) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 id = __ldcg(a.desc + c * 2 + 1);
+  if (id.x < 0) return;
+  int n = 1;  // pieces: CTA c's slot 1, then slot 0 of the CTAs after it
+  for (int i = c + 1; i < ctas; i += 32) {
+    const bool same = i + lane < ctas && __ldcg(a.desc + (i + lane) * 2).x == id.x;
+    const uint32_t other = ~__ballot_sync(0xffffffffu, same);
+    const int run = other ? __ffs(other) - 1 : 32;
+    n += run;
+    if (run < 32) break;
+  }
+  auto piece = [&](int i) { return a.part + ((int64_t)(c + i) * 2 + (i == 0 ? 1 : 0)) * 16 * (D + 2); };
+  for (int h = warp; h < id.w; h += 8) {
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + HR * D + 2 * h));
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+    float L = 0.f, acc[D / 32];
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float w = 0.f, x = 0.f;
+      if (i0 + lane < n) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(i0 + lane) + HR * D + 2 * h));
+        w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+        x = w * ml.y;
+      }
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+      L += x;
+#pragma unroll 4
+      for (int i = i0; i < min(n, i0 + 32); ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i - i0);
+        const float* p = piece(i) + h * D;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(wi, __ldcg(p + lane + 32 * e), acc[e]);
+      }
+    }
+    const float f = L == 0.f ? 0.f : 1.f / L;
+    T* p = static_cast<T*>(a.out) + (int64_t)id.y * a.o_s0 + (int64_t)(id.z + h) * a.o_s1;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) p[lane + 32 * e] = from_f32<T>(acc[e] * f);
+  }
+}
+
+// CTAs of the stream kernel: one per SM, fewer where the tables bound the work.
+int decode_grid(int num_seqs, int units_per_seq, int max_blocks, int block_size, int nw) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t tiles = (int64_t)num_seqs * units_per_seq * ((int64_t)max_blocks * block_size / kFp8Tile);
+  const int64_t per = (int64_t)nw * kFp8MinTiles;
+  const int64_t want = (tiles + per - 1) / per;
+  return (int)(want < 1 ? 1 : want < sms ? want : sms);
+}
+
+struct Fp8DecodePlan {
+  int head_groups, ng, nw, grid;
+  int64_t off_part, bytes;
+};
+
+int plan_decode(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                int max_blocks, int dtype, Fp8DecodePlan* pl) {
+  if (dtype != MVB_DTYPE_F16 && dtype != MVB_DTYPE_BF16) return MVB_ERR_DTYPE;
+  if (head_dim != 64 && head_dim != 128) return MVB_ERR_HEAD_DIM;
+  if (block_size < kFp8MinBlock || block_size > kFp8MaxBlock || (block_size & (block_size - 1)) != 0)
+    return MVB_ERR_BLOCK_SIZE;
+  if (num_seqs < 0 || num_seqs > kFp8DecodeMaxSeqs || num_heads <= 0 || num_kv_heads <= 0 || num_blocks <= 0 ||
+      max_blocks < 0)
+    return MVB_ERR_INVALID_ARG;
+  if (num_heads % num_kv_heads != 0) return MVB_ERR_HEADS;
+  const int G = num_heads / num_kv_heads;
+  pl->ng = G > 8 ? 2 : 1;
+  pl->head_groups = (G + 8 * pl->ng - 1) / (8 * pl->ng);
+  pl->nw = head_dim == 64 ? (pl->ng == 1 ? Fp8Geo<64, 1>::NW : Fp8Geo<64, 2>::NW)
+                          : (pl->ng == 1 ? Fp8Geo<128, 1>::NW : Fp8Geo<128, 2>::NW);
+  const int units = num_kv_heads * pl->head_groups;
+  // tile and (block, KV head) numbers are 32-bit
+  if ((int64_t)num_seqs * units * ((int64_t)max_blocks * block_size / kFp8Tile + 1) >= ((int64_t)1 << 31) ||
+      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31))
+    return MVB_ERR_INVALID_ARG;
+  pl->grid = decode_grid(num_seqs, units, max_blocks, block_size, pl->nw);
+  pl->off_part = ((int64_t)pl->grid * 32 + 255) / 256 * 256;
+  pl->bytes = pl->off_part + (int64_t)pl->grid * 2 * 16 * (head_dim + 2) * 4;
+  return MVB_OK;
+}
+
+template <typename T, int D, int NG>
+int launch_decode(const Fp8DecodeArgs& a, int grid, cudaStream_t stream) {
+  auto kern = fp8_decode_kernel<T, D, NG>;
+  const int smem = decode_smem<D, NG>(a.num_seqs);
+  // the largest batch's size at once: the attribute is set on the first call only
+  if (ensure_kernel_attrs(kern, decode_smem<D, NG>(kFp8DecodeMaxSeqs)) != cudaSuccess) return MVB_ERR_CUDA;
+  if (launch_pdl(kern, dim3(grid), dim3(Fp8Geo<D, NG>::NW * 32), smem, stream, a) != cudaSuccess) return MVB_ERR_CUDA;
+  if (grid == 1) return MVB_OK;  // no unit is cut between CTAs
+  auto merge = fp8_decode_merge_kernel<T, D, 8 * NG>;
+  if (ensure_kernel_attrs(merge, 0) != cudaSuccess) return MVB_ERR_CUDA;
+  return launch_pdl(merge, dim3(grid), dim3(256), 0, stream, a, grid) == cudaSuccess ? MVB_OK : MVB_ERR_CUDA;
+}
+
+template <typename T>
+int launch_decode_t(const Fp8DecodeArgs& a, int head_dim, const Fp8DecodePlan& pl, cudaStream_t stream) {
+  if (head_dim == 64)
+    return pl.ng == 1 ? launch_decode<T, 64, 1>(a, pl.grid, stream) : launch_decode<T, 64, 2>(a, pl.grid, stream);
+  return pl.ng == 1 ? launch_decode<T, 128, 1>(a, pl.grid, stream) : launch_decode<T, 128, 2>(a, pl.grid, stream);
+}
+
+}  // namespace
+}  // namespace mvb
+
+using namespace mvb;
+
+extern "C" int mvb_paged_decode_fp8_workspace(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                              int32_t head_dim, int32_t block_size, int32_t num_blocks,
+                                              int32_t max_blocks_per_seq, int32_t dtype, int64_t* bytes_out) {
+  Fp8DecodePlan pl;
+  const int st = plan_decode(num_seqs, num_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
+                             dtype, &pl);
+  if (st == MVB_OK && bytes_out) *bytes_out = pl.bytes;
+  return st;
+}
+
+extern "C" int mvb_paged_decode_fp8(const void* query, int64_t q_stride_seq, int64_t q_stride_head,
+                                    const void* key_cache, const void* value_cache, const float* kv_scale,
+                                    const int64_t* block_table, int64_t block_table_stride,
+                                    int32_t max_blocks_per_seq, const int32_t* kv_len, void* out,
+                                    int64_t out_stride_seq, int64_t out_stride_head, int32_t num_seqs,
+                                    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                    int32_t num_blocks, float scale, int32_t dtype, void* workspace,
+                                    int64_t workspace_bytes, int32_t* error_flags, void* stream) {
+  mvb::NvtxRange nvtx_range("mvb_paged_decode_fp8");
+  Fp8DecodePlan pl;
+  const int st = plan_decode(num_seqs, num_heads, num_kv_heads, head_dim, block_size, num_blocks, max_blocks_per_seq,
+                             dtype, &pl);
+  if (st != MVB_OK) return st;
+  if (num_seqs == 0) return MVB_OK;
+  if (!query || !key_cache || !value_cache || !kv_scale || !block_table || !kv_len || !out || !error_flags)
+    return MVB_ERR_INVALID_ARG;
+  if (max_blocks_per_seq > 0 && block_table_stride < max_blocks_per_seq) return MVB_ERR_INVALID_ARG;
+  auto al = [](const void* p, int64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (!al(query, 16) || q_stride_seq % 8 || q_stride_head % 8 || !al(out, 16) || out_stride_seq % 8 ||
+      out_stride_head % 8 || !al(key_cache, 16) || !al(value_cache, 16) || !al(kv_scale, 8))
+    return MVB_ERR_ALIGNMENT;
+  if (workspace == nullptr || workspace_bytes < pl.bytes || !al(workspace, 256)) return MVB_ERR_WORKSPACE;
+  Fp8DecodeArgs a;
+  a.q = query;
+  a.q_s0 = q_stride_seq;
+  a.q_s1 = q_stride_head;
+  a.kc = static_cast<const uint8_t*>(key_cache);
+  a.vc = static_cast<const uint8_t*>(value_cache);
+  a.scale = reinterpret_cast<const float2*>(kv_scale);
+  a.bt = block_table;
+  a.bt_s0 = block_table_stride;
+  a.max_blocks = max_blocks_per_seq;
+  a.kv_len = kv_len;
+  a.out = out;
+  a.o_s0 = out_stride_seq;
+  a.o_s1 = out_stride_head;
+  a.num_seqs = num_seqs;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.G = num_heads / num_kv_heads;
+  a.head_groups = pl.head_groups;
+  a.block_shift = 31 - __builtin_clz(block_size);
+  a.num_blocks = num_blocks;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.desc = static_cast<int4*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.off_part);
+  a.err = error_flags;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == MVB_DTYPE_BF16 ? launch_decode_t<__nv_bfloat16>(a, head_dim, pl, s)
+                                 : launch_decode_t<__half>(a, head_dim, pl, s);
+}

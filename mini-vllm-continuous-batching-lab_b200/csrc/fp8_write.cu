@@ -1,0 +1,442 @@
+// mvb_rope_kv_cache_write_fp8: rotary embedding of a step's queries and keys
+// and the write of the rotated keys and the values into an 8-bit paged cache
+// whose scales belong to (block, KV head).  Without the rotation it is the
+// plain write.
+//
+// What a call does to a block b it writes to, for each KV head and for keys and
+// values apart (x: the call's rows in float32, keys after the rotation):
+//   base  = 0 if the call writes slot 0 of b (the block starts anew), else b's scale
+//   s     = max(base, the smallest power of two that maps max |x| into 448)
+//   codes of the block's other rows = round(code * base / s)   where s > base > 0
+//   codes of the rows x             = round(x / s)
+// round is to the nearest e4m3 value, ties to even.  With powers of two the
+// quotients are exact, so rows that are rounded anew keep their values except
+// where these fall below the smallest normal code (2^-6 s), and what a block
+// holds does not depend on how its tokens were split into calls but for those.
+// The maximum runs over the finite elements; an infinity is stored as +-448 s.
+//
+// A rotated key is the exact rotation x cos + rot(x) sin rounded once to
+// float32 (rope_exact): the largest value of a block is often a coordinate that
+// turns by less than a float32 ulp (low frequencies), and a value beside
+// 448 * 2^k decides about the scale.
+//
+// Work split.  A block's scale needs the maximum over all the call's rows of
+// the block, so one warp owns (block, KV head, keys or values).  It belongs to
+// the CTA of the block's leader: the token that writes the block's lowest slot
+// of the call.  Leaders are found in one of two ways:
+//   * up to kFp8ScanTokens tokens, each token's CTA reads every slot of the
+//     call and keeps the rows of its own block in shared memory: one launch;
+//   * more tokens: a first kernel stores writer[slot] = token, and a CTA reads
+//     its block's entries.  An entry is believed only if slot_mapping[entry]
+//     is that slot, so the array needs no initialisation and keeps nothing from
+//     one call to the next.
+// Each token's CTA also rotates the token's query rows.
+// Bound: memory for long chunks; for a decode step the latency of slots ->
+// rows -> maximum -> codes.
+#include "fp8_common.cuh"
+
+namespace mvb {
+
+struct Fp8WriteArgs {
+  const void* q;  // nullptr: no query rows
+  int64_t q_s0, q_s1;
+  void* q_out;
+  int64_t qo_s0, qo_s1;
+  const void* k;
+  int64_t k_s0, k_s1;
+  void* k_out;  // optional rotated keys [T, KH, D] contiguous
+  const void* v;
+  int64_t v_s0, v_s1;
+  const int64_t* pos;  // nullptr: no rotation
+  const void* cos;
+  const void* sin;
+  int64_t table_rows;
+  uint8_t* kc;
+  uint8_t* vc;
+  float* scale;  // [num_blocks, KH, 2]
+  const int64_t* slots;
+  int* writer;  // [num_blocks * block_size], or nullptr: scan
+  int num_tokens, num_heads, num_kv_heads, block_size, num_blocks;
+  int* err;
+};
+
+namespace {
+
+constexpr int kFp8ScanTokens = 1024;
+constexpr int kFp8WriteThreads = 256;
+
+// x c + y s (y the signed partner) rounded once to float32.  16-bit tables: the
+// product of two 16-bit floats is exact in float32, one fma rounds the sum.
+// float32 tables: the products and the sum with their rounding errors (exact by
+// fma and by Knuth's two-sum), added back at the end.
+template <typename TAB>
+__device__ __forceinline__ float rope_exact(float x, float c, float y, float s) {
+  if constexpr (sizeof(TAB) == 2) {
+    return __fmaf_rn(x, c, __fmul_rn(y, s));
+  } else {
+    const float p1 = __fmul_rn(x, c), e1 = __fmaf_rn(x, c, -p1);
+    const float p2 = __fmul_rn(y, s), e2 = __fmaf_rn(y, s, -p2);
+    const float t = __fadd_rn(p1, p2);
+    const float b = __fsub_rn(t, p1);
+    const float e3 = __fadd_rn(__fsub_rn(p1, __fsub_rn(t, b)), __fsub_rn(p2, b));
+    return __fadd_rn(t, __fadd_rn(e3, __fadd_rn(e1, e2)));
+  }
+}
+
+// 8 consecutive elements as floats (16-byte aligned for 16-bit types, 32 for float).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(e[i]);
+  } else {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  uint4 r;
+  T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<uint4*>(p) = r;
+}
+
+// Elements [d0, d0 + 8) and [d0 + D/2, d0 + D/2 + 8) of one row, rotated when ROT.
+template <typename T, typename TAB, int D, bool ROT>
+__device__ __forceinline__ void load_row(const T* row, const TAB* cs, const TAB* sn, int d0, float (&lo)[8],
+                                         float (&hi)[8]) {
+  load8<T>(row + d0, lo);
+  load8<T>(row + D / 2 + d0, hi);
+  if constexpr (ROT) {
+    float cl[8], ch[8], sl[8], sh[8];
+    load8<TAB>(cs + d0, cl);
+    load8<TAB>(cs + D / 2 + d0, ch);
+    load8<TAB>(sn + d0, sl);
+    load8<TAB>(sn + D / 2 + d0, sh);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = lo[i], b = hi[i];
+      lo[i] = rope_exact<TAB>(a, cl[i], -b, sl[i]);
+      hi[i] = rope_exact<TAB>(b, ch[i], a, sh[i]);
+    }
+  }
+}
+
+// The token's slot if the token is written at all, else -1.
+template <bool ROT>
+__device__ __forceinline__ int64_t live_slot(const Fp8WriteArgs& a, int64_t total_slots, int t) {
+  int64_t s = __ldg(a.slots + t);
+  if (s >= total_slots) s = -1;
+  if constexpr (ROT) {
+    const int64_t p = __ldg(a.pos + t);
+    if (p < 0 || p >= a.table_rows) s = -1;
+  }
+  return s < 0 ? -1 : s;
+}
+
+template <bool ROT>
+__global__ void __launch_bounds__(256) fp8_writer_kernel(const Fp8WriteArgs a) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.num_tokens) return;
+  const int64_t s = live_slot<ROT>(a, (int64_t)a.num_blocks * a.block_size, t);
+  if (s >= 0) a.writer[s] = t;
+}
+
+template <typename T, typename TAB, int D, bool ROT>
+__global__ void __launch_bounds__(kFp8WriteThreads) fp8_write_kernel(const Fp8WriteArgs a) {
+  extern __shared__ int map[];  // [block_size] the call's token at each slot of this block, -1: none
+  constexpr int LPR = D / 16, RPP = 32 / LPR, NWARP = kFp8WriteThreads / 32;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int KH = a.num_kv_heads, BS = a.block_size;
+  const int64_t total_slots = (int64_t)a.num_blocks * BS;
+  const int64_t slot = live_slot<ROT>(a, total_slots, t);
+  const int64_t b0 = slot & ~(int64_t)(BS - 1);  // first slot of the block (BS is a power of two)
+  const int off = (int)(slot - b0);
+  if (tid == 0) {
+    const int64_t raw = __ldg(a.slots + t);
+    int bad = raw < -1 || raw >= total_slots ? MVB_DEV_SLOT_RANGE : 0;
+    if constexpr (ROT) {
+      const int64_t p = __ldg(a.pos + t);
+      if (p < 0 || p >= a.table_rows) bad |= MVB_DEV_POSITION;
+    }
+    if (bad) atomicOr(a.err, bad);
+  }
+
+  // ---- is this token its block's leader, and which tokens write the block ----
+  bool leader = false;
+  if (slot >= 0) {  // the same for all threads of the CTA
+    bool other;     // some lower slot of the block is written, or this slot by another token
+    if (a.writer == nullptr) {
+      for (int i = tid; i < BS; i += kFp8WriteThreads) map[i] = -1;
+      __syncthreads();
+      for (int u = tid; u < a.num_tokens; u += kFp8WriteThreads) {
+        const int64_t s = live_slot<ROT>(a, total_slots, u);
+        // two tokens of one slot: the later one is written, and the call is flagged
+        if (s >= 0 && (s & ~(int64_t)(BS - 1)) == b0 && atomicMax(map + (s - b0), u) >= 0)
+          atomicOr(a.err, MVB_DEV_DUP_SLOT);
+      }
+      __syncthreads();
+      other = map[off] != t;
+      for (int i = tid; i < off; i += kFp8WriteThreads) other |= map[i] >= 0;
+      leader = __syncthreads_or(other) == 0;
+    } else {
+      // a chunk's next token: its left neighbour writes the slot before it
+      bool next = false;
+      if (off > 0 && t > 0) next = live_slot<ROT>(a, total_slots, t - 1) == slot - 1;
+      other = false;
+      if (tid == 0) {
+        const int w = __ldcg(a.writer + slot);
+        other = w != t;  // this slot's entry is some token's of this call: another one wrote it last
+        if (other) atomicOr(a.err, MVB_DEV_DUP_SLOT);
+      }
+      if (!next) {
+        for (int i = tid; i < BS; i += kFp8WriteThreads) {
+          const int w = __ldcg(a.writer + b0 + i);
+          const bool ok = w >= 0 && w < a.num_tokens && live_slot<ROT>(a, total_slots, w) == b0 + i;
+          map[i] = ok ? w : -1;
+          other |= ok && i < off;
+        }
+      }
+      leader = __syncthreads_or(other || next) == 0;
+    }
+  }
+
+  // ---- the block's rows: one warp per (KV head, keys / values) ----
+  const int kv_items = leader ? 2 * KH : 0;
+  for (int it = warp; it < kv_items; it += NWARP) {
+    const int kvh = it >> 1, which = it & 1;
+    const int64_t bh = (b0 / BS) * KH + kvh;
+    float* sp = a.scale + bh * 2 + which;
+    const float old = map[0] >= 0 ? 0.f : *sp;
+    const float base = old > 0.f && old < INFINITY ? old : 0.f;  // not a scale yet (or never): nothing to keep
+    uint8_t* codes = (which ? a.vc : a.kc) + bh * BS * D;
+    const T* src = static_cast<const T*>(which ? a.v : a.k);
+    const int64_t s0 = which ? a.v_s0 : a.k_s0;
+    src += (int64_t)kvh * (which ? a.v_s1 : a.k_s1);
+    const int d0 = (lane % LPR) * 8;
+    const TAB* cs = static_cast<const TAB*>(a.cos);
+    const TAB* sn = static_cast<const TAB*>(a.sin);
+    auto row = [&](int r, float (&lo)[8], float (&hi)[8]) {
+      const int u = map[r];
+      if (u < 0) return false;
+      const T* p = src + (int64_t)u * s0;
+      if (ROT && which == 0) {
+        const int64_t at = __ldg(a.pos + u) * D;
+        load_row<T, TAB, D, ROT>(p, cs + at, sn + at, d0, lo, hi);
+      } else {
+        load_row<T, TAB, D, false>(p, cs, sn, d0, lo, hi);
+      }
+      return true;
+    };
+    float amax = 0.f;
+    for (int r = lane / LPR; r < BS; r += RPP) {
+      float lo[8], hi[8];
+      if (!row(r, lo, hi)) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = fabsf(lo[i]), y = fabsf(hi[i]);
+        amax = fmaxf(amax, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float s = fmaxf(base, fp8_scale_for(amax));
+    if (base > 0.f && s > base) {  // the scale has grown: the rows already there, 16 codes a lane
+      const float ratio = __fdiv_rn(base, s);
+      for (int c = lane; c < BS * (D / 16); c += 32) {
+        if (map[c / (D / 16)] >= 0) continue;
+        uint4* p = reinterpret_cast<uint4*>(codes) + c;
+        uint4 w = *p;
+        uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t lo, hi;
+          e4m3x4_to_f16(e[i], lo, hi);
+          const float2 x = __half22float2(*reinterpret_cast<__half2*>(&lo));
+          const float2 y = __half22float2(*reinterpret_cast<__half2*>(&hi));
+          e[i] = f32x4_to_e4m3(x.x * ratio, x.y * ratio, y.x * ratio, y.y * ratio);
+        }
+        *p = w;
+      }
+    }
+    const float inv = __frcp_rn(s);
+    for (int r = lane / LPR; r < BS; r += RPP) {
+      float lo[8], hi[8];
+      if (!row(r, lo, hi)) continue;
+      uint2 l, h;
+      l.x = f32x4_to_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv);
+      l.y = f32x4_to_e4m3(lo[4] * inv, lo[5] * inv, lo[6] * inv, lo[7] * inv);
+      h.x = f32x4_to_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv);
+      h.y = f32x4_to_e4m3(hi[4] * inv, hi[5] * inv, hi[6] * inv, hi[7] * inv);
+      uint8_t* p = codes + (int64_t)r * D + d0;
+      *reinterpret_cast<uint2*>(p) = l;
+      *reinterpret_cast<uint2*>(p + D / 2) = h;
+    }
+    __syncwarp();
+    if (lane == 0) *sp = s;
+  }
+
+  // ---- this token's query rows, and its key rows where the caller wants them ----
+  if constexpr (ROT) {
+    const int64_t p = __ldg(a.pos + t);
+    if (p < 0 || p >= a.table_rows) return;
+    const TAB* cs = static_cast<const TAB*>(a.cos) + p * D;
+    const TAB* sn = static_cast<const TAB*>(a.sin) + p * D;
+    const int H = a.num_heads, rows = H + (a.k_out != nullptr ? KH : 0);
+    // warps take these from the last one down: the first ones may still be at the block's rows
+    for (int it = (NWARP - 1 - warp) * 32 + lane; it < rows * LPR; it += kFp8WriteThreads) {
+      const int r = it / LPR, d0 = (it - r * LPR) * 8;
+      const T* src = r < H ? static_cast<const T*>(a.q) + (int64_t)t * a.q_s0 + (int64_t)r * a.q_s1
+                           : static_cast<const T*>(a.k) + (int64_t)t * a.k_s0 + (int64_t)(r - H) * a.k_s1;
+      T* dst = r < H ? static_cast<T*>(a.q_out) + (int64_t)t * a.qo_s0 + (int64_t)r * a.qo_s1
+                     : static_cast<T*>(a.k_out) + ((int64_t)t * KH + (r - H)) * D;
+      float lo[8], hi[8];
+      load_row<T, TAB, D, true>(src, cs, sn, d0, lo, hi);
+      store8<T>(dst + d0, lo);
+      store8<T>(dst + D / 2 + d0, hi);
+    }
+  }
+}
+
+template <typename T, typename TAB, int D, bool ROT>
+int launch_write(const Fp8WriteArgs& a, cudaStream_t stream) {
+  auto kern = fp8_write_kernel<T, TAB, D, ROT>;
+  if (ensure_kernel_attrs(kern, a.block_size * 4) != cudaSuccess) return MVB_ERR_CUDA;
+  if (a.writer != nullptr) {
+    auto first = fp8_writer_kernel<ROT>;
+    if (ensure_kernel_attrs(first, 0) != cudaSuccess) return MVB_ERR_CUDA;
+    if (launch_pdl(first, dim3((a.num_tokens + 255) / 256), dim3(256), 0, stream, a) != cudaSuccess)
+      return MVB_ERR_CUDA;
+  }
+  return launch_pdl(kern, dim3(a.num_tokens), dim3(kFp8WriteThreads), a.block_size * 4, stream, a) == cudaSuccess
+             ? MVB_OK
+             : MVB_ERR_CUDA;
+}
+
+template <typename T>
+int launch_write_t(const Fp8WriteArgs& a, int head_dim, bool f32_tables, cudaStream_t stream) {
+  if (a.pos == nullptr)
+    return head_dim == 64 ? launch_write<T, T, 64, false>(a, stream) : launch_write<T, T, 128, false>(a, stream);
+  if (f32_tables)
+    return head_dim == 64 ? launch_write<T, float, 64, true>(a, stream) : launch_write<T, float, 128, true>(a, stream);
+  return head_dim == 64 ? launch_write<T, T, 64, true>(a, stream) : launch_write<T, T, 128, true>(a, stream);
+}
+
+int write_fp8(Fp8WriteArgs a, int head_dim, int dtype, int table_dtype, void* workspace, int64_t workspace_bytes,
+              void* stream) {
+  if (dtype != MVB_DTYPE_F16 && dtype != MVB_DTYPE_BF16) return MVB_ERR_DTYPE;
+  if (a.pos != nullptr && table_dtype != dtype && table_dtype != MVB_DTYPE_F32) return MVB_ERR_DTYPE;
+  if (head_dim != 64 && head_dim != 128) return MVB_ERR_HEAD_DIM;
+  if (a.block_size < kFp8MinBlock || a.block_size > kFp8MaxBlock || (a.block_size & (a.block_size - 1)) != 0)
+    return MVB_ERR_BLOCK_SIZE;
+  if (a.num_tokens < 0 || a.num_kv_heads <= 0 || a.num_blocks <= 0) return MVB_ERR_INVALID_ARG;
+  if (a.num_tokens == 0) return MVB_OK;
+  if (!a.k || !a.v || !a.kc || !a.vc || !a.scale || !a.slots || !a.err) return MVB_ERR_INVALID_ARG;
+  auto al = [](const void* p, int64_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  auto al_s = [](int64_t s) { return s % 8 == 0; };  // 16-byte vectors of 16-bit elements
+  if (!al(a.k, 16) || !al(a.v, 16) || !al(a.kc, 16) || !al(a.vc, 16) || !al(a.scale, 4) || !al_s(a.k_s0) ||
+      !al_s(a.k_s1) || !al_s(a.v_s0) || !al_s(a.v_s1) || !al(a.k_out, 16))
+    return MVB_ERR_ALIGNMENT;
+  if (a.pos != nullptr &&
+      (!al(a.q, 16) || !al(a.q_out, 16) || !al(a.cos, 16) || !al(a.sin, 16) || !al_s(a.q_s0) || !al_s(a.q_s1) ||
+       !al_s(a.qo_s0) || !al_s(a.qo_s1)))
+    return MVB_ERR_ALIGNMENT;
+  a.writer = nullptr;
+  if (a.num_tokens > kFp8ScanTokens) {
+    if (workspace == nullptr || workspace_bytes < (int64_t)a.num_blocks * a.block_size * 4 || !al(workspace, 4))
+      return MVB_ERR_WORKSPACE;
+    a.writer = static_cast<int*>(workspace);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f32_tables = table_dtype == MVB_DTYPE_F32;
+  return dtype == MVB_DTYPE_BF16 ? launch_write_t<__nv_bfloat16>(a, head_dim, f32_tables, s)
+                                 : launch_write_t<__half>(a, head_dim, f32_tables, s);
+}
+
+}  // namespace
+}  // namespace mvb
+
+using namespace mvb;
+
+extern "C" int mvb_kv_cache_write_fp8_workspace(int32_t num_tokens, int32_t num_blocks, int32_t block_size,
+                                                int64_t* bytes_out) {
+  if (num_tokens < 0 || num_blocks <= 0 || block_size <= 0 || !bytes_out) return MVB_ERR_INVALID_ARG;
+  *bytes_out = num_tokens <= kFp8ScanTokens ? 0 : (int64_t)num_blocks * block_size * 4;
+  return MVB_OK;
+}
+
+extern "C" int mvb_kv_cache_write_fp8(const void* key, int64_t k_stride_token, int64_t k_stride_head,
+                                      const void* value, int64_t v_stride_token, int64_t v_stride_head,
+                                      void* key_cache, void* value_cache, float* kv_scale,
+                                      const int64_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
+                                      int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t dtype,
+                                      void* workspace, int64_t workspace_bytes, int32_t* error_flags, void* stream) {
+  mvb::NvtxRange nvtx_range("mvb_kv_cache_write_fp8");
+  Fp8WriteArgs a = {};
+  a.k = key;
+  a.k_s0 = k_stride_token;
+  a.k_s1 = k_stride_head;
+  a.v = value;
+  a.v_s0 = v_stride_token;
+  a.v_s1 = v_stride_head;
+  a.kc = static_cast<uint8_t*>(key_cache);
+  a.vc = static_cast<uint8_t*>(value_cache);
+  a.scale = kv_scale;
+  a.slots = slot_mapping;
+  a.num_tokens = num_tokens;
+  a.num_kv_heads = num_kv_heads;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.err = error_flags;
+  return write_fp8(a, head_dim, dtype, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int mvb_rope_kv_cache_write_fp8(
+    const void* query, int64_t q_stride_token, int64_t q_stride_head, void* query_out, int64_t qo_stride_token,
+    int64_t qo_stride_head, const void* key, int64_t k_stride_token, int64_t k_stride_head, const void* value,
+    int64_t v_stride_token, int64_t v_stride_head, const int64_t* positions, const void* cos_table,
+    const void* sin_table, int64_t table_rows, int32_t table_dtype, void* key_cache, void* value_cache,
+    float* kv_scale, const int64_t* slot_mapping, void* key_out, int32_t num_tokens, int32_t num_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t dtype, void* workspace,
+    int64_t workspace_bytes, int32_t* error_flags, void* stream) {
+  mvb::NvtxRange nvtx_range("mvb_rope_kv_cache_write_fp8");
+  if (num_heads <= 0 || table_rows <= 0) return MVB_ERR_INVALID_ARG;
+  if (num_tokens > 0 && (!query || !query_out || !positions || !cos_table || !sin_table)) return MVB_ERR_INVALID_ARG;
+  Fp8WriteArgs a = {};
+  a.q = query;
+  a.q_s0 = q_stride_token;
+  a.q_s1 = q_stride_head;
+  a.q_out = query_out;
+  a.qo_s0 = qo_stride_token;
+  a.qo_s1 = qo_stride_head;
+  a.k = key;
+  a.k_s0 = k_stride_token;
+  a.k_s1 = k_stride_head;
+  a.k_out = key_out;
+  a.v = value;
+  a.v_s0 = v_stride_token;
+  a.v_s1 = v_stride_head;
+  a.pos = positions;
+  a.cos = cos_table;
+  a.sin = sin_table;
+  a.table_rows = table_rows;
+  a.kc = static_cast<uint8_t*>(key_cache);
+  a.vc = static_cast<uint8_t*>(value_cache);
+  a.scale = kv_scale;
+  a.slots = slot_mapping;
+  a.num_tokens = num_tokens;
+  a.num_heads = num_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.err = error_flags;
+  return write_fp8(a, head_dim, dtype, table_dtype, workspace, workspace_bytes, stream);
+}

@@ -200,6 +200,174 @@ std::tuple<int64_t, at::Tensor> decode(const at::Tensor& query, const at::Tensor
   return {st, out};
 }
 
+// ---- the 8-bit cache -------------------------------------------------------
+// Workspaces of these calls are allocated per call from torch's caching
+// allocator on the current stream: they need no initialisation, so calls on
+// several streams and captured graphs never share one.
+
+bool rows16(const at::Tensor& t) {  // 16-byte aligned rows of 16-bit elements, last dimension contiguous
+  return t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % 8 == 0 &&
+         t.stride(1) % 8 == 0;
+}
+
+bool fp8_cache(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& scale, int64_t block_size, int dev) {
+  return kc.dim() == 4 && kc.sizes() == vc.sizes() && kc.scalar_type() == at::kFloat8_e4m3fn &&
+         vc.scalar_type() == at::kFloat8_e4m3fn && kc.is_contiguous() && vc.is_contiguous() &&
+         kc.size(2) == block_size && scale.dim() == 3 && scale.size(0) == kc.size(0) &&
+         scale.size(1) == kc.size(1) && scale.size(2) == 2 && scale.scalar_type() == at::kFloat &&
+         scale.is_contiguous() && kc.get_device() == dev && vc.get_device() == dev && scale.get_device() == dev &&
+         kc.numel() > 0;
+}
+
+bool index64(const at::Tensor& t, int dev) {
+  return t.scalar_type() == at::kLong && t.get_device() == dev && t.is_contiguous();
+}
+
+at::Tensor scratch(int64_t bytes, int dev) {
+  return at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, dev));
+}
+
+// positions / cos / sin / query are undefined for the write without a rotation.
+std::tuple<int64_t, at::Tensor, at::Tensor> write_fp8(
+    const c10::optional<at::Tensor>& query_opt, const at::Tensor& key, const at::Tensor& value,
+    const c10::optional<at::Tensor>& pos_opt, const c10::optional<at::Tensor>& cos_opt,
+    const c10::optional<at::Tensor>& sin_opt, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& scale,
+    const at::Tensor& slots, int64_t block_size, const c10::optional<at::Tensor>& query_out_opt, bool return_key,
+    int64_t err_ptr) {
+  const at::Tensor none;
+  const bool rot = pos_opt.has_value();
+  const int dt = dtype_code(key.scalar_type());
+  if (!(key.is_cuda() && key.dim() == 3 && key.sizes() == value.sizes() && key.size(0) > 0 &&
+        (dt == MVB_DTYPE_BF16 || dt == MVB_DTYPE_F16) && value.scalar_type() == key.scalar_type()))
+    return {kSlowPath, none, none};
+  const int dev = key.get_device();
+  if (!(value.get_device() == dev && fp8_cache(kc, vc, scale, block_size, dev) && kc.size(1) == key.size(1) &&
+        kc.size(3) == key.size(2) && rows16(key) && rows16(value) && slots.dim() == 1 &&
+        slots.size(0) == key.size(0) && index64(slots, dev)))
+    return {kSlowPath, none, none};
+  const int64_t T = key.size(0), KH = key.size(1), D = key.size(2), NB = kc.size(0);
+  c10::cuda::CUDAGuard guard(dev);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  int64_t ws_bytes = 0;
+  int st = mvb_kv_cache_write_fp8_workspace((int32_t)T, (int32_t)NB, (int32_t)block_size, &ws_bytes);
+  if (st != MVB_OK) return {st, none, none};
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = scratch(ws_bytes, dev);
+  void* wp = ws_bytes > 0 ? ws.data_ptr() : nullptr;
+  int32_t* err = reinterpret_cast<int32_t*>(err_ptr);
+  float* sp = scale.data_ptr<float>();
+  if (!rot) {
+    st = mvb_kv_cache_write_fp8(key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+                                value.stride(1), kc.data_ptr(), vc.data_ptr(), sp, slots.data_ptr<int64_t>(),
+                                (int32_t)T, (int32_t)KH, (int32_t)D, (int32_t)block_size, (int32_t)NB, dt, wp,
+                                ws_bytes, err, stream);
+    return {st, none, none};
+  }
+  const at::Tensor &query = *query_opt, &pos = *pos_opt, &cos = *cos_opt, &sin = *sin_opt;
+  const int tdt = dtype_code(cos.scalar_type());
+  if (!(query.dim() == 3 && query.size(0) == T && query.size(2) == D && query.get_device() == dev &&
+        query.scalar_type() == key.scalar_type() && rows16(query) && pos.dim() == 1 && pos.size(0) == T &&
+        index64(pos, dev) && cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.size(1) == D &&
+        sin.scalar_type() == cos.scalar_type() && (tdt == dt || tdt == MVB_DTYPE_F32) && cos.is_contiguous() &&
+        sin.is_contiguous() && cos.get_device() == dev && sin.get_device() == dev &&
+        reinterpret_cast<uintptr_t>(cos.data_ptr()) % 16 == 0 &&
+        reinterpret_cast<uintptr_t>(sin.data_ptr()) % 16 == 0))
+    return {kSlowPath, none, none};
+  at::Tensor qo;
+  if (query_out_opt.has_value()) {
+    qo = *query_out_opt;
+    if (!(qo.sizes() == query.sizes() && qo.scalar_type() == query.scalar_type() && qo.get_device() == dev &&
+          rows16(qo)))
+      return {kSlowPath, none, none};
+  } else {
+    qo = at::empty(query.sizes(), query.options());
+  }
+  at::Tensor ko;
+  if (return_key) ko = at::empty(key.sizes(), key.options());
+  st = mvb_rope_kv_cache_write_fp8(
+      query.data_ptr(), query.stride(0), query.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1), key.data_ptr(),
+      key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), pos.data_ptr<int64_t>(),
+      cos.data_ptr(), sin.data_ptr(), cos.size(0), tdt, kc.data_ptr(), vc.data_ptr(), sp, slots.data_ptr<int64_t>(),
+      return_key ? ko.data_ptr() : nullptr, (int32_t)T, (int32_t)query.size(1), (int32_t)KH, (int32_t)D,
+      (int32_t)block_size, (int32_t)NB, dt, wp, ws_bytes, err, stream);
+  return {st, qo, ko};
+}
+
+std::tuple<int64_t, at::Tensor> decode_fp8(const at::Tensor& query, const at::Tensor& kc, const at::Tensor& vc,
+                                           const at::Tensor& scale, const at::Tensor& block_table,
+                                           const at::Tensor& kv_len, int64_t block_size, double softmax_scale,
+                                           const c10::optional<at::Tensor>& out_opt, int64_t err_ptr) {
+  const at::Tensor none;
+  if (!(query.is_cuda() && query.dim() == 3 && query.size(0) > 0)) return {kSlowPath, none};
+  const int dev = query.get_device(), dt = dtype_code(query.scalar_type());
+  if (!(fp8_cache(kc, vc, scale, block_size, dev) && kc.size(3) == query.size(2) &&
+        query.size(1) % kc.size(1) == 0 && rows16(query) && block_table.dim() == 2 &&
+        block_table.size(0) == query.size(0) && block_table.scalar_type() == at::kLong &&
+        block_table.get_device() == dev && block_table.stride(1) == 1 && kv_len.dim() == 1 &&
+        kv_len.size(0) == query.size(0) && kv_len.scalar_type() == at::kInt && kv_len.get_device() == dev &&
+        kv_len.is_contiguous()))
+    return {kSlowPath, none};
+  at::Tensor out;
+  if (out_opt.has_value()) {
+    out = *out_opt;
+    if (!(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type() && out.get_device() == dev &&
+          rows16(out)))
+      return {kSlowPath, none};
+  }
+  const int32_t nd = (int32_t)query.size(0), H = (int32_t)query.size(1), D = (int32_t)query.size(2),
+                KH = (int32_t)kc.size(1), NB = (int32_t)kc.size(0), BS = (int32_t)block_size,
+                maxb = (int32_t)block_table.size(1);
+  c10::cuda::CUDAGuard guard(dev);
+  int64_t ws_bytes = 0;
+  int st = mvb_paged_decode_fp8_workspace(nd, H, KH, D, BS, NB, maxb, dt, &ws_bytes);
+  if (st != MVB_OK) return {st, none};
+  if (!out.defined()) out = at::empty(query.sizes(), query.options());
+  at::Tensor ws = scratch(ws_bytes, dev);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  st = mvb_paged_decode_fp8(query.data_ptr(), query.stride(0), query.stride(1), kc.data_ptr(), vc.data_ptr(),
+                            scale.data_ptr<float>(), block_table.data_ptr<int64_t>(), block_table.stride(0), maxb,
+                            kv_len.data_ptr<int32_t>(), out.data_ptr(), out.stride(0), out.stride(1), nd, H, KH, D,
+                            BS, NB, (float)softmax_scale, dt, ws.data_ptr(), ws_bytes,
+                            reinterpret_cast<int32_t*>(err_ptr), stream);
+  return {st, out};
+}
+
+std::tuple<int64_t, at::Tensor> prefill_fp8(const at::Tensor& query, const at::Tensor& kc, const at::Tensor& vc,
+                                            const at::Tensor& scale, const at::Tensor& block_table,
+                                            const at::Tensor& seq_rows, const at::Tensor& cached_len,
+                                            const at::Tensor& query_len, int64_t block_size, double softmax_scale,
+                                            const c10::optional<at::Tensor>& out_opt, int64_t err_ptr) {
+  const at::Tensor none;
+  if (!(query.is_cuda() && query.dim() == 3 && query.size(0) > 0)) return {kSlowPath, none};
+  const int dev = query.get_device(), dt = dtype_code(query.scalar_type());
+  if (!(fp8_cache(kc, vc, scale, block_size, dev) && kc.size(3) == query.size(2) &&
+        query.size(1) % kc.size(1) == 0 && rows16(query) && block_table.dim() == 2 &&
+        block_table.scalar_type() == at::kLong && block_table.get_device() == dev && block_table.stride(1) == 1 &&
+        seq_rows.dim() == 1 && seq_rows.size(0) > 0 && cached_len.sizes() == seq_rows.sizes() &&
+        query_len.sizes() == seq_rows.sizes() && index64(seq_rows, dev) && index64(cached_len, dev) &&
+        index64(query_len, dev)))
+    return {kSlowPath, none};
+  at::Tensor out;
+  if (out_opt.has_value()) {
+    out = *out_opt;
+    if (!(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type() && out.get_device() == dev &&
+          rows16(out)))
+      return {kSlowPath, none};
+  } else {
+    out = at::empty(query.sizes(), query.options());
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  const int st = mvb_paged_prefill_fp8(
+      query.data_ptr(), query.stride(0), query.stride(1), kc.data_ptr(), vc.data_ptr(), scale.data_ptr<float>(),
+      block_table.data_ptr<int64_t>(), block_table.size(0), block_table.stride(0), (int32_t)block_table.size(1),
+      seq_rows.data_ptr<int64_t>(), cached_len.data_ptr<int64_t>(), query_len.data_ptr<int64_t>(),
+      (int32_t)seq_rows.size(0), (int32_t)query.size(0), out.data_ptr(), out.stride(0), out.stride(1),
+      (int32_t)query.size(1), (int32_t)kc.size(1), (int32_t)query.size(2), (int32_t)block_size, (int32_t)kc.size(0),
+      (float)softmax_scale, dt, reinterpret_cast<int32_t*>(err_ptr), stream);
+  return {st, out};
+}
+
 // Stream-ordered staging for a serving loop, one CUDA call each on raw handles
 // (a torch.cuda.Stream's cuda_stream, a torch.cuda.Event's cuda_event): the
 // torch-level copy_ / wait_event / record / set_stream calls cost about a
@@ -242,6 +410,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("SLOW_PATH") = kSlowPath;
   m.def("kv_write", &kv_write);
   m.def("decode", &decode);
+  m.def("write_fp8", &write_fp8);
+  m.def("decode_fp8", &decode_fp8);
+  m.def("prefill_fp8", &prefill_fp8);
   m.def("stream_copy", &stream_copy);
   m.def("stream_wait_events", &stream_wait_events);
   m.def("event_record", &event_record);
