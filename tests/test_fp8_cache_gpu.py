@@ -599,3 +599,32 @@ def test_backend_serves_from_an_8_bit_pool(dtype):
         backend.write_kv_cache(0, rows(1, KH).float(), rows(1, KH).float(), torch.zeros(1, dtype=torch.int64, device=DEV))
     pool.reset()
     assert all((s == 0).all() for s in pool.kv_scales)
+
+
+def test_prefill_nan_values_reach_only_the_rows_that_attend_them():
+    """NaN at some positions and columns of the values: NaN where a row attends them, nothing elsewhere."""
+    H, KH, D, bs, c, n = 14, 2, 64, 16, 40, 300
+    q, kc, vc, sc, table = prefill_case(6, [c], [n], (H, KH, D), bs, torch.bfloat16)
+    at = [(130, 0, 3), (131, 0, 63), (250, 1, 17), (339, 1, 0)]  # position, KV head, column
+    for p, h, d in at:
+        bits(vc)[table[0, p // bs], h, p % bs, d] = 0xFF
+    out = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, [0], [c], [n], bs)
+    want = torch.zeros(n, H, D, dtype=torch.bool, device=DEV)
+    for p, h, d in at:
+        want[max(0, p - c):, h * 7:(h + 1) * 7, d] = True
+        bits(vc)[table[0, p // bs], h, p % bs, d] = 0
+    assert torch.equal(torch.isnan(out), want)
+    k, v = F.dequant(kc, sc, 0, table[0], c + n), F.dequant(vc, sc, 1, table[0], c + n)
+    ref, tol = F.attend(q, k, v, c + 1, D ** -0.5)
+    F.check(torch.where(want, ref.to(q.dtype), out), ref, tol)
+
+
+def test_prefill_value_scales_that_grow():
+    """Value scales that rise by 2^9 from block to block, so that the accumulators' reference moves again and again."""
+    H, KH, D, bs, n = 8, 2, 128, 16, 700
+    q, kc, vc, sc, table = prefill_case(7, [0], [n], (H, KH, D), bs, torch.bfloat16)
+    for i in range(44):
+        sc[table[0, i], :, 1] *= 2.0 ** (-60 + 9 * (i // 8))
+    out = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, [0], [0], [n], bs)
+    # rows of the first 128 positions attend small values only, and are not lost beside what comes later
+    check_prefill(out, q, kc, vc, sc, table, [0], [n], bs)
