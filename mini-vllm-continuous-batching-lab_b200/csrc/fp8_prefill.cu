@@ -8,23 +8,28 @@
 // two tiles of 128 rows and walks the keys 128 at a time up to its last row's
 // limit:   S = Q K_codes^T,   P = exp2(S c_g - m),   O += P V.
 //
-// Roles (13 warps):
+// Roles (4 warpgroups; registers move from the last two to the softmax):
 //   * warps 0-3 and 4-7: the softmax of row tile 0 and 1, one row per thread.
-//     They read S from tensor memory twice (maximum, then exponentials), write
-//     P as f16 over it, and rescale O in tensor memory only when a row's
-//     maximum has risen by more than 8 (in powers of two; P <= 2^8 then);
-//   * warps 8-11: the loaders.  They read codes through the block table one
-//     tile ahead, turn them into f16 (exact) and store K and V tiles in the
-//     128-byte swizzled layout that the tensor core reads, 2 stages each;
+//     They hold a row of S in registers, write P as f16 to tensor memory (beside
+//     S for head_dim 64; over it for 128, where nothing is left), and rescale O
+//     there only when a row's maximum has risen by more than 8 (in powers of two;
+//     P <= 2^8 then);
+//   * warps 8-11: the loaders.  They copy codes through the block table one step
+//     ahead into shared memory (cp.async; block ids and scales are read four to
+//     eight steps ahead), turn them into f16 (exact) and store K and V tiles in
+//     the 128-byte swizzled layout that the tensor core reads, 2 stages each (K 1
+//     for head_dim 128, where shared memory ends).  Codes held in registers
+//     instead spilled, and the reloads made a step of head_dim 128 9900 cycles;
 //   * warp 12: issues the tensor-core products (tcgen05.mma, 128 x 128 and
-//     128 x D per tile): S of one row tile runs while the other is in its softmax.
+//     128 x D per tile): one row tile's run while the other is in its softmax.
 //
 // Scales.  A block's key scale is one factor of 16 columns of S (a group), so it
-// joins the softmax scale in the exponent's multiply-add at no cost.  Values
-// enter as code * 2^e, e the exponent of (the power of two in) the block's scale
-// over a reference R of the tile's largest; the product is exact in f16 for
-// scales from 2^-15 R to 2^7 R, and R (and O with it) moves when a scale passes
-// 2^7 R.  The rest of a scale that is no power of two multiplies P.
+// joins the softmax scale in the exponent's multiply-add at no cost.  A value
+// scale v joins the exponent too: P = p v / R, with the sum of p undone per
+// group, and O is in units of R, a power of two.  R is the first step's largest
+// scale and moves (O with it) when a scale passes 2^7 R.  The exponent takes v / R
+// down to 2^-4, where P's f16 still has 10 bits for p >= 2^-10; the rest of a
+// smaller scale goes into the f16 codes (exact to 2^-15 R).
 //
 // The query enters as f16, each row times a power of two that brings its
 // largest element into [1, 2) (as in the decode kernel, fp8_decode.cu).
@@ -70,27 +75,35 @@ constexpr int kTileRows = 128;               // rows of one row tile (tensor-cor
 constexpr int kCtaRows = 2 * kTileRows;      // (token, head) rows of one CTA
 constexpr int kKeys = 128;                   // keys per step
 constexpr int kGroups = kKeys / 16;          // 16-key groups: each lies in one block
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 512;
+// Registers of the warpgroups: 2 softmax, loaders, products; launched with 128 each.
+constexpr int kSoftmaxRegs = 200, kLoaderRegs = 64, kMmaRegs = 48;
+static_assert(2 * kSoftmaxRegs + kLoaderRegs + kMmaRegs <= 4 * 128, "a split of what the block was launched with");
+constexpr int kMinValueExp = -4;
 constexpr int kInfos = 4;                    // steps whose side information is kept
 constexpr int kTmemCols = 512;
 
 // Side information of one step, written by the loaders.
 struct StepInfo {
   float ks[kGroups];  // key scales
-  float vf[kGroups];  // value scale over its power of two, in [1, 2)
+  float ve[kGroups];  // log2 of the part of (value scale / R) that goes into P
+  float vu[kGroups];  // 2^-ve
   float r;            // reference R of the values (O is in units of it)
   float rf;           // the previous step's R over this one's
   int bad;            // bit g: the group's block id is invalid, its keys are left out
-  int nan[4];         // per loader warp: the step's values hold NaN
+  int nan[4];         // per loader warp: its keys' values hold NaN, and their masks are written
 };
 
 template <int D> struct Geo {
   static constexpr int QBYTES = kTileRows * D * 2, KBYTES = kKeys * D * 2;
   static constexpr int NMASK = kInfos * kKeys * (D / 16) * 2;  // a bit per (key, column)
-  static constexpr int Q = 0, K = 2 * QBYTES, V = K + 2 * KBYTES, MASK = V + 2 * KBYTES;
-  static constexpr int INFO = MASK + NMASK, BARS = INFO + kInfos * (int)sizeof(StepInfo);
+  static constexpr int KST = D == 64 ? 2 : 1;                  // stages of K
+  static constexpr int Q = 0, K = 2 * QBYTES, V = K + KST * KBYTES, RAW = V + 2 * KBYTES;  // RAW: codes of K, of V
+  static constexpr int MASK = RAW + KBYTES, INFO = MASK + NMASK, BARS = INFO + kInfos * (int)sizeof(StepInfo);
   static constexpr int BYTES = BARS + 128 + 1024;  // + alignment
-  static constexpr int S_COL = 0, O_COL = 256;     // tensor-memory columns: S 2 x 128, O 2 x D
+  // tensor-memory columns: S 2 x 128, O 2 x D, P 2 x 64
+  static constexpr bool P_APART = D == 64;
+  static constexpr int S_COL = 0, O_COL = 256, P_COL = P_APART ? 384 : 0, P_STEP = P_APART ? 64 : 128;
 };
 
 // Barriers (indices).
@@ -113,7 +126,7 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 32 consecutive columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -168,6 +181,22 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// A load that stays where it is issued, ahead of its use (a plain read-only load
+// is moved down to it by the compiler).
+__device__ __forceinline__ int64_t ld_ahead8(const void* p) {
+  int64_t r;
+  asm volatile("ld.global.nc.s64 %0, [%1];" : "=l"(r) : "l"(p));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -180,9 +209,6 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, __half2 f) {
 __device__ __forceinline__ uint32_t swz(int row, int panel, int c) {
   return (uint32_t)(panel * (kKeys * 128) + row * 128 + ((c ^ (row & 7)) << 4));
 }
-// The power of two in a positive scale (0 for 0 and for scales below 2^-126).
-__device__ __forceinline__ float pow2_of(float s) { return __uint_as_float(__float_as_uint(s) & 0x7f800000u); }
-
 // Waits of all roles: bounded, and given up when another role has given up.
 struct Waiter {
   uint32_t bars;
@@ -203,46 +229,6 @@ struct Waiter {
     return __all_sync(0xffffffffu, (*this)(i, parity)) != 0;
   }
 };
-
-// Columns [0, 32) of a chunk of S as P (f16 pairs), their sum added to l.
-// EDGE: the step holds keys that some row does not attend (lim: the row's keys in
-// this chunk; bad: bits of the chunk's two groups that are left out).
-template <bool EDGE>
-__device__ __forceinline__ float chunk_max(const uint32_t (&s)[32], float mx, const float* c, int lim, int bad) {
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = __uint_as_float(s[16 * g + i]);
-      if (EDGE && (16 * g + i >= lim || (bad >> g & 1))) v = -INFINITY;
-      x[i & 3] = fmaxf(x[i & 3], v);
-    }
-    mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * c[g]);
-  }
-  return mx;
-}
-template <bool EDGE>
-__device__ __forceinline__ void chunk_exp(const uint32_t (&s)[32], uint32_t (&p)[16], float m, const float* c,
-                                          const float* vf, int lim, int bad, float (&l)[2]) {
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    float e[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float y = fmaf(__uint_as_float(s[16 * g + i]), c[g], -m);
-      if (EDGE && (16 * g + i >= lim || (bad >> g & 1))) y = -INFINITY;
-      e[i] = fast_exp2(y);
-      l[i & 1] += e[i];
-    }
-    if (vf[g] != 1.f) {  // a value scale that is no power of two
-#pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] *= vf[g];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[8 * g + i] = pack_h2(e[2 * i], e[2 * i + 1]);
-  }
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8PrefillArgs a) {
@@ -369,11 +355,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   const uint32_t tmem = s_tmem;
 
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ================================ softmax =================================
     const int tile = warp >> 2, r = row0 + tile * kTileRows + (warp & 3) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + G_::S_COL + tile * kKeys, o_at = tmem + lanes + G_::O_COL + tile * D;
+      const uint32_t s_at = tmem + lanes + G_::S_COL + tile * kKeys, o_at = tmem + lanes + G_::O_COL + tile * D,
+                     p_at = tmem + lanes + G_::P_COL + tile * G_::P_STEP;
       const bool live = r < rows;
       const int tok = live ? r / a.G : 0, head = live ? r - tok * a.G : 0;
       const int lim = live ? (int)cached + tok + 1 : kv_end;  // rows past the chunk are zeros that attend all
@@ -422,9 +410,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         if (!(f.nan[0] | f.nan[1] | f.nan[2] | f.nan[3])) return;
         const int n = min(kKeys, lim - j * kKeys);
         for (int k = 0; k < n; ++k)
+          if (f.nan[k / (512 / D) & 3])  // the warp that loaded the key
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i)
-            nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kInfos) * kKeys + k) * (D / 16))[i];
+            for (int i = 0; i < D / 32; ++i)
+              nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kInfos) * kKeys + k) * (D / 16))[i];
       };
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
@@ -433,52 +422,80 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
           break;
         }
         tc_fence_after();
-        if (j > 0) take_nan(j - 1);  // (its products are done: S of this step was issued after them)
         const StepInfo& f = infos[j % kInfos];
+        uint32_t s[kKeys];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) tmem_ld32(s_at + 32 * h, s + 32 * h);
         const int rem = lim - j * kKeys, bad = f.bad;
-        const bool edge = __any_sync(0xffffffffu, rem < kKeys) || bad != 0;
-        float c[kGroups];
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) c[g] = qs * f.ks[g];
-        uint32_t s[32];
-        float mx = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          tmem_ld32(s_at + 32 * h, s);
-          tc_wait_ld();
-          mx = edge ? chunk_max<true>(s, mx, c + 2 * h, rem - 32 * h, bad >> (2 * h))
-                    : chunk_max<false>(s, mx, c + 2 * h, 0, 0);
-        }
-        const bool jump = mx > m + 8.f;
         const float rf = f.rf;
-        if (__any_sync(0xffffffffu, jump) || rf != 1.f) {
+        tc_wait_ld();
+        if (__any_sync(0xffffffffu, rem < kKeys) || bad != 0) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (i >= rem || (bad >> (i / 16) & 1)) s[i] = 0xff800000u;  // -inf
+        }
+        float c[kGroups], top[kGroups], mx = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          c[g] = fmaxf(qs * f.ks[g], 1.2e-38f);  // (not 0: -inf stays -inf)
+          top[g] = fmaxf(__uint_as_float(s[16 * g]), __uint_as_float(s[16 * g + 1]));
+        }
+#pragma unroll
+        for (int i = 2; i < 16; i += 2)
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g)
+            top[g] = fmaxf(fmaxf(top[g], __uint_as_float(s[16 * g + i])), __uint_as_float(s[16 * g + i + 1]));
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, top[g] * c[g]);
+        const bool jump = mx > m + 8.f;
+        const bool move = __any_sync(0xffffffffu, jump) || rf != 1.f;
+        float fac = rf;
+        if (move) {
           const float mn = jump ? mx : m, al = jump ? fast_exp2(m - mn) : 1.f;
           m = mn;
           l[0] *= al;
           l[1] *= al;
-          if (j > 0) {
-            const float fac = al * rf;
-#pragma unroll
-            for (int h = 0; h < D / 32; ++h) {
-              uint32_t o[32];
-              tmem_ld32(o_at + 32 * h, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fac);
-              tmem_st32(o_at + 32 * h, o);
-            }
+          fac *= al;
+        }
+        // the last step's products read P and added to O
+        if (j > 0) {
+          if (!wait.warp(kPvDone + tile, (j - 1) & 1)) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          take_nan(j - 1);
         }
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           uint32_t p[16];
-          tmem_ld32(s_at + 32 * h, s);
-          tc_wait_ld();
-          if (edge)
-            chunk_exp<true>(s, p, m, c + 2 * h, f.vf + 2 * h, rem - 32 * h, bad >> (2 * h), l);
-          else
-            chunk_exp<false>(s, p, m, c + 2 * h, f.vf + 2 * h, 0, 0, l);
-          tmem_st16(s_at + 16 * h, p);  // over columns of S that have been read
+#pragma unroll
+          for (int gg = 0; gg < 2; ++gg) {
+            const int g = 2 * h + gg;
+            // a row that has attended nothing yet: m and all of s are -inf, and P is 0
+            const float mm = m == -INFINITY ? 0.f : m - f.ve[g];
+            float e[16], t[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              e[i] = fast_exp2(fmaf(__uint_as_float(s[16 * g + i]), c[g], -mm));
+              t[i & 1] += e[i];
+            }
+            l[gg] = fmaf(t[0] + t[1], f.vu[g], l[gg]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[8 * gg + i] = pack_h2(e[2 * i], e[2 * i + 1]);
+          }
+          tmem_st16(p_at + 16 * h, p);
+        }
+        if (move && j > 0) {
+#pragma unroll
+          for (int h = 0; h < D / 32; ++h) {
+            uint32_t o[32];
+            tmem_ld32(o_at + 32 * h, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fac);
+            tmem_st32(o_at + 32 * h, o);
+          }
         }
         tc_wait_st();
         tc_fence_before();
@@ -512,169 +529,219 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       }
     }
   } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
     // ================================ loaders =================================
     constexpr int CH = D / 16, N = kKeys * CH / 128;  // 16-code chunks per row, chunks per thread and tile
     const int lt = tid - 256, lw = warp - 8;
     const int64_t* bt = a.bt + srow * a.bt_s0;
-    const int BSm = (1 << a.block_shift) - 1, grp = lane & (kGroups - 1);
-    // lane g (and g + 8, ..): where 16-key group g of a step lies: (block, KV head) row, -1 behind the last key or bad
-    auto find = [&](int j, bool& bad) {
-      const int p = j * kKeys + 16 * grp;
+    const int BSm = (1 << a.block_shift) - 1;
+    // Four steps at a time, one 16-key group per lane: where it lies ((block, KV
+    // head) row, -1 behind the last key or bad) and its block's scales.
+    auto find = [&](int j4, bool& bad) {
+      const int p = j4 * kKeys + 16 * lane;
       bad = false;
       if (p >= kv_end) return -1;
-      const int64_t b = __ldg(bt + (p >> a.block_shift));
+      const int64_t b = ld_ahead8(bt + (p >> a.block_shift));
       bad = b < 0 || b >= a.num_blocks;
       return bad ? -1 : (int)(b * a.num_kv_heads + kvh);
     };
-    uint4 kr[N], vr[N];
-    auto fetch = [&](uint4 (&d)[N], const uint8_t* base, int j, int row) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int key = lt / CH + i * (128 / CH), p = j * kKeys + key;
-        const int rw = __shfl_sync(0xffffffffu, row, key >> 4);
-        d[i] = make_uint4(0, 0, 0, 0);
-        if (rw >= 0 && p < kv_end)
-          d[i] = __ldg(reinterpret_cast<const uint4*>(base + (((int64_t)rw << a.block_shift) + (p & BSm)) * D) +
-                       lt % CH);
-      }
+    auto scales = [&](int row) {
+      const int64_t v = row >= 0 ? ld_ahead8(a.scale + row) : 0;
+      return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
     };
-    bool bad, bad_n = false;
-    int row = find(0, bad), row_n = -1;
-    float2 sc = row >= 0 ? __ldg(a.scale + row) : make_float2(0.f, 0.f);
-    fetch(kr, a.kc, 0, row);
-    fetch(vr, a.vc, 0, row);
-    if (steps > 1) row_n = find(1, bad_n);
-    float R = 1.f;
+    const int key0 = lt / CH, ch = lt % CH;
+    // This thread's chunk i of step j: key key0 + i * (128 / CH), codes [16 ch, 16 ch + 16).  It goes to a place of
+    // the thread's own (zeros behind the last key).
+    auto raw = [&](bool v, int i) { return smem + G_::RAW + (v ? G_::KBYTES / 2 : 0) + (i * 128 + lt) * 16; };
+    auto fetch = [&](bool v, int j, int rows4, int i) {
+      const int key = key0 + i * (128 / CH), p = j * kKeys + key;
+      const int rw = __shfl_sync(0xffffffffu, rows4, (j & 3) * kGroups + (key >> 4));
+      const bool ok = rw >= 0 && p < kv_end;
+      const int64_t at = ok ? (((int64_t)rw << a.block_shift) + (p & BSm)) * D + ch * 16 : 0;
+      cp_async_16(smem_u32(raw(v, i)), (v ? a.vc : a.kc) + at, ok ? 16 : 0);
+    };
+    auto store = [&](uint8_t* tile, int i, const uint32_t (&h)[8]) {
+      const int key = key0 + i * (128 / CH);
+      // (the second panel's lanes write their halves in the other order: both at once would meet in the same banks)
+      const bool swap = (ch / 4) & 1;
+      const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
+      *reinterpret_cast<uint4*>(tile + swz(key, ch / 4, 2 * (ch % 4) + swap)) = swap ? y : x;
+      *reinterpret_cast<uint4*>(tile + swz(key, ch / 4, 2 * (ch % 4) + !swap)) = swap ? x : y;
+    };
+    bool bad, bad_n;
+    int row = find(0, bad), row_n = find(4, bad_n);
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) fetch(false, 0, row, i);
+    cp_async_commit();
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) fetch(true, 0, row, i);
+    cp_async_commit();
+    float2 sc = scales(row), sc_n = make_float2(0.f, 0.f);
+    int top = 0;          // largest exponent field of the value scales of this lane's step
+    int RE = 127;         // exponent field of R
     for (int j = 0; j < steps; ++j) {
-      const int st = j & 1;
-      float2 sc_n = row_n >= 0 ? __ldg(a.scale + row_n) : make_float2(0.f, 0.f);
-      // the values' reference, and each group's factor
-      float vp = pow2_of(sc.y), top = vp;
+      const int st = j & 1, kst = j % G_::KST, q = (j & 3) * kGroups;
+      const int vexp = (int)(__float_as_uint(sc.y) >> 23) & 0xff;  // 0: a scale of 0 or below 2^-126
+      if ((j & 3) == 0) {
+        top = vexp;
 #pragma unroll
-      for (int o = 1; o < kGroups; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 1; o < kGroups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
+      const int step_top = __shfl_sync(0xffffffffu, top, q);
       float rf = 1.f;
-      if (j == 0)
-        R = top > 0.f ? top : 1.f;
-      else if (top > 128.f * R) {
-        rf = R / top;
-        R = top;
+      if (j == 0) {
+        RE = step_top > 0 ? step_top : 127;
+      } else if (step_top > RE + 7) {
+        rf = step_top - RE < 127 ? __uint_as_float((uint32_t)(127 + RE - step_top) << 23) : 0.f;
+        RE = step_top;
       }
-      const float vscale = vp / R;
+      const int e = vexp > 0 ? vexp - RE : 0, ep = max(e, kMinValueExp);
+      // what of the scale goes into the codes
+      const float rest = row >= 0 && vexp == 0 ? 0.f
+                         : e == ep             ? 1.f
+                         : e - ep > -127       ? __uint_as_float((uint32_t)(127 + e - ep) << 23)
+                                               : 0.f;
+      const float vf = vexp > 0 ? __uint_as_float(__float_as_uint(sc.y) & 0x7fffffu | 0x3f800000u) : 1.f;
+      const uint32_t in_step = ((1u << kGroups) - 1) << q;
+      const bool any_rest = (__ballot_sync(0xffffffffu, rest != 1.f) & in_step) != 0;
+      const uint32_t bads = __ballot_sync(0xffffffffu, bad) >> q & ((1u << kGroups) - 1);
       StepInfo& f = infos[j % kInfos];
-      const uint32_t badmask = __ballot_sync(0xffffffffu, bad) & ((1u << kGroups) - 1);
-      if (lw == 0) {
-        if (lane < kGroups) {
-          f.ks[lane] = sc.x;
-          f.vf[lane] = vp > 0.f ? sc.y / vp : 1.f;
-        }
-        if (lane == 0) {
-          f.r = R;
+      if (lw == 0 && lane >= q && lane < q + kGroups) {
+        const int g = lane - q;
+        f.ks[g] = sc.x;
+        f.ve[g] = (float)ep + (vf == 1.f ? 0.f : log2f(vf));
+        f.vu[g] = __uint_as_float((uint32_t)(127 - ep) << 23) / vf;
+        if (g == 0) {
+          f.r = __uint_as_float((uint32_t)RE << 23);
           f.rf = rf;
-          f.bad = (int)badmask;
-          if (badmask) atomicOr(a.err, MVB_DEV_BLOCK_ID);
+          f.bad = (int)bads;
+          if (bads) atomicOr(a.err, MVB_DEV_BLOCK_ID);
         }
       }
-      if (j >= 2 && !wait.warp(kKEmpty + st, (j / 2 - 1) & 1)) break;
-      uint8_t* kd = smem + G_::K + st * G_::KBYTES;
-#pragma unroll
+      if (j >= G_::KST && !wait.warp(kKEmpty + kst, (j / G_::KST - 1) & 1)) break;
+      cp_async_wait<1>();  // this step's K (its V may be on the way)
+      const int rows_next = ((j + 1) & 3) == 0 ? row_n : row;
+#pragma unroll 2
       for (int i = 0; i < N; ++i) {
-        const int key = lt / CH + i * (128 / CH), ch = lt % CH;
-        uint4 w0, w1;
-        e4m3x4_to_f16(kr[i].x, w0.x, w0.y);
-        e4m3x4_to_f16(kr[i].y, w0.z, w0.w);
-        e4m3x4_to_f16(kr[i].z, w1.x, w1.y);
-        e4m3x4_to_f16(kr[i].w, w1.z, w1.w);
-        *reinterpret_cast<uint4*>(kd + swz(key, ch / 4, 2 * (ch % 4))) = w0;
-        *reinterpret_cast<uint4*>(kd + swz(key, ch / 4, 2 * (ch % 4) + 1)) = w1;
+        uint32_t h[8];
+        const uint4 x = *reinterpret_cast<const uint4*>(raw(false, i));
+        e4m3x4_to_f16(x.x, h[0], h[1]);
+        e4m3x4_to_f16(x.y, h[2], h[3]);
+        e4m3x4_to_f16(x.z, h[4], h[5]);
+        e4m3x4_to_f16(x.w, h[6], h[7]);
+        store(smem + G_::K + kst * G_::KBYTES, i, h);
+        fetch(false, j + 1, rows_next, i);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(wait.bar(kKFull + st));
-      if (j + 1 < steps) fetch(kr, a.kc, j + 1, row_n);
+      cp_async_commit();
+      __syncwarp();  // (the products' thread makes the stores visible to the tensor core)
+      if (lane == 0) mbar_arrive(wait.bar(kKFull + kst));
 
       if (j >= 2 && !wait.warp(kVEmpty + st, (j / 2 - 1) & 1)) break;
-      uint8_t* vd = smem + G_::V + st * G_::KBYTES;
-      bool any_nan = false;
-#pragma unroll
+      cp_async_wait<1>();  // this step's V (the next one's K may be on the way)
+      // bytes 0x7f and 0xff are NaN: they are taken out of the values and noted in the masks
+      uint32_t seen = 0;
+#pragma unroll 2
       for (int i = 0; i < N; ++i) {
-        const int key = lt / CH + i * (128 / CH), ch = lt % CH;
-        uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, nan16 = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bytes 0x7f and 0xff: NaN
-          if (n) {
+        const uint4 x = *reinterpret_cast<const uint4*>(raw(true, i));
+        seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
+                ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+      }
+      const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
+      if (any_nan) {
+        for (int i = 0; i < N; ++i) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(raw(true, i));
+          uint32_t nan16 = 0;
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
             w[k] &= ~((n >> 7) * 0xffu);
             nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
           }
+          masks[((j % kInfos) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
         }
-        any_nan |= nan16 != 0;
-        masks[((j % kInfos) * kKeys + key) * CH + ch] = (uint16_t)nan16;
-        const __half2 vs = __float2half2_rn(__shfl_sync(0xffffffffu, vscale, key >> 4));
-        uint32_t h[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          e4m3x4_to_f16(w[k], h[2 * k], h[2 * k + 1]);
-          h[2 * k] = mul_h2(h[2 * k], vs);
-          h[2 * k + 1] = mul_h2(h[2 * k + 1], vs);
-        }
-        *reinterpret_cast<uint4*>(vd + swz(key, ch / 4, 2 * (ch % 4))) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(vd + swz(key, ch / 4, 2 * (ch % 4) + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
-      any_nan = __any_sync(0xffffffffu, any_nan);
       if (lane == 0) f.nan[lw] = any_nan;
-      fence_proxy_async_smem();
+#pragma unroll 2
+      for (int i = 0; i < N; ++i) {
+        uint32_t h[8];
+        const uint4 x = *reinterpret_cast<const uint4*>(raw(true, i));
+        e4m3x4_to_f16(x.x, h[0], h[1]);
+        e4m3x4_to_f16(x.y, h[2], h[3]);
+        e4m3x4_to_f16(x.z, h[4], h[5]);
+        e4m3x4_to_f16(x.w, h[6], h[7]);
+        if (any_rest) {
+          const __half2 r2 = __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
+#pragma unroll
+          for (int k = 0; k < 8; ++k) h[k] = mul_h2(h[k], r2);
+        }
+        store(smem + G_::V + st * G_::KBYTES, i, h);
+        fetch(true, j + 1, rows_next, i);
+      }
+      cp_async_commit();
       __syncwarp();
       if (lane == 0) mbar_arrive(wait.bar(kVFull + st));
-      if (j + 1 < steps) fetch(vr, a.vc, j + 1, row_n);
-      row = row_n;
-      bad = bad_n;
-      sc = sc_n;
-      row_n = -1;
-      bad_n = false;
-      if (j + 2 < steps) row_n = find(j + 2, bad_n);
+      if ((j & 3) == 1) sc_n = scales(row_n);
+      if ((j & 3) == 3) {
+        row = row_n;
+        bad = bad_n;
+        sc = sc_n;
+        row_n = find(j + 5, bad_n);
+      }
     }
-  } else if (lane == 0) {
+    cp_async_wait<0>();  // nothing lands after the CTA has left
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    if (warp == 12 && lane == 0) {
     // ========================= tensor-core products ===========================
     const uint32_t base = smem_u32(smem);
     constexpr uint32_t SW = mma_word(kKeys, false), PW = mma_word(D, true);
-    auto scores = [&](int i, int st) {  // S_i = Q_i K^T: 16 columns (32 bytes of a panel's row) a step
+    auto scores = [&](int i, int kst) {  // S_i = Q_i K^T: 16 columns (32 bytes of a panel's row) a step
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const uint32_t off = (uint32_t)((k / 4) * (kKeys * 128) + (k % 4) * 32);
         mma_ss(tmem + G_::S_COL + i * kKeys, smem_desc(base + G_::Q + i * G_::QBYTES + off, 16, 1024),
-               smem_desc(base + G_::K + st * G_::KBYTES + off, 16, 1024), SW, k > 0);
+               smem_desc(base + G_::K + kst * G_::KBYTES + off, 16, 1024), SW, k > 0);
       }
       tc_commit(wait.bar(kSFull + i));
     };
     auto values = [&](int i, int st, bool add) {  // O_i += P_i V: 16 keys (2 KB of a panel) a step
 #pragma unroll
       for (int k = 0; k < kKeys / 16; ++k)
-        mma_ts(tmem + G_::O_COL + i * D, tmem + G_::S_COL + i * kKeys + 8 * k,
+        mma_ts(tmem + G_::O_COL + i * D, tmem + G_::P_COL + i * G_::P_STEP + 8 * k,
                smem_desc(base + G_::V + st * G_::KBYTES + k * 2048, kKeys * 128, 1024), PW, add || k > 0);
       tc_commit(wait.bar(kPvDone + i));
     };
     bool ok = wait(kQ, 0) && wait(kKFull, 0);
     if (ok) {
+      fence_proxy_async_smem();
       tc_fence_after();
       for (int i = 0; i < tiles; ++i) scores(i, 0);
       tc_commit(wait.bar(kKEmpty));
     }
+    auto ready = [&](int i, int parity) {
+      if (!wait(i, parity)) return false;
+      fence_proxy_async_smem();  // tiles were stored through the generic proxy
+      tc_fence_after();
+      return true;
+    };
     for (int j = 0; ok && j < steps; ++j) {
-      const int st = j & 1, sn = st ^ 1;
+      const int st = j & 1, kn = (j + 1) % G_::KST;
+      const bool next = j + 1 < steps;
+      auto next_scores = [&](int i) {
+        if (i == 0 && !ready(kKFull + kn, ((j + 1) / G_::KST) & 1)) return false;
+        scores(i, kn);
+        if (i == tiles - 1) tc_commit(wait.bar(kKEmpty + kn));
+        return true;
+      };
       for (int i = 0; ok && i < tiles; ++i) {
-        ok = (i > 0 || wait(kVFull + st, (j / 2) & 1)) && wait(kPReady + i, j & 1);
+        ok = ready(kPReady + i, j & 1);
+        // P apart: S has been read, and the next step's softmax need not wait for P V
+        if (ok && G_::P_APART && next) ok = next_scores(i);
+        if (ok && i == 0) ok = ready(kVFull + st, (j / 2) & 1);
         if (!ok) break;
-        tc_fence_after();
         values(i, st, j > 0);
         if (i == tiles - 1) tc_commit(wait.bar(kVEmpty + st));
-        if (j + 1 < steps) {
-          // S of the next step overwrites P: the products that read it come first
-          ok = (i > 0 || wait(kKFull + sn, ((j + 1) / 2) & 1)) && wait(kPvDone + i, j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          scores(i, sn);
-          if (i == tiles - 1) tc_commit(wait.bar(kKEmpty + sn));
-        }
+        // P over S: the products that read it come before S of the next step
+        if (!G_::P_APART && next) ok = ready(kPvDone + i, j & 1) && next_scores(i);
       }
     }
     if (!ok) {
@@ -684,6 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       fence_mbar_init();
       tc_commit(wait.bar(kNumBars));
       mbar_wait_bounded(wait.bar(kNumBars), 0);
+    }
     }
   }
   __syncwarp();
@@ -696,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
 template <typename T, int D>
 int launch_prefill_fp8(const Fp8PrefillArgs& a, cudaStream_t stream) {
   auto kern = fp8_prefill_kernel<T, D>;
-  static_assert(2 * (kFp8PrefillMaxChunks + 1) * 4 <= 4 * Geo<D>::KBYTES, "the prefixes fit the stages");
+  static_assert(2 * (kFp8PrefillMaxChunks + 1) * 4 <= 3 * Geo<D>::KBYTES, "the prefixes fit the stages");
   static_assert(Geo<D>::BYTES <= 227 * 1024 - 512, "shared memory of one CTA");
   if (ensure_kernel_attrs(kern, Geo<D>::BYTES) != cudaSuccess) return MVB_ERR_CUDA;
   const int64_t tiles = ((int64_t)a.total_q * a.G + kCtaRows - 1) / kCtaRows + a.n;
