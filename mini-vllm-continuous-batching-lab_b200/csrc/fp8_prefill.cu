@@ -77,10 +77,11 @@ constexpr int kKeys = 128;                   // keys per step
 constexpr int kGroups = kKeys / 16;          // 16-key groups: each lies in one block
 constexpr int kThreads = 512;
 // Registers of the warpgroups: 2 softmax, loaders, products; launched with 128 each.
-constexpr int kSoftmaxRegs = 200, kLoaderRegs = 64, kMmaRegs = 48;
+constexpr int kSoftmaxRegs = 192, kLoaderRegs = 80, kMmaRegs = 48;
 static_assert(2 * kSoftmaxRegs + kLoaderRegs + kMmaRegs <= 4 * 128, "a split of what the block was launched with");
 constexpr int kMinValueExp = -4;
-constexpr int kInfos = 4;                    // steps whose side information is kept
+constexpr int kInfos = 8;                    // steps whose side information is kept (two batches of four)
+constexpr int kMasks = 4;                    // steps whose NaN masks are kept
 constexpr int kTmemCols = 512;
 
 // Side information of one step, written by the loaders.
@@ -96,7 +97,7 @@ struct StepInfo {
 
 template <int D> struct Geo {
   static constexpr int QBYTES = kTileRows * D * 2, KBYTES = kKeys * D * 2;
-  static constexpr int NMASK = kInfos * kKeys * (D / 16) * 2;  // a bit per (key, column)
+  static constexpr int NMASK = kMasks * kKeys * (D / 16) * 2;  // a bit per (key, column)
   static constexpr int KST = D == 64 ? 2 : 1;                  // stages of K
   static constexpr int Q = 0, K = 2 * QBYTES, V = K + KST * KBYTES, RAW = V + 2 * KBYTES;  // RAW: codes of K, of V
   static constexpr int MASK = RAW + KBYTES, INFO = MASK + NMASK, BARS = INFO + kInfos * (int)sizeof(StepInfo);
@@ -122,8 +123,11 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void tc_commit(uint32_t bar, int lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead)
+      : "memory");
 }
 // 32 consecutive columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
@@ -167,18 +171,28 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint
 constexpr uint32_t mma_word(int n, bool b_mn_major) {
   return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(kTileRows / 16) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t word, bool add) {
+// The products' warp stays together and one lane (`lead`) issues: operands that
+// are the same for the whole warp are in uniform registers then, where the
+// instruction wants them.  (Issued from a branch of one lane, every operand is
+// moved there first, and four products take 660 cycles to issue.)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t word, bool add, int lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(word), "r"((int)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(word),
+      "r"((int)add), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t word, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t word, bool add, int lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(word),
-      "r"((int)add)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(word),
+      "r"((int)add), "r"(lead)
       : "memory");
+}
+__device__ __forceinline__ int elect_one() {
+  int r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, int bytes) {
@@ -333,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   wait.stop = &s_stop;
   wait.err = a.err;
   StepInfo* infos = reinterpret_cast<StepInfo*>(smem + G_::INFO);
-  uint16_t* masks = reinterpret_cast<uint16_t*>(smem + G_::MASK);  // [kInfos][kKeys][D / 16]
+  uint16_t* masks = reinterpret_cast<uint16_t*>(smem + G_::MASK);  // [kMasks][kKeys][D / 16]
   if (warp == 12) tmem_alloc(smem_u32(&s_tmem));
   if (tid == 0) {
     s_stop = 0;
@@ -413,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
           if (f.nan[k / (512 / D) & 3])  // the warp that loaded the key
 #pragma unroll
             for (int i = 0; i < D / 32; ++i)
-              nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kInfos) * kKeys + k) * (D / 16))[i];
+              nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kMasks) * kKeys + k) * (D / 16))[i];
       };
       bool ok = true;
       for (int j = 0; j < steps; ++j) {
@@ -532,226 +546,245 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
     // ================================ loaders =================================
     constexpr int CH = D / 16, N = kKeys * CH / 128;  // 16-code chunks per row, chunks per thread and tile
-    const int lt = tid - 256, lw = warp - 8;
+    constexpr uint32_t NONE = 0xffffffffu;
+    const int lw = warp - 8;
     const int64_t* bt = a.bt + srow * a.bt_s0;
-    const int BSm = (1 << a.block_shift) - 1;
-    // Four steps at a time, one 16-key group per lane: where it lies ((block, KV
-    // head) row, -1 behind the last key or bad) and its block's scales.
+    const int BSm = (1 << a.block_shift) - 1, gshift = a.block_shift - 4;
+    // Four steps at a time, one 16-key group per lane: its number among the cache's groups (NONE behind the last
+    // key or for a bad block id), and its block's scales.
     auto find = [&](int j4, bool& bad) {
       const int p = j4 * kKeys + 16 * lane;
       bad = false;
-      if (p >= kv_end) return -1;
+      if (p >= kv_end) return NONE;
       const int64_t b = ld_ahead8(bt + (p >> a.block_shift));
       bad = b < 0 || b >= a.num_blocks;
-      return bad ? -1 : (int)(b * a.num_kv_heads + kvh);
+      return bad ? NONE : ((uint32_t)(b * a.num_kv_heads + kvh) << gshift) + ((uint32_t)(p & BSm) >> 4);
     };
-    auto scales = [&](int row) {
-      const int64_t v = row >= 0 ? ld_ahead8(a.scale + row) : 0;
+    auto scales = [&](uint32_t group) {
+      const int64_t v = group != NONE ? ld_ahead8(a.scale + (group >> gshift)) : 0;
       return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
     };
-    const int key0 = lt / CH, ch = lt % CH;
-    // This thread's chunk i of step j: key key0 + i * (128 / CH), codes [16 ch, 16 ch + 16).  It goes to a place of
-    // the thread's own (zeros behind the last key).
-    auto raw = [&](bool v, int i) { return smem + G_::RAW + (v ? G_::KBYTES / 2 : 0) + (i * 128 + lt) * 16; };
-    auto fetch = [&](bool v, int j, int rows4, int i) {
-      const int key = key0 + i * (128 / CH), p = j * kKeys + key;
-      const int rw = __shfl_sync(0xffffffffu, rows4, (j & 3) * kGroups + (key >> 4));
-      const bool ok = rw >= 0 && p < kv_end;
-      const int64_t at = ok ? (((int64_t)rw << a.block_shift) + (p & BSm)) * D + ch * 16 : 0;
-      cp_async_16(smem_u32(raw(v, i)), (v ? a.vc : a.kc) + at, ok ? 16 : 0);
-    };
-    auto store = [&](uint8_t* tile, int i, const uint32_t (&h)[8]) {
-      const int key = key0 + i * (128 / CH);
-      // (the second panel's lanes write their halves in the other order: both at once would meet in the same banks)
-      const bool swap = (ch / 4) & 1;
-      const uint4 x = make_uint4(h[0], h[1], h[2], h[3]), y = make_uint4(h[4], h[5], h[6], h[7]);
-      *reinterpret_cast<uint4*>(tile + swz(key, ch / 4, 2 * (ch % 4) + swap)) = swap ? y : x;
-      *reinterpret_cast<uint4*>(tile + swz(key, ch / 4, 2 * (ch % 4) + !swap)) = swap ? x : y;
-    };
-    bool bad, bad_n;
-    int row = find(0, bad), row_n = find(4, bad_n);
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) fetch(false, 0, row, i);
-    cp_async_commit();
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) fetch(true, 0, row, i);
-    cp_async_commit();
-    float2 sc = scales(row), sc_n = make_float2(0.f, 0.f);
-    int top = 0;          // largest exponent field of the value scales of this lane's step
-    int RE = 127;         // exponent field of R
-    for (int j = 0; j < steps; ++j) {
-      const int st = j & 1, kst = j % G_::KST, q = (j & 3) * kGroups;
-      const int vexp = (int)(__float_as_uint(sc.y) >> 23) & 0xff;  // 0: a scale of 0 or below 2^-126
-      if ((j & 3) == 0) {
-        top = vexp;
+    // This thread's chunk i of a step: key key0 + i * (128 / CH), codes [16 ch, 16 ch + 16).  Eight lanes hold the
+    // chunks of one panel of two keys, whose swizzled places are in different banks.
+    const int ch = CH == 4 ? lane & 3 : (lane & 3) | (lane >> 1 & 4);
+    const int key0 = CH == 4 ? lw * 8 + (lane >> 2) : lw * 4 + ((lane >> 2 & 1) | (lane >> 3 & 2));
+    uint8_t* const raw = smem + G_::RAW + (lw * 32 + lane) * 16;  // its codes of K, then V: + 2048 i
+    const uint32_t to0 = swz(key0, ch / 4, 2 * (ch % 4)), to1 = to0 ^ 16;  // its places in a tile: + i * STEP
+    constexpr uint32_t STEP = (128 / CH) * 128;
+    const uint32_t from = (uint32_t)((key0 & 15) * D + ch * 16);
+    auto fetch = [&](bool v, int j, uint32_t groups) {
+      const uint8_t* base = (v ? a.vc : a.kc) + from;
+      const uint32_t dst = smem_u32(raw) + (v ? G_::KBYTES / 2 : 0);
+      const bool tail = (j + 1) * kKeys > kv_end;
 #pragma unroll
-        for (int o = 1; o < kGroups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      }
-      const int step_top = __shfl_sync(0xffffffffu, top, q);
-      float rf = 1.f;
-      if (j == 0) {
-        RE = step_top > 0 ? step_top : 127;
-      } else if (step_top > RE + 7) {
-        rf = step_top - RE < 127 ? __uint_as_float((uint32_t)(127 + RE - step_top) << 23) : 0.f;
-        RE = step_top;
-      }
-      const int e = vexp > 0 ? vexp - RE : 0, ep = max(e, kMinValueExp);
-      // what of the scale goes into the codes
-      const float rest = row >= 0 && vexp == 0 ? 0.f
-                         : e == ep             ? 1.f
-                         : e - ep > -127       ? __uint_as_float((uint32_t)(127 + e - ep) << 23)
-                                               : 0.f;
-      const float vf = vexp > 0 ? __uint_as_float(__float_as_uint(sc.y) & 0x7fffffu | 0x3f800000u) : 1.f;
-      const uint32_t in_step = ((1u << kGroups) - 1) << q;
-      const bool any_rest = (__ballot_sync(0xffffffffu, rest != 1.f) & in_step) != 0;
-      const uint32_t bads = __ballot_sync(0xffffffffu, bad) >> q & ((1u << kGroups) - 1);
-      StepInfo& f = infos[j % kInfos];
-      if (lw == 0 && lane >= q && lane < q + kGroups) {
-        const int g = lane - q;
-        f.ks[g] = sc.x;
-        f.ve[g] = (float)ep + (vf == 1.f ? 0.f : log2f(vf));
-        f.vu[g] = __uint_as_float((uint32_t)(127 - ep) << 23) / vf;
-        if (g == 0) {
-          f.r = __uint_as_float((uint32_t)RE << 23);
-          f.rf = rf;
-          f.bad = (int)bads;
-          if (bads) atomicOr(a.err, MVB_DEV_BLOCK_ID);
-        }
-      }
-      if (j >= G_::KST && !wait.warp(kKEmpty + kst, (j / G_::KST - 1) & 1)) break;
-      cp_async_wait<1>();  // this step's K (its V may be on the way)
-      const int rows_next = ((j + 1) & 3) == 0 ? row_n : row;
-#pragma unroll 2
       for (int i = 0; i < N; ++i) {
-        uint32_t h[8];
-        const uint4 x = *reinterpret_cast<const uint4*>(raw(false, i));
-        e4m3x4_to_f16(x.x, h[0], h[1]);
-        e4m3x4_to_f16(x.y, h[2], h[3]);
-        e4m3x4_to_f16(x.z, h[4], h[5]);
-        e4m3x4_to_f16(x.w, h[6], h[7]);
-        store(smem + G_::K + kst * G_::KBYTES, i, h);
-        fetch(false, j + 1, rows_next, i);
+        const int key = key0 + i * (128 / CH);
+        const uint32_t grp = __shfl_sync(0xffffffffu, groups, (j & 3) * kGroups + (key >> 4));
+        const bool ok = grp != NONE && !(tail && j * kKeys + key >= kv_end);
+        cp_async_16(dst + 2048 * i, base + (ok ? (uint64_t)grp * (16 * D) : 0), ok ? 16 : 0);
       }
       cp_async_commit();
+    };
+    bool bad, bad_n;
+    uint32_t grp = find(0, bad), grp_n = find(4, bad_n);
+    fetch(false, 0, grp);
+    fetch(true, 0, grp);
+    float2 sc = scales(grp), sc_n = make_float2(0.f, 0.f);
+    int RE = 127;                                // exponent field of R
+    uint32_t rests = 0;                          // lanes whose group's value scale goes into the codes in part
+    float rest = 1.f;
+    for (int j = 0; j < steps; ++j) {
+      const int st = j & 1, kst = j % G_::KST, q = (j & 3) * kGroups;
+      if (q == 0) {  // side information of four steps
+        const int vexp = (int)(__float_as_uint(sc.y) >> 23) & 0xff;  // 0: a scale of 0 or below 2^-126
+        int top = vexp, mine = 0;  // largest exponent field of the step; R's of this lane's step
+        float rf = 1.f;
+#pragma unroll
+        for (int o = 1; o < kGroups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int t = __shfl_sync(0xffffffffu, top, k * kGroups);
+          const int was = RE;
+          if (j + k == 0)
+            RE = t > 0 ? t : 127;
+          else if (t > RE + 7)
+            RE = t;
+          if (lane >> 3 == k) {
+            mine = RE;
+            if (j + k > 0 && RE != was) rf = RE - was < 127 ? __uint_as_float((uint32_t)(127 + was - RE) << 23) : 0.f;
+          }
+        }
+        const int e = vexp > 0 ? vexp - mine : 0, ep = max(e, kMinValueExp);
+        rest = grp != NONE && vexp == 0 ? 0.f
+               : e == ep                ? 1.f
+               : e - ep > -127          ? __uint_as_float((uint32_t)(127 + e - ep) << 23)
+                                        : 0.f;
+        rests = __ballot_sync(0xffffffffu, rest != 1.f);
+        const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+        if (lw == 0) {
+          const float vf = vexp > 0 ? __uint_as_float((__float_as_uint(sc.y) & 0x7fffffu) | 0x3f800000u) : 1.f;
+          StepInfo& f = infos[(j + (lane >> 3)) % kInfos];
+          const int g = lane & (kGroups - 1);
+          f.ks[g] = sc.x;
+          f.ve[g] = (float)ep + (vf == 1.f ? 0.f : log2f(vf));
+          f.vu[g] = __uint_as_float((uint32_t)(127 - ep) << 23) / vf;
+          if (g == 0) {
+            f.r = __uint_as_float((uint32_t)mine << 23);
+            f.rf = rf;
+            f.bad = (int)(bads >> (lane & ~7) & ((1u << kGroups) - 1));
+          }
+          if (lane == 0 && bads) atomicOr(a.err, MVB_DEV_BLOCK_ID);
+        }
+        __syncwarp();
+      }
+      const uint32_t groups_next = ((j + 1) & 3) == 0 ? grp_n : grp;
+      if (j >= G_::KST && !wait.warp(kKEmpty + kst, (j / G_::KST - 1) & 1)) break;
+      cp_async_wait<1>();  // this step's K (its V may be on the way)
+      {
+        uint8_t* tile = smem + G_::K + kst * G_::KBYTES;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+          uint4 lo4, hi4;
+          e4m3x4_to_f16(x.x, lo4.x, lo4.y);
+          e4m3x4_to_f16(x.y, lo4.z, lo4.w);
+          e4m3x4_to_f16(x.z, hi4.x, hi4.y);
+          e4m3x4_to_f16(x.w, hi4.z, hi4.w);
+          *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
+          *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
+        }
+      }
       __syncwarp();  // (the products' thread makes the stores visible to the tensor core)
       if (lane == 0) mbar_arrive(wait.bar(kKFull + kst));
+      fetch(false, j + 1, groups_next);  // nothing behind the last key
 
       if (j >= 2 && !wait.warp(kVEmpty + st, (j / 2 - 1) & 1)) break;
       cp_async_wait<1>();  // this step's V (the next one's K may be on the way)
-      // bytes 0x7f and 0xff are NaN: they are taken out of the values and noted in the masks
-      uint32_t seen = 0;
-#pragma unroll 2
-      for (int i = 0; i < N; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(raw(true, i));
-        seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
-                ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
-      }
-      const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
-      if (any_nan) {
-        for (int i = 0; i < N; ++i) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(raw(true, i));
-          uint32_t nan16 = 0;
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-            w[k] &= ~((n >> 7) * 0xffu);
-            nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
+      {
+        uint8_t* tile = smem + G_::V + st * G_::KBYTES;
+        const uint8_t* from_v = raw + G_::KBYTES / 2;
+        uint32_t seen = 0;
+        auto store = [&](uint4 x, int i) {
+          uint4 lo4, hi4;
+          e4m3x4_to_f16(x.x, lo4.x, lo4.y);
+          e4m3x4_to_f16(x.y, lo4.z, lo4.w);
+          e4m3x4_to_f16(x.z, hi4.x, hi4.y);
+          e4m3x4_to_f16(x.w, hi4.z, hi4.w);
+          if (rests >> q & ((1u << kGroups) - 1)) {
+            const __half2 r2 =
+                __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
+            lo4 = make_uint4(mul_h2(lo4.x, r2), mul_h2(lo4.y, r2), mul_h2(lo4.z, r2), mul_h2(lo4.w, r2));
+            hi4 = make_uint4(mul_h2(hi4.x, r2), mul_h2(hi4.y, r2), mul_h2(hi4.z, r2), mul_h2(hi4.w, r2));
           }
-          masks[((j % kInfos) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
-        }
-      }
-      if (lane == 0) f.nan[lw] = any_nan;
-#pragma unroll 2
-      for (int i = 0; i < N; ++i) {
-        uint32_t h[8];
-        const uint4 x = *reinterpret_cast<const uint4*>(raw(true, i));
-        e4m3x4_to_f16(x.x, h[0], h[1]);
-        e4m3x4_to_f16(x.y, h[2], h[3]);
-        e4m3x4_to_f16(x.z, h[4], h[5]);
-        e4m3x4_to_f16(x.w, h[6], h[7]);
-        if (any_rest) {
-          const __half2 r2 = __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
+          *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
+          *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
+        };
 #pragma unroll
-          for (int k = 0; k < 8; ++k) h[k] = mul_h2(h[k], r2);
+        for (int i = 0; i < N; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(from_v + 2048 * i);
+          // a byte 0x7f or 0xff is NaN: its low seven bits and one more reach the eighth
+          seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
+                  ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+          store(x, i);
         }
-        store(smem + G_::V + st * G_::KBYTES, i, h);
-        fetch(true, j + 1, rows_next, i);
+        const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
+        if (any_nan) {  // once more with zeros in their place, and the masks
+#pragma unroll 1
+          for (int i = 0; i < N; ++i) {
+            uint4 x = *reinterpret_cast<const uint4*>(from_v + 2048 * i);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+            uint32_t nan16 = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              w[k] &= ~((n >> 7) * 0xffu);
+              nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
+            }
+            masks[((j % kMasks) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
+            store(x, i);
+          }
+        }
+        if (lane == 0) infos[j % kInfos].nan[lw] = any_nan;
       }
-      cp_async_commit();
       __syncwarp();
       if (lane == 0) mbar_arrive(wait.bar(kVFull + st));
-      if ((j & 3) == 1) sc_n = scales(row_n);
+      fetch(true, j + 1, groups_next);
+      if ((j & 3) == 1) sc_n = scales(grp_n);
       if ((j & 3) == 3) {
-        row = row_n;
+        grp = grp_n;
         bad = bad_n;
         sc = sc_n;
-        row_n = find(j + 5, bad_n);
+        grp_n = find(j + 5, bad_n);
       }
     }
     cp_async_wait<0>();  // nothing lands after the CTA has left
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp == 12 && lane == 0) {
-    // ========================= tensor-core products ===========================
-    const uint32_t base = smem_u32(smem);
-    constexpr uint32_t SW = mma_word(kKeys, false), PW = mma_word(D, true);
-    auto scores = [&](int i, int kst) {  // S_i = Q_i K^T: 16 columns (32 bytes of a panel's row) a step
+    if (warp == 12) {
+      // ========================= tensor-core products ===========================
+      const uint32_t base = smem_u32(smem);
+      const int lead = elect_one();
+      constexpr uint32_t SW = mma_word(kKeys, false), PW = mma_word(D, true);
+      auto scores = [&](int i, int kst) {  // S_i = Q_i K^T: 16 columns (32 bytes of a panel's row) a step
+        const uint64_t qd = smem_desc(base + G_::Q + i * G_::QBYTES, 16, 1024);
+        const uint64_t kd = smem_desc(base + G_::K + kst * G_::KBYTES, 16, 1024);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (uint32_t)((k / 4) * (kKeys * 128) + (k % 4) * 32);
-        mma_ss(tmem + G_::S_COL + i * kKeys, smem_desc(base + G_::Q + i * G_::QBYTES + off, 16, 1024),
-               smem_desc(base + G_::K + kst * G_::KBYTES + off, 16, 1024), SW, k > 0);
-      }
-      tc_commit(wait.bar(kSFull + i));
-    };
-    auto values = [&](int i, int st, bool add) {  // O_i += P_i V: 16 keys (2 KB of a panel) a step
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (uint32_t)((k / 4) * (kKeys * 128) + (k % 4) * 32) >> 4;
+          mma_ss(tmem + G_::S_COL + i * kKeys, qd + off, kd + off, SW, k > 0, lead);
+        }
+        tc_commit(wait.bar(kSFull + i), lead);
+      };
+      auto values = [&](int i, int st, bool add) {  // O_i += P_i V: 16 keys (2 KB of a panel) a step
+        const uint64_t vd = smem_desc(base + G_::V + st * G_::KBYTES, kKeys * 128, 1024);
 #pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k)
-        mma_ts(tmem + G_::O_COL + i * D, tmem + G_::P_COL + i * G_::P_STEP + 8 * k,
-               smem_desc(base + G_::V + st * G_::KBYTES + k * 2048, kKeys * 128, 1024), PW, add || k > 0);
-      tc_commit(wait.bar(kPvDone + i));
-    };
-    bool ok = wait(kQ, 0) && wait(kKFull, 0);
-    if (ok) {
-      fence_proxy_async_smem();
-      tc_fence_after();
-      for (int i = 0; i < tiles; ++i) scores(i, 0);
-      tc_commit(wait.bar(kKEmpty));
-    }
-    auto ready = [&](int i, int parity) {
-      if (!wait(i, parity)) return false;
-      fence_proxy_async_smem();  // tiles were stored through the generic proxy
-      tc_fence_after();
-      return true;
-    };
-    for (int j = 0; ok && j < steps; ++j) {
-      const int st = j & 1, kn = (j + 1) % G_::KST;
-      const bool next = j + 1 < steps;
-      auto next_scores = [&](int i) {
-        if (i == 0 && !ready(kKFull + kn, ((j + 1) / G_::KST) & 1)) return false;
-        scores(i, kn);
-        if (i == tiles - 1) tc_commit(wait.bar(kKEmpty + kn));
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_ts(tmem + G_::O_COL + i * D, tmem + G_::P_COL + i * G_::P_STEP + 8 * k, vd + (k * 2048 >> 4), PW,
+                 add || k > 0, lead);
+        tc_commit(wait.bar(kPvDone + i), lead);
+      };
+      auto ready = [&](int i, int parity) {
+        if (!wait.warp(i, parity)) return false;
+        fence_proxy_async_smem();  // tiles were stored through the generic proxy
+        tc_fence_after();
         return true;
       };
-      for (int i = 0; ok && i < tiles; ++i) {
-        ok = ready(kPReady + i, j & 1);
-        // P apart: S has been read, and the next step's softmax need not wait for P V
-        if (ok && G_::P_APART && next) ok = next_scores(i);
-        if (ok && i == 0) ok = ready(kVFull + st, (j / 2) & 1);
-        if (!ok) break;
-        values(i, st, j > 0);
-        if (i == tiles - 1) tc_commit(wait.bar(kVEmpty + st));
-        // P over S: the products that read it come before S of the next step
-        if (!G_::P_APART && next) ok = ready(kPvDone + i, j & 1) && next_scores(i);
+      bool ok = ready(kQ, 0) && ready(kKFull, 0);
+      if (ok) {
+        for (int i = 0; i < tiles; ++i) scores(i, 0);
+        tc_commit(wait.bar(kKEmpty), lead);
       }
-    }
-    if (!ok) {
-      // given up: wait for whatever was issued before the tensor memory goes (the last commit's barrier has
-      // one arrival per phase, so its phase is unknown here: use one that nothing else waits on any more)
-      mbar_init(wait.bar(kNumBars), 1);
-      fence_mbar_init();
-      tc_commit(wait.bar(kNumBars));
-      mbar_wait_bounded(wait.bar(kNumBars), 0);
-    }
+      for (int j = 0; ok && j < steps; ++j) {
+        const int st = j & 1, kn = (j + 1) % G_::KST;
+        const bool next = j + 1 < steps;
+        auto next_scores = [&](int i) {
+          if (i == 0 && !ready(kKFull + kn, ((j + 1) / G_::KST) & 1)) return false;
+          scores(i, kn);
+          if (i == tiles - 1) tc_commit(wait.bar(kKEmpty + kn), lead);
+          return true;
+        };
+        for (int i = 0; ok && i < tiles; ++i) {
+          ok = ready(kPReady + i, j & 1);
+          // P apart: S has been read, and the next step's softmax need not wait for P V
+          if (ok && G_::P_APART && next) ok = next_scores(i);
+          if (ok && i == 0) ok = ready(kVFull + st, (j / 2) & 1);
+          if (!ok) break;
+          values(i, st, j > 0);
+          if (i == tiles - 1) tc_commit(wait.bar(kVEmpty + st), lead);
+          // P over S: the products that read it come before S of the next step
+          if (!G_::P_APART && next) ok = ready(kPvDone + i, j & 1) && next_scores(i);
+        }
+      }
+      if (!ok) {
+        // given up: wait for whatever was issued before the tensor memory goes (on a barrier that nothing else uses)
+        if (lead) {
+          mbar_init(wait.bar(kNumBars), 1);
+          fence_mbar_init();
+        }
+        __syncwarp();
+        tc_commit(wait.bar(kNumBars), lead);
+        mbar_wait_bounded(wait.bar(kNumBars), 0);
+      }
     }
   }
   __syncwarp();
@@ -798,9 +831,10 @@ extern "C" int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, in
     return MVB_ERR_INVALID_ARG;
   if (num_heads % num_kv_heads != 0) return MVB_ERR_HEADS;
   const int G = num_heads / num_kv_heads;
-  // rows of a KV head, positions of a sequence and (block, KV head) numbers are 32-bit
+  // rows of a KV head, positions of a sequence, (block, KV head) and 16-token group numbers are 32-bit
   if ((int64_t)total_q * G >= ((int64_t)1 << 30) || (int64_t)max_blocks_per_seq * block_size >= ((int64_t)1 << 30) ||
-      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31))
+      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31) ||
+      (int64_t)num_blocks * num_kv_heads * (block_size / 16) >= 0xffffffffll)
     return MVB_ERR_INVALID_ARG;
   if (num_chunks == 0 || total_q == 0) return MVB_OK;
   if (!query || !key_cache || !value_cache || !kv_scale || !block_table || !seq_rows || !cached_len || !query_len ||
