@@ -8,19 +8,19 @@
 // two tiles of 128 rows and walks the keys 128 at a time up to its last row's
 // limit:   S = Q K_codes^T,   P = exp2(S c_g - m),   O += P V.
 //
-// Roles (4 warpgroups; registers move from the last two to the softmax):
+// Roles (5 warpgroups; registers move from the last three to the softmax):
 //   * warps 0-3 and 4-7: the softmax of row tile 0 and 1, one row per thread.
-//     They hold a row of S in registers, write P as f16 to tensor memory (beside
-//     S for head_dim 64; over it for 128, where nothing is left), and rescale O
-//     there only when a row's maximum has risen by more than 8 (in powers of two;
-//     P <= 2^8 then);
-//   * warps 8-11: the loaders.  They copy codes through the block table one step
-//     ahead into shared memory (cp.async; block ids and scales are read four to
-//     eight steps ahead), turn them into f16 (exact) and store K and V tiles in
-//     the 128-byte swizzled layout that the tensor core reads, 2 stages each (K 1
-//     for head_dim 128, where shared memory ends).  Codes held in registers
-//     instead spilled, and the reloads made a step of head_dim 128 9900 cycles;
-//   * warp 12: issues the tensor-core products (tcgen05.mma, 128 x 128 and
+//     They read S in halves of 64 columns (the first half twice: a whole row in
+//     registers leaves none for the loaders), write P as f16 to tensor memory
+//     (beside S for head_dim 64; over its second half for 128, where nothing is
+//     left), and rescale O there only when a row's maximum has risen by more
+//     than 8 (in powers of two; P <= 2^8 then);
+//   * warps 8-11 and 12-15: the loaders of K and of V.  They copy codes through
+//     the block table one step ahead into shared memory (cp.async; block ids and
+//     scales are read four to eight steps ahead), turn them into f16 (exact) and
+//     store tiles in the 128-byte swizzled layout that the tensor core reads, 2
+//     stages each (K 1 for head_dim 128, where shared memory ends);
+//   * warp 16: issues the tensor-core products (tcgen05.mma, 128 x 128 and
 //     128 x D per tile): one row tile's run while the other is in its softmax.
 //
 // Scales.  A block's key scale is one factor of 16 columns of S (a group), so it
@@ -44,6 +44,8 @@
 // Every wait is bounded (kWaitSpinLimit); one that runs out sets
 // MVB_DEV_TIMEOUT, tells the other roles to leave, and the CTA waits (bounded)
 // for its products in flight before it frees its tensor memory.
+#include <type_traits>
+
 #include "fp8_common.cuh"
 
 namespace mvb {
@@ -75,10 +77,10 @@ constexpr int kTileRows = 128;               // rows of one row tile (tensor-cor
 constexpr int kCtaRows = 2 * kTileRows;      // (token, head) rows of one CTA
 constexpr int kKeys = 128;                   // keys per step
 constexpr int kGroups = kKeys / 16;          // 16-key groups: each lies in one block
-constexpr int kThreads = 512;
-// Registers of the warpgroups: 2 softmax, loaders, products; launched with 128 each.
-constexpr int kSoftmaxRegs = 192, kLoaderRegs = 80, kMmaRegs = 48;
-static_assert(2 * kSoftmaxRegs + kLoaderRegs + kMmaRegs <= 4 * 128, "a split of what the block was launched with");
+constexpr int kThreads = 640;
+// Registers of the warpgroups: 2 softmax, 2 loaders, products; launched with 96 each.
+constexpr int kSoftmaxRegs = 136, kLoaderRegs = 80, kMmaRegs = 48;
+static_assert(2 * kSoftmaxRegs + 2 * kLoaderRegs + kMmaRegs <= 5 * 96, "a split of what the block was launched with");
 constexpr int kMinValueExp = -4;
 constexpr int kInfos = 8;                    // steps whose side information is kept (two batches of four)
 constexpr int kMasks = 4;                    // steps whose NaN masks are kept
@@ -104,7 +106,7 @@ template <int D> struct Geo {
   static constexpr int BYTES = BARS + 128 + 1024;  // + alignment
   // tensor-memory columns: S 2 x 128, O 2 x D, P 2 x 64
   static constexpr bool P_APART = D == 64;
-  static constexpr int S_COL = 0, O_COL = 256, P_COL = P_APART ? 384 : 0, P_STEP = P_APART ? 64 : 128;
+  static constexpr int S_COL = 0, O_COL = 256, P_COL = P_APART ? 384 : 64, P_STEP = P_APART ? 64 : 128;
 };
 
 // Barriers (indices).
@@ -208,6 +210,24 @@ __device__ __forceinline__ void cp_async_wait() {
 __device__ __forceinline__ int64_t ld_ahead8(const void* p) {
   int64_t r;
   asm volatile("ld.global.nc.s64 %0, [%1];" : "=l"(r) : "l"(p));
+  return r;
+}
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
 
@@ -348,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   wait.err = a.err;
   StepInfo* infos = reinterpret_cast<StepInfo*>(smem + G_::INFO);
   uint16_t* masks = reinterpret_cast<uint16_t*>(smem + G_::MASK);  // [kMasks][kKeys][D / 16]
-  if (warp == 12) tmem_alloc(smem_u32(&s_tmem));
+  if (warp == 16) tmem_alloc(smem_u32(&s_tmem));
   if (tid == 0) {
     s_stop = 0;
     mbar_init(wait.bar(kQ), 4 * tiles);
@@ -415,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         __syncwarp();
         if (lane == 0) mbar_arrive(wait.bar(kQ));
       }
-      float m = -INFINITY, l[2] = {0.f, 0.f};
+      float m = -INFINITY, l = 0.f;
       uint32_t nanbits[D / 32];
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) nanbits[i] = 0u;
@@ -429,76 +449,83 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
             for (int i = 0; i < D / 32; ++i)
               nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kMasks) * kKeys + k) * (D / 16))[i];
       };
-      bool ok = true;
-      for (int j = 0; j < steps; ++j) {
-        if (!wait.warp(kSFull + tile, j & 1)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      // One step of the softmax; EDGE: it holds keys that some row does not attend.
+      auto step = [&](int j, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
         const StepInfo& f = infos[j % kInfos];
-        uint32_t s[kKeys];
+        uint32_t s[64];
+        const int rem = lim - j * kKeys;
+        auto read_half = [&](int h) {  // 64 columns of S, -inf where the row does not attend the key
+          tmem_ld32(s_at + 64 * h, s);
+          tmem_ld32(s_at + 64 * h + 32, s + 32);
+          tc_wait_ld();
+          if constexpr (EDGE) {
+            const int bad = f.bad >> (4 * h), n = rem - 64 * h;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) tmem_ld32(s_at + 32 * h, s + 32 * h);
-        const int rem = lim - j * kKeys, bad = f.bad;
-        const float rf = f.rf;
-        tc_wait_ld();
-        if (__any_sync(0xffffffffu, rem < kKeys) || bad != 0) {
+            for (int i = 0; i < 64; ++i)
+              if (i >= n || (bad >> (i / 16) & 1)) s[i] = 0xff800000u;
+          }
+        };
+        auto col = [&](int i) { return __uint_as_float(s[i]); };
+        float c[kGroups], mx = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (i >= rem || (bad >> (i / 16) & 1)) s[i] = 0xff800000u;  // -inf
+        for (int h = 0; h < 2; ++h) {
+          read_half(h);
+          float top[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            c[4 * h + g] = fmaxf(qs * f.ks[4 * h + g], 1.2e-38f);  // (not 0: -inf stays -inf)
+            top[g] = fmaxf(col(16 * g), col(16 * g + 1));
+          }
+#pragma unroll
+          for (int i = 2; i < 16; i += 2)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) top[g] = fmaxf(fmaxf(top[g], col(16 * g + i)), col(16 * g + i + 1));
+#pragma unroll
+          for (int g = 0; g < 4; ++g) mx = fmaxf(mx, top[g] * c[4 * h + g]);
         }
-        float c[kGroups], top[kGroups], mx = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          c[g] = fmaxf(qs * f.ks[g], 1.2e-38f);  // (not 0: -inf stays -inf)
-          top[g] = fmaxf(__uint_as_float(s[16 * g]), __uint_as_float(s[16 * g + 1]));
-        }
-#pragma unroll
-        for (int i = 2; i < 16; i += 2)
-#pragma unroll
-          for (int g = 0; g < kGroups; ++g)
-            top[g] = fmaxf(fmaxf(top[g], __uint_as_float(s[16 * g + i])), __uint_as_float(s[16 * g + i + 1]));
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, top[g] * c[g]);
         const bool jump = mx > m + 8.f;
+        const float rf = f.rf;
         const bool move = __any_sync(0xffffffffu, jump) || rf != 1.f;
         float fac = rf;
         if (move) {
           const float mn = jump ? mx : m, al = jump ? fast_exp2(m - mn) : 1.f;
           m = mn;
-          l[0] *= al;
-          l[1] *= al;
+          l *= al;
           fac *= al;
         }
         // the last step's products read P and added to O
         if (j > 0) {
-          if (!wait.warp(kPvDone + tile, (j - 1) & 1)) {
-            ok = false;
-            break;
-          }
+          if (!wait.warp(kPvDone + tile, (j - 1) & 1)) return false;
           tc_fence_after();
           take_nan(j - 1);
         }
+        // a row that has attended nothing yet: m and all of s are -inf, and P is 0
+        const float base = EDGE && m == -INFINITY ? 0.f : -m;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t p[16];
+        for (int half = 1; half >= 0; --half) {  // the second half is at hand; P may lie over it
+          if (half == 0) read_half(0);
 #pragma unroll
-          for (int gg = 0; gg < 2; ++gg) {
-            const int g = 2 * h + gg;
-            // a row that has attended nothing yet: m and all of s are -inf, and P is 0
-            const float mm = m == -INFINITY ? 0.f : m - f.ve[g];
-            float e[16], t[2] = {0.f, 0.f};
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              e[i] = fast_exp2(fmaf(__uint_as_float(s[16 * g + i]), c[g], -mm));
-              t[i & 1] += e[i];
+            for (int gg = 0; gg < 2; ++gg) {
+              const int g = 4 * half + 2 * h + gg;
+              const float2 cc = make_float2(c[g], c[g]), mm = make_float2(base + f.ve[g], base + f.ve[g]);
+              float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const int k = 32 * h + 16 * gg + i;
+                float2 e = fma2(make_float2(col(k), col(k + 1)), cc, mm);
+                e.x = fast_exp2(e.x);
+                e.y = fast_exp2(e.y);
+                t = add2(t, e);
+                p[8 * gg + i / 2] = pack_h2(e.x, e.y);
+              }
+              l = fmaf(t.x + t.y, f.vu[g], l);
             }
-            l[gg] = fmaf(t[0] + t[1], f.vu[g], l[gg]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[8 * gg + i] = pack_h2(e[2 * i], e[2 * i + 1]);
+            tmem_st16(p_at + 32 * half + 16 * h, p);
           }
-          tmem_st16(p_at + 16 * h, p);
         }
         if (move && j > 0) {
 #pragma unroll
@@ -515,12 +542,22 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(wait.bar(kPReady + tile));
+        return true;
+      };
+      bool ok = true;
+      for (int j = 0; ok && j < steps; ++j) {
+        ok = wait.warp(kSFull + tile, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, lim - j * kKeys < kKeys) || infos[j % kInfos].bad != 0)
+          ok = step(j, std::true_type());
+        else
+          ok = step(j, std::false_type());
       }
       if (ok && wait.warp(kPvDone + tile, (steps - 1) & 1)) {
         tc_fence_after();
         take_nan(steps - 1);
-        const float sum = l[0] + l[1];
-        const float inv = sum == 0.f ? 0.f : infos[(steps - 1) % kInfos].r / sum;
+        const float inv = l == 0.f ? 0.f : infos[(steps - 1) % kInfos].r / l;
         T* op = out + (int64_t)(q0 + tok) * a.o_s0 + (int64_t)(h0 + head) * a.o_s1;
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
@@ -542,12 +579,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         }
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
     // ================================ loaders =================================
     constexpr int CH = D / 16, N = kKeys * CH / 128;  // 16-code chunks per row, chunks per thread and tile
     constexpr uint32_t NONE = 0xffffffffu;
-    const int lw = warp - 8;
+    const bool is_v = warp >= 12;
+    const int lw = warp & 3;
     const int64_t* bt = a.bt + srow * a.bt_s0;
     const int BSm = (1 << a.block_shift) - 1, gshift = a.block_shift - 4;
     // Four steps at a time, one 16-key group per lane: its number among the cache's groups (NONE behind the last
@@ -568,27 +606,25 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     // chunks of one panel of two keys, whose swizzled places are in different banks.
     const int ch = CH == 4 ? lane & 3 : (lane & 3) | (lane >> 1 & 4);
     const int key0 = CH == 4 ? lw * 8 + (lane >> 2) : lw * 4 + ((lane >> 2 & 1) | (lane >> 3 & 2));
-    uint8_t* const raw = smem + G_::RAW + (lw * 32 + lane) * 16;  // its codes of K, then V: + 2048 i
+    uint8_t* const raw = smem + G_::RAW + (is_v ? G_::KBYTES / 2 : 0) + (lw * 32 + lane) * 16;  // its codes: + 2048 i
     const uint32_t to0 = swz(key0, ch / 4, 2 * (ch % 4)), to1 = to0 ^ 16;  // its places in a tile: + i * STEP
     constexpr uint32_t STEP = (128 / CH) * 128;
-    const uint32_t from = (uint32_t)((key0 & 15) * D + ch * 16);
-    auto fetch = [&](bool v, int j, uint32_t groups) {
-      const uint8_t* base = (v ? a.vc : a.kc) + from;
-      const uint32_t dst = smem_u32(raw) + (v ? G_::KBYTES / 2 : 0);
+    const uint8_t* const from = (is_v ? a.vc : a.kc) + ((key0 & 15) * D + ch * 16);
+    const uint32_t dst = smem_u32(raw);
+    auto fetch = [&](int j, uint32_t groups) {
       const bool tail = (j + 1) * kKeys > kv_end;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int key = key0 + i * (128 / CH);
         const uint32_t grp = __shfl_sync(0xffffffffu, groups, (j & 3) * kGroups + (key >> 4));
         const bool ok = grp != NONE && !(tail && j * kKeys + key >= kv_end);
-        cp_async_16(dst + 2048 * i, base + (ok ? (uint64_t)grp * (16 * D) : 0), ok ? 16 : 0);
+        cp_async_16(dst + 2048 * i, from + (ok ? (uint64_t)grp * (16 * D) : 0), ok ? 16 : 0);
       }
       cp_async_commit();
     };
     bool bad, bad_n;
     uint32_t grp = find(0, bad), grp_n = find(4, bad_n);
-    fetch(false, 0, grp);
-    fetch(true, 0, grp);
+    fetch(0, grp);
     float2 sc = scales(grp), sc_n = make_float2(0.f, 0.f);
     int RE = 127;                                // exponent field of R
     uint32_t rests = 0;                          // lanes whose group's value scale goes into the codes in part
@@ -621,13 +657,18 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
                                         : 0.f;
         rests = __ballot_sync(0xffffffffu, rest != 1.f);
         const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-        if (lw == 0) {
+        if (!is_v && lw == 0) {
           const float vf = vexp > 0 ? __uint_as_float((__float_as_uint(sc.y) & 0x7fffffu) | 0x3f800000u) : 1.f;
           StepInfo& f = infos[(j + (lane >> 3)) % kInfos];
           const int g = lane & (kGroups - 1);
+          float ve = (float)ep, vu = __uint_as_float((uint32_t)(127 - ep) << 23);
+          if (vf != 1.f) {
+            ve += log2f(vf);
+            vu /= vf;
+          }
           f.ks[g] = sc.x;
-          f.ve[g] = (float)ep + (vf == 1.f ? 0.f : log2f(vf));
-          f.vu[g] = __uint_as_float((uint32_t)(127 - ep) << 23) / vf;
+          f.ve[g] = ve;
+          f.vu[g] = vu;
           if (g == 0) {
             f.r = __uint_as_float((uint32_t)mine << 23);
             f.rf = rf;
@@ -638,77 +679,79 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         __syncwarp();
       }
       const uint32_t groups_next = ((j + 1) & 3) == 0 ? grp_n : grp;
-      if (j >= G_::KST && !wait.warp(kKEmpty + kst, (j / G_::KST - 1) & 1)) break;
-      cp_async_wait<1>();  // this step's K (its V may be on the way)
-      {
-        uint8_t* tile = smem + G_::K + kst * G_::KBYTES;
+      if (!is_v) {
+        if (j >= G_::KST && !wait.warp(kKEmpty + kst, (j / G_::KST - 1) & 1)) break;
+        cp_async_wait<0>();
+        {
+          uint8_t* tile = smem + G_::K + kst * G_::KBYTES;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
-          uint4 lo4, hi4;
-          e4m3x4_to_f16(x.x, lo4.x, lo4.y);
-          e4m3x4_to_f16(x.y, lo4.z, lo4.w);
-          e4m3x4_to_f16(x.z, hi4.x, hi4.y);
-          e4m3x4_to_f16(x.w, hi4.z, hi4.w);
-          *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
-          *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
-        }
-      }
-      __syncwarp();  // (the products' thread makes the stores visible to the tensor core)
-      if (lane == 0) mbar_arrive(wait.bar(kKFull + kst));
-      fetch(false, j + 1, groups_next);  // nothing behind the last key
-
-      if (j >= 2 && !wait.warp(kVEmpty + st, (j / 2 - 1) & 1)) break;
-      cp_async_wait<1>();  // this step's V (the next one's K may be on the way)
-      {
-        uint8_t* tile = smem + G_::V + st * G_::KBYTES;
-        const uint8_t* from_v = raw + G_::KBYTES / 2;
-        uint32_t seen = 0;
-        auto store = [&](uint4 x, int i) {
-          uint4 lo4, hi4;
-          e4m3x4_to_f16(x.x, lo4.x, lo4.y);
-          e4m3x4_to_f16(x.y, lo4.z, lo4.w);
-          e4m3x4_to_f16(x.z, hi4.x, hi4.y);
-          e4m3x4_to_f16(x.w, hi4.z, hi4.w);
-          if (rests >> q & ((1u << kGroups) - 1)) {
-            const __half2 r2 =
-                __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
-            lo4 = make_uint4(mul_h2(lo4.x, r2), mul_h2(lo4.y, r2), mul_h2(lo4.z, r2), mul_h2(lo4.w, r2));
-            hi4 = make_uint4(mul_h2(hi4.x, r2), mul_h2(hi4.y, r2), mul_h2(hi4.z, r2), mul_h2(hi4.w, r2));
-          }
-          *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
-          *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
-        };
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint4 x = *reinterpret_cast<const uint4*>(from_v + 2048 * i);
-          // a byte 0x7f or 0xff is NaN: its low seven bits and one more reach the eighth
-          seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
-                  ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
-          store(x, i);
-        }
-        const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
-        if (any_nan) {  // once more with zeros in their place, and the masks
-#pragma unroll 1
           for (int i = 0; i < N; ++i) {
-            uint4 x = *reinterpret_cast<const uint4*>(from_v + 2048 * i);
-            uint32_t* w = reinterpret_cast<uint32_t*>(&x);
-            uint32_t nan16 = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-              w[k] &= ~((n >> 7) * 0xffu);
-              nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+            uint4 lo4, hi4;
+            e4m3x4_to_f16(x.x, lo4.x, lo4.y);
+            e4m3x4_to_f16(x.y, lo4.z, lo4.w);
+            e4m3x4_to_f16(x.z, hi4.x, hi4.y);
+            e4m3x4_to_f16(x.w, hi4.z, hi4.w);
+            *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
+            *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wait.bar(kKFull + kst));
+      } else {
+        if (j >= 2 && !wait.warp(kVEmpty + st, (j / 2 - 1) & 1)) break;
+        cp_async_wait<0>();
+        {
+          uint8_t* tile = smem + G_::V + st * G_::KBYTES;
+                  uint32_t seen = 0;
+          auto store = [&](uint4 x, int i) {
+            uint4 lo4, hi4;
+            e4m3x4_to_f16(x.x, lo4.x, lo4.y);
+            e4m3x4_to_f16(x.y, lo4.z, lo4.w);
+            e4m3x4_to_f16(x.z, hi4.x, hi4.y);
+            e4m3x4_to_f16(x.w, hi4.z, hi4.w);
+            if (rests >> q & ((1u << kGroups) - 1)) {
+              const __half2 r2 =
+                  __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
+              lo4 = make_uint4(mul_h2(lo4.x, r2), mul_h2(lo4.y, r2), mul_h2(lo4.z, r2), mul_h2(lo4.w, r2));
+              hi4 = make_uint4(mul_h2(hi4.x, r2), mul_h2(hi4.y, r2), mul_h2(hi4.z, r2), mul_h2(hi4.w, r2));
             }
-            masks[((j % kMasks) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
+            *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
+            *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
+          };
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+            // a byte 0x7f or 0xff is NaN: its low seven bits and one more reach the eighth
+            seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
+                    ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
             store(x, i);
           }
+          const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
+          if (any_nan) {  // once more with zeros in their place, and the masks
+#pragma unroll 1
+            for (int i = 0; i < N; ++i) {
+              uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+              uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+              uint32_t nan16 = 0;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                w[k] &= ~((n >> 7) * 0xffu);
+                nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
+              }
+              masks[((j % kMasks) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
+              store(x, i);
+            }
+          }
+          if (lane == 0) infos[j % kInfos].nan[lw] = any_nan;
         }
-        if (lane == 0) infos[j % kInfos].nan[lw] = any_nan;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wait.bar(kVFull + st));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(wait.bar(kVFull + st));
-      fetch(true, j + 1, groups_next);
+      fetch(j + 1, groups_next);  // nothing behind the last key
       if ((j & 3) == 1) sc_n = scales(grp_n);
       if ((j & 3) == 3) {
         grp = grp_n;
@@ -720,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     cp_async_wait<0>();  // nothing lands after the CTA has left
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
-    if (warp == 12) {
+    if (warp == 16) {
       // ========================= tensor-core products ===========================
       const uint32_t base = smem_u32(smem);
       const int lead = elect_one();
@@ -745,7 +788,6 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       };
       auto ready = [&](int i, int parity) {
         if (!wait.warp(i, parity)) return false;
-        fence_proxy_async_smem();  // tiles were stored through the generic proxy
         tc_fence_after();
         return true;
       };
@@ -791,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_free(tmem);
+  if (warp == 16) tmem_free(tmem);
 }
 
 template <typename T, int D>
