@@ -10,11 +10,12 @@
 //
 // Roles (5 warpgroups; registers move from the last three to the softmax):
 //   * warps 0-3 and 4-7: the softmax of row tile 0 and 1, one row per thread.
-//     They read S in halves of 64 columns (the first half twice: a whole row in
-//     registers leaves none for the loaders), write P as f16 to tensor memory
-//     (beside S for head_dim 64; over its second half for 128, where nothing is
-//     left), and rescale O there only when a row's maximum has risen by more
-//     than 8 (in powers of two; P <= 2^8 then);
+//     A step takes its exponentials against the maximum so far and notes the
+//     largest exponent on the way: S is read once, 32 columns at a time.  Only
+//     when a row's exponent passes 8 (in powers of two; P <= 2^8 otherwise) is
+//     the maximum moved, O rescaled in tensor memory and the step taken again.
+//     P goes to tensor memory as f16 (beside S for head_dim 64; over it for 128,
+//     where nothing is left);
 //   * warps 8-11 and 12-15: the loaders of K and of V.  They copy codes through
 //     the block table one step ahead into shared memory (cp.async; block ids and
 //     scales are read four to eight steps ahead), turn them into f16 (exact) and
@@ -79,8 +80,8 @@ constexpr int kKeys = 128;                   // keys per step
 constexpr int kGroups = kKeys / 16;          // 16-key groups: each lies in one block
 constexpr int kThreads = 640;
 // Registers of the warpgroups: 2 softmax, 2 loaders, products; launched with 96 each.
-constexpr int kSoftmaxRegs = 136, kLoaderRegs = 80, kMmaRegs = 48;
-static_assert(2 * kSoftmaxRegs + 2 * kLoaderRegs + kMmaRegs <= 5 * 96, "a split of what the block was launched with");
+template <int D> struct Regs { static constexpr int SOFTMAX = 152, LOADER = 64, MMA = 48; };
+template <> struct Regs<64> { static constexpr int SOFTMAX = 128, LOADER = 88, MMA = 48; };
 constexpr int kMinValueExp = -4;
 constexpr int kInfos = 8;                    // steps whose side information is kept (two batches of four)
 constexpr int kMasks = 4;                    // steps whose NaN masks are kept
@@ -106,7 +107,7 @@ template <int D> struct Geo {
   static constexpr int BYTES = BARS + 128 + 1024;  // + alignment
   // tensor-memory columns: S 2 x 128, O 2 x D, P 2 x 64
   static constexpr bool P_APART = D == 64;
-  static constexpr int S_COL = 0, O_COL = 256, P_COL = P_APART ? 384 : 64, P_STEP = P_APART ? 64 : 128;
+  static constexpr int S_COL = 0, O_COL = 256, P_COL = P_APART ? 384 : 0, P_STEP = P_APART ? 64 : 128;
 };
 
 // Barriers (indices).
@@ -144,6 +145,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -155,7 +165,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
@@ -244,29 +254,31 @@ __device__ __forceinline__ uint32_t swz(int row, int panel, int c) {
   return (uint32_t)(panel * (kKeys * 128) + row * 128 + ((c ^ (row & 7)) << 4));
 }
 // Waits of all roles: bounded, and given up when another role has given up.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* stop, int* err) {
+  for (int n = 0; n < kWaitSpinLimit; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 63) == 63 && *stop) return false;
+  }
+  *stop = 1;
+  atomicOr(err, MVB_DEV_TIMEOUT);
+  return false;
+}
 struct Waiter {
   uint32_t bars;
   volatile int* stop;
   int* err;
   __device__ __forceinline__ uint32_t bar(int i) const { return bars + 8 * i; }
-  __device__ __forceinline__ bool operator()(int i, int parity) const {
-    for (int n = 0; n < kWaitSpinLimit; ++n) {
-      if (mbar_try_wait(bar(i), (uint32_t)parity)) return true;
-      if ((n & 63) == 63 && *stop) return false;
-    }
-    *stop = 1;
-    atomicOr(err, MVB_DEV_TIMEOUT);
-    return false;
-  }
   // All lanes of a warp, which stay together whatever each of them saw.
   __device__ __forceinline__ bool warp(int i, int parity) const {
-    return __all_sync(0xffffffffu, (*this)(i, parity)) != 0;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar(i), (uint32_t)parity))) return true;
+    return __all_sync(0xffffffffu, wait_on(bar(i), (uint32_t)parity, stop, err)) != 0;
   }
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8PrefillArgs a) {
   using G_ = Geo<D>;
+  static_assert(2 * Regs<D>::SOFTMAX + 2 * Regs<D>::LOADER + Regs<D>::MMA <= 5 * 96, "what the block was launched with");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int s_tot[2][kThreads / 32];
@@ -389,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   const uint32_t tmem = s_tmem;
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<D>::SOFTMAX));
     // ================================ softmax =================================
     const int tile = warp >> 2, r = row0 + tile * kTileRows + (warp & 3) * 32 + lane;
     if (tile < tiles) {
@@ -453,79 +465,103 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       auto step = [&](int j, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
         const StepInfo& f = infos[j % kInfos];
-        uint32_t s[64];
         const int rem = lim - j * kKeys;
-        auto read_half = [&](int h) {  // 64 columns of S, -inf where the row does not attend the key
-          tmem_ld32(s_at + 64 * h, s);
-          tmem_ld32(s_at + 64 * h + 32, s + 32);
-          tc_wait_ld();
+        // columns read at a time, two reads in flight; P over S waits in registers until the step holds
+        constexpr int CW = G_::P_APART ? 32 : 16, NC = kKeys / CW;
+        uint32_t s[2][CW];
+        auto read = [&](int h) {
+          if constexpr (CW == 32)
+            tmem_ld32(s_at + CW * h, s[h & 1]);
+          else
+            tmem_ld16(s_at + CW * h, s[h & 1]);
+        };
+        auto mask = [&](int h) {  // -inf where the row does not attend the key
           if constexpr (EDGE) {
-            const int bad = f.bad >> (4 * h), n = rem - 64 * h;
+            const int bad = f.bad >> (CW / 16 * h), n = rem - CW * h;
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i >= n || (bad >> (i / 16) & 1)) s[i] = 0xff800000u;
+            for (int i = 0; i < CW; ++i)
+              if (i >= n || (bad >> (i / 16) & 1)) s[h & 1][i] = 0xff800000u;
           }
         };
-        auto col = [&](int i) { return __uint_as_float(s[i]); };
-        float c[kGroups], mx = -INFINITY;
+        auto factor = [&](int g) { return fmaxf(qs * f.ks[g], 1.2e-38f); };  // (not 0: -inf stays -inf)
+        if (__any_sync(0xffffffffu, m == -INFINITY)) {  // a row's first keys: its maximum before anything else
+          float mx = m;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          read_half(h);
-          float top[4];
+          for (int h = 0; h < NC; ++h) {
+            read(h);
+            tc_wait_ld();
+            mask(h);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            c[4 * h + g] = fmaxf(qs * f.ks[4 * h + g], 1.2e-38f);  // (not 0: -inf stays -inf)
-            top[g] = fmaxf(col(16 * g), col(16 * g + 1));
+            for (int g = 0; g < CW / 16; ++g) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; i += 2)
+                top = fmaxf(fmaxf(top, __uint_as_float(s[h & 1][16 * g + i])),
+                            __uint_as_float(s[h & 1][16 * g + i + 1]));
+              mx = fmaxf(mx, top * factor(CW / 16 * h + g));
+            }
           }
-#pragma unroll
-          for (int i = 2; i < 16; i += 2)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) top[g] = fmaxf(fmaxf(top[g], col(16 * g + i)), col(16 * g + i + 1));
-#pragma unroll
-          for (int g = 0; g < 4; ++g) mx = fmaxf(mx, top[g] * c[4 * h + g]);
+          if (m == -INFINITY) m = mx;  // (l and O are 0)
         }
-        const bool jump = mx > m + 8.f;
         const float rf = f.rf;
-        const bool move = __any_sync(0xffffffffu, jump) || rf != 1.f;
         float fac = rf;
-        if (move) {
-          const float mn = jump ? mx : m, al = jump ? fast_exp2(m - mn) : 1.f;
-          m = mn;
-          l *= al;
-          fac *= al;
-        }
+        bool move = rf != 1.f;
+        read(NC - 1);
         // the last step's products read P and added to O
         if (j > 0) {
           if (!wait.warp(kPvDone + tile, (j - 1) & 1)) return false;
           tc_fence_after();
           take_nan(j - 1);
         }
-        // a row that has attended nothing yet: m and all of s are -inf, and P is 0
-        const float base = EDGE && m == -INFINITY ? 0.f : -m;
+        uint32_t p[G_::P_APART ? 16 : 64];
+        for (;;) {
+          // a row that has attended nothing yet: m and all of s are -inf, and P is 0
+          const float base = EDGE && m == -INFINITY ? 0.f : -m;
+          float sum = 0.f, over = -INFINITY;  // the largest exponent
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {  // the second half is at hand; P may lie over it
-          if (half == 0) read_half(0);
+          for (int h = NC - 1; h >= 0; --h) {
+            const uint32_t(&x)[CW] = s[h & 1];
+            tc_wait_ld();
+            if (h > 0) read(h - 1);
+            mask(h);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t p[16];
-#pragma unroll
-            for (int gg = 0; gg < 2; ++gg) {
-              const int g = 4 * half + 2 * h + gg;
-              const float2 cc = make_float2(c[g], c[g]), mm = make_float2(base + f.ve[g], base + f.ve[g]);
+            for (int gg = 0; gg < CW / 16; ++gg) {
+              const int g = CW / 16 * h + gg;
+              const float c = factor(g), ve = f.ve[g];
+              const float2 cc = make_float2(c, c), mm = make_float2(base + ve, base + ve);
               float2 t = make_float2(0.f, 0.f);
+              float top = -INFINITY;
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
-                const int k = 32 * h + 16 * gg + i;
-                float2 e = fma2(make_float2(col(k), col(k + 1)), cc, mm);
+                float2 e = fma2(make_float2(__uint_as_float(x[16 * gg + i]), __uint_as_float(x[16 * gg + i + 1])), cc, mm);
+                top = fmaxf(fmaxf(top, e.x), e.y);
                 e.x = fast_exp2(e.x);
                 e.y = fast_exp2(e.y);
                 t = add2(t, e);
-                p[8 * gg + i / 2] = pack_h2(e.x, e.y);
+                p[(G_::P_APART ? 0 : CW / 2 * h) + 8 * gg + i / 2] = pack_h2(e.x, e.y);
               }
-              l = fmaf(t.x + t.y, f.vu[g], l);
+              sum = fmaf(t.x + t.y, f.vu[g], sum);
+              over = fmaxf(over, top - ve);
             }
-            tmem_st16(p_at + 32 * half + 16 * h, p);
+            if constexpr (G_::P_APART) tmem_st16(p_at + CW / 2 * h, p);
           }
+          const bool jump = over > 8.f;
+          if (!__any_sync(0xffffffffu, jump)) {
+            l += sum;
+            break;
+          }
+          if (jump) {  // (over is at most 0 the next time)
+            const float al = fast_exp2(-over);
+            m += over;
+            l *= al;
+            fac *= al;
+          }
+          move = true;
+          read(NC - 1);
+        }
+        if constexpr (!G_::P_APART) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) tmem_st16(p_at + 16 * h, p + 16 * h);
         }
         if (move && j > 0) {
 #pragma unroll
@@ -580,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       }
     }
   } else if (warp < 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<D>::LOADER));
     // ================================ loaders =================================
     constexpr int CH = D / 16, N = kKeys * CH / 128;  // 16-code chunks per row, chunks per thread and tile
     constexpr uint32_t NONE = 0xffffffffu;
@@ -613,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     const uint32_t dst = smem_u32(raw);
     auto fetch = [&](int j, uint32_t groups) {
       const bool tail = (j + 1) * kKeys > kv_end;
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < N; ++i) {
         const int key = key0 + i * (128 / CH);
         const uint32_t grp = __shfl_sync(0xffffffffu, groups, (j & 3) * kGroups + (key >> 4));
@@ -684,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         cp_async_wait<0>();
         {
           uint8_t* tile = smem + G_::K + kst * G_::KBYTES;
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < N; ++i) {
             const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
             uint4 lo4, hi4;
@@ -720,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
             *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
             *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
           };
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < N; ++i) {
             const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
             // a byte 0x7f or 0xff is NaN: its low seven bits and one more reach the eighth
@@ -762,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     }
     cp_async_wait<0>();  // nothing lands after the CTA has left
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<D>::MMA));
     if (warp == 16) {
       // ========================= tensor-core products ===========================
       const uint32_t base = smem_u32(smem);
