@@ -10,12 +10,12 @@
 //
 // Roles (5 warpgroups; registers move from the last three to the softmax):
 //   * warps 0-3 and 4-7: the softmax of row tile 0 and 1, one row per thread.
-//     A step takes its exponentials against the maximum so far and notes the
-//     largest exponent on the way: S is read once, 32 columns at a time.  Only
-//     when a row's exponent passes 8 (in powers of two; P <= 2^8 otherwise) is
-//     the maximum moved, O rescaled in tensor memory and the step taken again.
-//     P goes to tensor memory as f16 (beside S for head_dim 64; over it for 128,
-//     where nothing is left);
+//     A step takes its exponentials against a maximum of earlier steps and reads
+//     S once.  P may then exceed 1; only when 16 of them add up to more than 2^14
+//     (so that f16 never overflows) is the maximum taken anew, O rescaled in
+//     tensor memory and the step repeated.  A maximum per step cost 128 of its
+//     some 600 instructions.  P goes to tensor memory as f16 (beside S for
+//     head_dim 64; over it for 128, where nothing is left);
 //   * warps 8-11 and 12-15: the loaders of K and of V.  They copy codes through
 //     the block table one step ahead into shared memory (cp.async; block ids and
 //     scales are read four to eight steps ahead), turn them into f16 (exact) and
@@ -88,10 +88,9 @@ constexpr int kMasks = 4;                    // steps whose NaN masks are kept
 constexpr int kTmemCols = 512;
 
 // Side information of one step, written by the loaders.
-struct StepInfo {
-  float ks[kGroups];  // key scales
-  float ve[kGroups];  // log2 of the part of (value scale / R) that goes into P
-  float vu[kGroups];  // 2^-ve
+struct alignas(16) StepInfo {
+  // per group: the key scale; log2 of the part ve of (value scale / R) that goes into P; 2^-ve
+  float4 g[kGroups];
   float r;            // reference R of the values (O is in units of it)
   float rf;           // the previous step's R over this one's
   int bad;            // bit g: the group's block id is invalid, its keys are left out
@@ -483,30 +482,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
               if (i >= n || (bad >> (i / 16) & 1)) s[h & 1][i] = 0xff800000u;
           }
         };
-        auto factor = [&](int g) { return fmaxf(qs * f.ks[g], 1.2e-38f); };  // (not 0: -inf stays -inf)
-        if (__any_sync(0xffffffffu, m == -INFINITY)) {  // a row's first keys: its maximum before anything else
-          float mx = m;
-#pragma unroll
-          for (int h = 0; h < NC; ++h) {
-            read(h);
-            tc_wait_ld();
-            mask(h);
-#pragma unroll
-            for (int g = 0; g < CW / 16; ++g) {
-              float top = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 16; i += 2)
-                top = fmaxf(fmaxf(top, __uint_as_float(s[h & 1][16 * g + i])),
-                            __uint_as_float(s[h & 1][16 * g + i + 1]));
-              mx = fmaxf(mx, top * factor(CW / 16 * h + g));
-            }
-          }
-          if (m == -INFINITY) m = mx;  // (l and O are 0)
-        }
+        auto factor = [&](float ks) { return fmaxf(qs * ks, 1.2e-38f); };  // (not 0: -inf stays -inf)
+        bool anew = __any_sync(0xffffffffu, m == -INFINITY);  // a row's first keys
         const float rf = f.rf;
         float fac = rf;
         bool move = rf != 1.f;
-        read(NC - 1);
         // the last step's products read P and added to O
         if (j > 0) {
           if (!wait.warp(kPvDone + tile, (j - 1) & 1)) return false;
@@ -515,49 +495,72 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         }
         uint32_t p[G_::P_APART ? 16 : 64];
         for (;;) {
+          if (anew) {
+            float mx = m;
+#pragma unroll
+            for (int h = 0; h < NC; ++h) {
+              read(h);
+              tc_wait_ld();
+              mask(h);
+#pragma unroll
+              for (int g = 0; g < CW / 16; ++g) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2)
+                  top = fmaxf(fmaxf(top, __uint_as_float(s[h & 1][16 * g + i])),
+                              __uint_as_float(s[h & 1][16 * g + i + 1]));
+                mx = fmaxf(mx, top * factor(f.g[CW / 16 * h + g].x));
+              }
+            }
+            const float al = mx == m ? 1.f : fast_exp2(m - mx);  // (0 for a row's first keys, where l and O are 0)
+            m = mx;
+            l *= al;
+            fac *= al;
+            move = true;
+          }
+          read(NC - 1);
+          float4 info[2][CW / 16];  // of the columns at hand and of the next ones
+#pragma unroll
+          for (int g = 0; g < CW / 16; ++g) info[(NC - 1) & 1][g] = f.g[CW / 16 * (NC - 1) + g];
           // a row that has attended nothing yet: m and all of s are -inf, and P is 0
           const float base = EDGE && m == -INFINITY ? 0.f : -m;
-          float sum = 0.f, over = -INFINITY;  // the largest exponent
+          float sum = 0.f, most = 0.f;
 #pragma unroll
           for (int h = NC - 1; h >= 0; --h) {
             const uint32_t(&x)[CW] = s[h & 1];
             tc_wait_ld();
-            if (h > 0) read(h - 1);
+            if (h > 0) {
+              read(h - 1);
+#pragma unroll
+              for (int g = 0; g < CW / 16; ++g) info[(h - 1) & 1][g] = f.g[CW / 16 * (h - 1) + g];
+            }
             mask(h);
 #pragma unroll
             for (int gg = 0; gg < CW / 16; ++gg) {
-              const int g = CW / 16 * h + gg;
-              const float c = factor(g), ve = f.ve[g];
-              const float2 cc = make_float2(c, c), mm = make_float2(base + ve, base + ve);
-              float2 t = make_float2(0.f, 0.f);
-              float top = -INFINITY;
+              const float4 in = info[h & 1][gg];
+              const float c = factor(in.x), b = base + in.y;
+              const float2 cc = make_float2(c, c), mm = make_float2(b, b);
+              float2 t[2];
 #pragma unroll
               for (int i = 0; i < 16; i += 2) {
                 float2 e = fma2(make_float2(__uint_as_float(x[16 * gg + i]), __uint_as_float(x[16 * gg + i + 1])), cc, mm);
-                top = fmaxf(fmaxf(top, e.x), e.y);
                 e.x = fast_exp2(e.x);
                 e.y = fast_exp2(e.y);
-                t = add2(t, e);
+                t[i / 2 & 1] = i < 4 ? e : add2(t[i / 2 & 1], e);
                 p[(G_::P_APART ? 0 : CW / 2 * h) + 8 * gg + i / 2] = pack_h2(e.x, e.y);
               }
-              sum = fmaf(t.x + t.y, f.vu[g], sum);
-              over = fmaxf(over, top - ve);
+              t[0] = add2(t[0], t[1]);
+              const float u = t[0].x + t[0].y;
+              most = fmaxf(most, u);
+              sum = fmaf(u, in.z, sum);
             }
             if constexpr (G_::P_APART) tmem_st16(p_at + CW / 2 * h, p);
           }
-          const bool jump = over > 8.f;
-          if (!__any_sync(0xffffffffu, jump)) {
+          anew = __any_sync(0xffffffffu, most > 16384.f);
+          if (!anew) {
             l += sum;
             break;
           }
-          if (jump) {  // (over is at most 0 the next time)
-            const float al = fast_exp2(-over);
-            m += over;
-            l *= al;
-            fac *= al;
-          }
-          move = true;
-          read(NC - 1);
         }
         if constexpr (!G_::P_APART) {
 #pragma unroll
@@ -702,9 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
             ve += log2f(vf);
             vu /= vf;
           }
-          f.ks[g] = sc.x;
-          f.ve[g] = ve;
-          f.vu[g] = vu;
+          f.g[g] = make_float4(sc.x, ve, vu, 0.f);
           if (g == 0) {
             f.r = __uint_as_float((uint32_t)mine << 23);
             f.rf = rf;
