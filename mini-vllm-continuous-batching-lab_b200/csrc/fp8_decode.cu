@@ -8,11 +8,12 @@
 // group; 16 heads are two column blocks), so 7 heads waste one column where
 // heads as rows would waste 9 of 16:
 //   S^T[16 tokens, 8 heads] = K_codes Q^T,   O^T[D, 8 heads] = V_codes^T P^T.
-// * Codes go to f16 (exact) in registers, straight from global memory: the sum
-//   over D may run in any order, so a lane's 16 contiguous bytes of a K row
-//   serve four k-steps, and its 8 (D = 64) or 16 contiguous bytes of four V rows
-//   are D/8 rows of O^T.  No shared memory lies between the cache and the tensor
-//   core.
+// * A tile is 16 D contiguous bytes of K and of V.  Each warp copies its tiles
+//   into a ring of its own (cp.async, Fp8Geo::STAGES tiles) and turns codes into
+//   f16 (exact) in registers: the sum over D may run in any order, so a lane's 16
+//   contiguous bytes of a K row serve four k-steps, and its 8 (D = 64) or 16
+//   contiguous bytes of four V rows are D/8 rows of O^T.  The tiles held in
+//   registers instead, two ahead, reached 59 % of the memory's rate.
 // * The query enters as f16, each head's row times a power of two that brings
 //   its largest element into [1, 2): exact for f16 queries and for bf16 ones but
 //   for elements below 2^-14 of the row's largest, which lose bits under 2^-24
@@ -62,31 +63,43 @@ constexpr int kFp8DecodeMaxSeqs = 8192;
 // A warp gets at least this many tiles where the batch has few.
 constexpr int kFp8MinTiles = 2;
 
-// Geometry by head_dim and column blocks: warps per CTA and tiles a warp loads ahead.
+// Geometry by head_dim and column blocks: warps per CTA and tiles in a warp's
+// ring.  The rings, a piece per warp and the prefix of the largest batch fill
+// shared memory.
 template <int D, int NG> struct Fp8Geo;
-template <> struct Fp8Geo<64, 1> { static constexpr int NW = 16, DEPTH = 2; };
-template <> struct Fp8Geo<64, 2> { static constexpr int NW = 12, DEPTH = 2; };
-template <> struct Fp8Geo<128, 1> { static constexpr int NW = 12, DEPTH = 2; };
-template <> struct Fp8Geo<128, 2> { static constexpr int NW = 8, DEPTH = 2; };
+template <> struct Fp8Geo<64, 1> { static constexpr int NW = 16, STAGES = 5; };
+template <> struct Fp8Geo<64, 2> { static constexpr int NW = 12, STAGES = 5; };
+template <> struct Fp8Geo<128, 1> { static constexpr int NW = 12, STAGES = 3; };
+template <> struct Fp8Geo<128, 2> { static constexpr int NW = 8, STAGES = 4; };
 
-template <int D, int NG>
-int decode_smem(int num_seqs) {
-  constexpr int NW = Fp8Geo<D, NG>::NW, HR = 8 * NG;
-  return NW * 2 * HR * (D + 2) * 4 + NW * 2 * 16 + (2 * num_seqs + 1) * 4;
-}
+template <int D, int NG> struct Fp8Smem {
+  static constexpr int NW = Fp8Geo<D, NG>::NW, TILE = 2 * 16 * D;  // K, then V
+  static constexpr int PIECE = 8 * NG * (D + 2) * 4;  // bytes of one partial state: O [8 NG][D], then (m, l) [8 NG]
+  static constexpr int RING = 0, PARTS = RING + NW * Fp8Geo<D, NG>::STAGES * TILE, IDS = PARTS + NW * PIECE;
+  static constexpr int PRE = IDS + NW * 2 * 16;
+  static constexpr int bytes(int num_seqs) { return PRE + (num_seqs + 1) * 4; }
+  static_assert(Fp8Geo<D, NG>::STAGES * TILE >= PIECE, "a warp's second piece lies in its ring");
+  static_assert(bytes(kFp8DecodeMaxSeqs) + 128 <= 227 * 1024, "shared memory of one CTA");
+};
 
-__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// 16-byte chunk c of token r of a tile in shared memory: the chunks that eight
+// lanes (K) or sixteen lanes (V, 8 bytes each at D = 64) read at once lie in
+// different banks, for the token order of the rows below.
+template <int D>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  if constexpr (D == 64) return (uint32_t)(r * 64 + ((c ^ ((r >> 2 & 1) << 1)) << 4));
+  else return (uint32_t)(r * 128 + ((c ^ ((r >> 1 & 3) << 1) ^ ((r & 1) << 2)) << 4));
+}
+// Token of row r (0-7, and 8 more) of a tile's product.
+__device__ __forceinline__ int token_of(int r) { return r ^ (r >> 1 & 1); }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -140,15 +153,18 @@ __device__ __forceinline__ float2 merge_row(int n, float m, float l, bool norm, 
 
 template <typename T, int D, int NG>
 __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(const Fp8DecodeArgs a) {
-  constexpr int NW = Fp8Geo<D, NG>::NW, DEPTH = Fp8Geo<D, NG>::DEPTH;
+  using Sm = Fp8Smem<D, NG>;
+  constexpr int NW = Fp8Geo<D, NG>::NW, ST = Fp8Geo<D, NG>::STAGES;
   constexpr int HR = 8 * NG, MT = D / 16, KS = D / 16, KW = D / 64;
-  constexpr int PIECE = HR * (D + 2);  // floats of one partial state: O [HR][D], then (m, l) [HR]
   extern __shared__ __align__(16) uint8_t smem[];
-  float* parts = reinterpret_cast<float*>(smem);                       // [NW][2][PIECE]
-  int4* ids = reinterpret_cast<int4*>(smem + NW * 2 * PIECE * 4);      // [NW][2] {unit, seq, k, ends in this CTA}
-  int* pre = reinterpret_cast<int*>(ids + NW * 2);                     // [Nd + 1] tile prefix
-  int* ctxs = pre + a.num_seqs + 1;                                    // [Nd] tokens (0: left out)
+  int4* ids = reinterpret_cast<int4*>(smem + Sm::IDS);  // [NW][2] {unit, seq, k, ends in this CTA}
+  int* pre = reinterpret_cast<int*>(smem + Sm::PRE);    // [Nd + 1] tile prefix
   __shared__ int sums[NW];
+  // A warp's partial states: slot 0 of a unit that began before its range, slot 1 (in its ring, at the end) of one
+  // that runs on.
+  auto part_of = [&](int w, int slot) {
+    return reinterpret_cast<float*>(smem + (slot == 0 ? Sm::PARTS + w * Sm::PIECE : Sm::RING + w * ST * Sm::TILE));
+  };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
@@ -169,7 +185,6 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
                       : ((int64_t)c + (1 << a.block_shift) - 1) >> a.block_shift > a.max_blocks ? MVB_DEV_TABLE_SHORT
                                                                                                : 0;
       const int n = bad ? 0 : ((c + kFp8Tile - 1) / kFp8Tile) * KHG;
-      ctxs[i] = bad ? 0 : c;
       pre[i] = n;
       mine += n;
       if (bad && blockIdx.x == 0) atomicOr(a.err, bad);
@@ -198,7 +213,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
   }
   // rows of sequences that cannot be served: zeros
   for (int i = blockIdx.x * NW + warp; i < Nd; i += gridDim.x * NW) {
-    if (ctxs[i] != 0) continue;
+    if (pre[i] != pre[i + 1]) continue;
     for (int e = lane; e < a.num_heads * D; e += 32)
       out[(int64_t)i * a.o_s0 + (int64_t)(e / D) * a.o_s1 + e % D] = from_f32<T>(0.f);
   }
@@ -221,68 +236,59 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     }
     Unit u;
     u.seq = lo;
-    u.ctx = ctxs[lo];
+    u.ctx = __ldg(a.kv_len + lo);
     const int n = (u.ctx + kFp8Tile - 1) / kFp8Tile;
     u.k = (tile - pre[lo]) / n;
     u.start = pre[lo] + u.k * n;
     u.end = u.start + n;
     return u;
   };
-  const int BSm = (1 << a.block_shift) - 1;
-  // Lane-wise: where tile `tile` of the stream lies: (block, KV head) row and
-  // the tile's first token in the block; row -1 for a bad block id.
-  auto find_tile = [&](int tile, int& row, int& at) {
+  const int BSm = (1 << a.block_shift) - 1, gshift = a.block_shift - 4;
+  constexpr uint32_t NONE = 0xffffffffu;
+  // Lane-wise: tile `tile` of the stream, numbered among the cache's 16-token groups; NONE for a bad block id.
+  auto find_tile = [&](int tile) {
     const Unit u = unit_at(tile);
     const int tok = (tile - u.start) * kFp8Tile;
     const int64_t b = __ldg(a.bt + (int64_t)u.seq * a.bt_s0 + (tok >> a.block_shift));
-    at = tok & BSm;
-    row = b >= 0 && b < a.num_blocks ? (int)b * a.num_kv_heads + u.k / a.head_groups : -1;
-    if (row < 0) atomicOr(a.err, MVB_DEV_BLOCK_ID);
+    if (b >= 0 && b < a.num_blocks)
+      return ((uint32_t)((int)b * a.num_kv_heads + u.k / a.head_groups) << gshift) + ((uint32_t)(tok & BSm) >> 4);
+    atomicOr(a.err, MVB_DEV_BLOCK_ID);
+    return NONE;
   };
 
   if (r0 < r1) {
     // 32 tiles' places and scales at a time, one per lane; the next 32 are fetched ahead
-    int row = -1, at = 0, row_n = -1, at_n = 0;
-    float2 sc = make_float2(0.f, 0.f);
-    if (r0 + lane < r1) find_tile(r0 + lane, row, at);
-    if (row >= 0) sc = __ldg(a.scale + row);
-    if (r0 + 32 + lane < r1) find_tile(r0 + 32 + lane, row_n, at_n);
-
-    uint4 kr[DEPTH][2 * KW];  // rows g and g + 8, 16 bytes per 64 columns
-    uint4 vr[DEPTH][KW == 1 ? 2 : 4];  // rows 2t, 2t+1, 2t+8, 2t+9: 8 (16) bytes each
-    auto tile_off = [&](int j) -> int64_t {  // byte offset of the tile `j` places into the current 32 (may be the next's)
-      const int rw = j < 32 ? __shfl_sync(0xffffffffu, row, j & 31) : __shfl_sync(0xffffffffu, row_n, j & 31);
-      const int ta = j < 32 ? __shfl_sync(0xffffffffu, at, j & 31) : __shfl_sync(0xffffffffu, at_n, j & 31);
-      return (((int64_t)max(rw, 0) << a.block_shift) + ta) * D;
-    };
-    auto load_k = [&](uint4 (&k)[2 * KW], int64_t off) {
-      const uint8_t* p = a.kc + off + 16 * t4;
+    uint32_t grp = NONE, grp_n = NONE;
+    if (r0 + lane < r1) grp = find_tile(r0 + lane);
+    // lane's chunks of a tile: 16 bytes each 512 bytes, and where they go
+    constexpr int NCH = D / 32;
+    uint32_t to[NCH];
 #pragma unroll
-      for (int c = 0; c < KW; ++c) {
-        k[2 * c] = ld_stream16(p + g * D + 64 * c);
-        k[2 * c + 1] = ld_stream16(p + (g + 8) * D + 64 * c);
+    for (int i = 0; i < NCH; ++i) {
+      const int c = i * 32 + lane;
+      to[i] = chunk_at<D>(c / (D / 16), c % (D / 16));
+    }
+    const uint32_t ring = smem_u32(smem + Sm::RING + warp * ST * Sm::TILE);
+    int put = 0;  // stage that is filled next
+    // Start the copies of the tile `j` places into the current 32 (or the next 32's).
+    auto issue = [&](int j) {
+      const uint32_t g = __shfl_sync(0xffffffffu, j < 32 ? grp : grp_n, j & 31);
+      const uint64_t off = (uint64_t)(g == NONE ? 0u : g) * (16 * D) + lane * 16;
+      const uint32_t dst = ring + put * Sm::TILE;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        cp_async_16(dst + to[i], a.kc + off + 512 * i);
+        cp_async_16(dst + 16 * D + to[i], a.vc + off + 512 * i);
       }
-    };
-    auto load_v = [&](uint4 (&v)[KW == 1 ? 2 : 4], int64_t off) {
-      const uint8_t* p = a.vc + off + 2 * t4 * D + (D / 8) * g;
-      if constexpr (KW == 1) {
-        const uint2 x = ld_stream8(p), y = ld_stream8(p + D), z = ld_stream8(p + 8 * D), w = ld_stream8(p + 9 * D);
-        v[0] = make_uint4(x.x, x.y, y.x, y.y);
-        v[1] = make_uint4(z.x, z.y, w.x, w.y);
-      } else {
-        v[0] = ld_stream16(p);
-        v[1] = ld_stream16(p + D);
-        v[2] = ld_stream16(p + 8 * D);
-        v[3] = ld_stream16(p + 9 * D);
-      }
+      put = put + 1 == ST ? 0 : put + 1;
     };
 #pragma unroll
-    for (int b = 0; b < DEPTH; ++b)
-      if (r0 + b < r1) {
-        const int64_t off = tile_off(b);
-        load_k(kr[b], off);
-        load_v(vr[b], off);
-      }
+    for (int b = 0; b < ST - 1; ++b) {
+      if (r0 + b < r1) issue(b);
+      cp_async_commit();
+    }
+    float2 sc = grp != NONE ? __ldg(a.scale + (grp >> gshift)) : make_float2(0.f, 0.f), sc_n = sc;
+    if (r0 + 32 + lane < r1) grp_n = find_tile(r0 + 32 + lane);
 
     Unit u = unit_at(r0);
     uint32_t qf[NG][KS][2];
@@ -338,7 +344,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     auto end_unit = [&]() {
       const bool whole = u.start >= r0 && u.end <= r1;
       const int slot = u.start < r0 ? 0 : 1;
-      float* P = parts + (warp * 2 + slot) * PIECE;
+      float* P = part_of(warp, slot);
       if (!whole && lane == 0) ids[warp * 2 + slot] = make_int4(u.start, u.seq, u.k, u.end <= c1 ? 1 : 0);
 #pragma unroll
       for (int n = 0; n < NG; ++n)
@@ -375,29 +381,57 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     };
     begin_unit();
 
-    int j = 0;  // the tile's place in the current 32
-    for (int tile = r0; tile < r1;) {
+    // rows g and g + 8 of K, and rows 2t, 2t + 1, 2t + 8, 2t + 9 of V, in a stage
+    const int tok_g = token_of(g);
+    const uint32_t k_at = chunk_at<D>(tok_g, t4);  // (8 tokens on: + 8 D; 64 columns on: the chunk's bit 2)
+    uint32_t v_at[2];
 #pragma unroll
-      for (int b = 0; b < DEPTH; ++b) {
-        if (tile < r1) {
-          if (tile == u.end) {
-            end_unit();
-            u = unit_at(tile);
-            begin_unit();
-          }
-          const int rw = __shfl_sync(0xffffffffu, row, j);
-          const float ks = __shfl_sync(0xffffffffu, sc.x, j), vs = __shfl_sync(0xffffffffu, sc.y, j);
-          int valid = rw < 0 ? 0 : u.ctx - (tile - u.start) * kFp8Tile;  // tokens of the tile that count
-          const bool more = tile + DEPTH < r1;
-          const int64_t next = more ? tile_off(j + DEPTH) : 0;
+    for (int i = 0; i < 2; ++i)
+      v_at[i] = KW == 1 ? chunk_at<D>(token_of(2 * t4 + i), g >> 1) + 8 * (g & 1) : chunk_at<D>(token_of(2 * t4 + i), g);
+    int j = 0, get = 0;  // the tile's place in the current 32; its stage
+    for (int tile = r0; tile < r1; ++tile) {
+      if (tile == u.end) {
+        end_unit();
+        u = unit_at(tile);
+        begin_unit();
+      }
+      cp_async_wait<ST - 2>();  // this tile is here
+      __syncwarp();             // for all lanes, and they are done with the last one
+      if (tile + ST - 1 < r1) issue(j + ST - 1);
+      cp_async_commit();
+      const uint8_t* stage = smem + Sm::RING + (warp * ST + get) * Sm::TILE;
+      get = get + 1 == ST ? 0 : get + 1;
+      const float ks = __shfl_sync(0xffffffffu, sc.x, j), vs = __shfl_sync(0xffffffffu, sc.y, j);
+      // tokens of the tile that count
+      const int valid = __shfl_sync(0xffffffffu, grp, j) == NONE ? 0 : u.ctx - (tile - u.start) * kFp8Tile;
+      uint4 kr[2 * KW];
+#pragma unroll
+      for (int c = 0; c < KW; ++c) {
+        kr[2 * c] = *reinterpret_cast<const uint4*>(stage + (k_at ^ (c << 6)));
+        kr[2 * c + 1] = *reinterpret_cast<const uint4*>(stage + (k_at ^ (c << 6)) + 8 * D);
+      }
+      constexpr int WR = D / 32;  // words of one V row in this lane
+      uint32_t v[4 * WR];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* p = stage + 16 * D + v_at[i & 1] + (i >> 1) * 8 * D;
+        if constexpr (KW == 1) {
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
+          v[2 * i] = x.x, v[2 * i + 1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+        }
+      }
+      {
           // S^T = K Q^T
           float s[NG][4];
 #pragma unroll
           for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
           for (int c = 0; c < KW; ++c) {
-            const uint32_t* x = reinterpret_cast<const uint32_t*>(&kr[b][2 * c]);
-            const uint32_t* y = reinterpret_cast<const uint32_t*>(&kr[b][2 * c + 1]);
+            const uint32_t* x = reinterpret_cast<const uint32_t*>(&kr[2 * c]);
+            const uint32_t* y = reinterpret_cast<const uint32_t*>(&kr[2 * c + 1]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t a0, a1, a2, a3;
@@ -407,8 +441,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
               for (int n = 0; n < NG; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][4 * c + k][0], qf[n][4 * c + k][1]);
             }
           }
-          if (more) load_k(kr[b], next);
-          // logits (powers of two) above the running maximum; tokens g and g + 8
+          // logits (powers of two) above the running maximum; rows g and g + 8
           float y[NG][4];
           bool jump = false;
 #pragma unroll
@@ -416,7 +449,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               y[n][i] = fmaf(s[n][i], qs[n][i & 1] * ks, -m[n][i & 1]);
-              if (g + (i >> 1) * 8 >= valid) y[n][i] = -INFINITY;
+              if (tok_g + (i >> 1) * 8 >= valid) y[n][i] = -INFINITY;
               jump |= y[n][i] > 8.f;
             }
           }
@@ -427,8 +460,8 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
               for (int c = 0; c < 2; ++c) {
                 const float f = qs[n][c] * ks;
                 float mx = m[n][c];
-                if (g < valid) mx = fmaxf(mx, s[n][c] * f);
-                if (g + 8 < valid) mx = fmaxf(mx, s[n][c + 2] * f);
+                if (tok_g < valid) mx = fmaxf(mx, s[n][c] * f);
+                if (tok_g + 8 < valid) mx = fmaxf(mx, s[n][c + 2] * f);
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -440,8 +473,8 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
                   o[n][i][c] *= al;
                   o[n][i][c + 2] *= al;
                 }
-                y[n][c] = g < valid ? fmaf(s[n][c], f, -mx) : -INFINITY;
-                y[n][c + 2] = g + 8 < valid ? fmaf(s[n][c + 2], f, -mx) : -INFINITY;
+                y[n][c] = tok_g < valid ? fmaf(s[n][c], f, -mx) : -INFINITY;
+                y[n][c + 2] = tok_g + 8 < valid ? fmaf(s[n][c + 2], f, -mx) : -INFINITY;
               }
           }
           uint32_t pb[NG][2];
@@ -456,12 +489,10 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
             pb[n][1] = movmatrix(pack_h2(y[n][2], y[n][3]));
           }
           // O^T += vs * (V^T P^T); rows past the last token may hold any bits
-          uint32_t* v = reinterpret_cast<uint32_t*>(&vr[b][0]);
-          constexpr int WR = D / 32;  // words of one V row in this lane
           if (valid < kFp8Tile) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (2 * t4 + (i & 1) + (i >> 1) * 8 >= valid)
+              if (token_of(2 * t4 + (i & 1)) + (i >> 1) * 8 >= valid)
 #pragma unroll
                 for (int w = 0; w < WR; ++w) v[i * WR + w] = 0u;
           }
@@ -483,19 +514,18 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
               }
             }
           }
-          if (more) load_v(vr[b], next);
-          ++tile;
-          if (++j == 32) {
-            j = 0;
-            row = row_n;
-            at = at_n;
-            sc = row >= 0 ? __ldg(a.scale + row) : make_float2(0.f, 0.f);
-            row_n = -1;
-            if (tile + 32 + lane < r1) find_tile(tile + 32 + lane, row_n, at_n);
-          }
+        if (++j == 32) {
+          j = 0;
+          grp = grp_n;
+          sc = sc_n;
+          grp_n = NONE;
+          if (tile + 33 + lane < r1) grp_n = find_tile(tile + 33 + lane);
+        } else if (j == 16) {
+          sc_n = grp_n != NONE ? __ldg(a.scale + (grp_n >> gshift)) : make_float2(0.f, 0.f);
         }
       }
     }
+    __syncwarp();  // the ring has been read, and no copy is on its way: the last piece may lie in it
     end_unit();
   }
   __syncthreads();
@@ -517,7 +547,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     const bool has = mine < NW && (lane == 0 || ids[mine * 2].x == id.x);
     const uint32_t mask = __ballot_sync(0xffffffffu, has);
     const int n = 32 - __clz(mask);
-    auto piece = [&](int i) { return parts + ((first + i) * 2 + (i == 0 && cand < NW ? 1 : 0)) * PIECE; };
+    auto piece = [&](int i) { return part_of(first + i, i == 0 && cand < NW ? 1 : 0); };
     float pm = -INFINITY, pl = 0.f;
     if (has) {
       const float2 ml = *reinterpret_cast<const float2*>(piece(lane) + HR * D + 2 * h);
@@ -624,9 +654,10 @@ int plan_decode(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int
   pl->nw = head_dim == 64 ? (pl->ng == 1 ? Fp8Geo<64, 1>::NW : Fp8Geo<64, 2>::NW)
                           : (pl->ng == 1 ? Fp8Geo<128, 1>::NW : Fp8Geo<128, 2>::NW);
   const int units = num_kv_heads * pl->head_groups;
-  // tile and (block, KV head) numbers are 32-bit
+  // tile, (block, KV head) and 16-token group numbers are 32-bit
   if ((int64_t)num_seqs * units * ((int64_t)max_blocks * block_size / kFp8Tile + 1) >= ((int64_t)1 << 31) ||
-      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31))
+      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31) ||
+      (int64_t)num_blocks * num_kv_heads * (block_size / 16) >= 0xffffffffll)
     return MVB_ERR_INVALID_ARG;
   pl->grid = decode_grid(num_seqs, units, max_blocks, block_size, pl->nw);
   pl->off_part = ((int64_t)pl->grid * 32 + 255) / 256 * 256;
@@ -637,9 +668,9 @@ int plan_decode(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int
 template <typename T, int D, int NG>
 int launch_decode(const Fp8DecodeArgs& a, int grid, cudaStream_t stream) {
   auto kern = fp8_decode_kernel<T, D, NG>;
-  const int smem = decode_smem<D, NG>(a.num_seqs);
+  const int smem = Fp8Smem<D, NG>::bytes(a.num_seqs);
   // the largest batch's size at once: the attribute is set on the first call only
-  if (ensure_kernel_attrs(kern, decode_smem<D, NG>(kFp8DecodeMaxSeqs)) != cudaSuccess) return MVB_ERR_CUDA;
+  if (ensure_kernel_attrs(kern, Fp8Smem<D, NG>::bytes(kFp8DecodeMaxSeqs)) != cudaSuccess) return MVB_ERR_CUDA;
   if (launch_pdl(kern, dim3(grid), dim3(Fp8Geo<D, NG>::NW * 32), smem, stream, a) != cudaSuccess) return MVB_ERR_CUDA;
   if (grid == 1) return MVB_OK;  // no unit is cut between CTAs
   auto merge = fp8_decode_merge_kernel<T, D, 8 * NG>;
