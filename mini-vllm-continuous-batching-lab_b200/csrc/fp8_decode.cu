@@ -19,11 +19,16 @@
 //   for elements below 2^-14 of the row's largest, which lose bits under 2^-24
 //   of it.
 // * All tokens of a tile lie in one block, so the key scale is one factor of the
-//   tile's logits and the value scale one factor of its O^T contribution; both
-//   multiply 32-bit results.
-// * p enters as f16 (11 bits; the output has 8 or 11).  The running maximum m is
-//   moved only when a logit exceeds it by 8 (in powers of two): p <= 2^8 then,
-//   and a tile needs no reduction across lanes, only a vote.
+//   tile's logits.  The value scale v joins the exponent: P = p v / R, with the
+//   sum of p undone per tile, O in units of R, a power of two: the first tile's
+//   scale, moved (O with it) when a scale passes 2^7 R.  The exponent takes v / R
+//   down to 2^-4, where P's f16 still has 10 bits for p >= 2^-10; the rest of a
+//   smaller scale goes into the f16 codes (exact to 2^-15 R).
+// * P enters as f16 (11 bits; the output has 8 or 11), against a maximum m of
+//   earlier tiles; m is taken anew only when a lane's P add up to more than 2^14,
+//   so a tile needs no reduction across lanes, only a vote.
+// * With a factor on every output of a tile and a maximum per tile, one tile at a
+//   time, it took 204 instructions per tile of head_dim 64 and was bound by them.
 //
 // Work split: the tiles of all (sequence, KV head, head group) units in order
 // are one stream, cut into equal ranges, one per warp of a grid of at most one
@@ -33,6 +38,8 @@
 // fp8_decode_merge_kernel joins in CTA order.  The workspace holds nothing from
 // one call to the next and needs no initialisation.
 // Bound: memory (1 byte per element; 28 operations per byte at 7 heads).
+#include <type_traits>
+
 #include "fp8_common.cuh"
 
 namespace mvb {
@@ -60,6 +67,8 @@ namespace {
 
 constexpr int kFp8Tile = 16;
 constexpr int kFp8DecodeMaxSeqs = 8192;
+// log2 of (value scale / reference) that P takes up.
+constexpr float kMinValueExp = -4.f, kMaxValueExp = 7.f;
 // A warp gets at least this many tiles where the batch has few.
 constexpr int kFp8MinTiles = 2;
 
@@ -107,6 +116,10 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, __half2 f) {
+  const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), f);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -282,23 +295,41 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
       }
       put = put + 1 == ST ? 0 : put + 1;
     };
+    // tiles on their way or at hand before each step, which takes one or two (D = 64) and starts as many
+    constexpr int AHEAD = D == 64 ? ST - 2 : ST - 1;
 #pragma unroll
-    for (int b = 0; b < ST - 1; ++b) {
+    for (int b = 0; b < AHEAD; ++b) {
       if (r0 + b < r1) issue(b);
       cp_async_commit();
     }
-    float2 sc = grp != NONE ? __ldg(a.scale + (grp >> gshift)) : make_float2(0.f, 0.f), sc_n = sc;
+    // a group's key scale and log2 of its value scale (exact for a power of two)
+    auto scales = [&](uint32_t group) {
+      if (group == NONE) return make_float2(0.f, 0.f);
+      float2 x = __ldg(a.scale + (group >> gshift));
+      const uint32_t bits = __float_as_uint(x.y);
+      x.y = (bits & 0x7fffffu) == 0 && bits != 0 ? (float)((int)(bits >> 23) - 127) : log2f(x.y);
+      return x;
+    };
+    float2 sc = scales(grp), sc_n = sc;
+    uint32_t bad = __ballot_sync(0xffffffffu, grp == NONE);  // places of the current 32 without a block
     if (r0 + 32 + lane < r1) grp_n = find_tile(r0 + 32 + lane);
 
     Unit u = unit_at(r0);
+    int j = 0, get = 0;  // the current tile's place in the current 32, and its stage
     uint32_t qf[NG][KS][2];
     float qs[NG][2];  // per column (heads 2t, 2t + 1): softmax scale, log2 e, the query row's power of two
     float o[NG][MT][4], m[NG][2], l[NG][2];
     int h0 = 0, nh = 0;
+    float R = 0.f;       // log2 of the reference that O is in units of, once a tile has given it
+    bool have_r = false;
+    bool fresh = true;   // the unit has no maximum yet
     auto begin_unit = [&]() {
       const int kvh = u.k / a.head_groups, hg = u.k - kvh * a.head_groups;
       h0 = kvh * a.G + hg * HR;
       nh = min(HR, a.G - hg * HR);
+      R = 0.f;
+      have_r = false;
+      fresh = true;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         const int h = 8 * n + g;
@@ -344,6 +375,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     auto end_unit = [&]() {
       const bool whole = u.start >= r0 && u.end <= r1;
       const int slot = u.start < r0 ? 0 : 1;
+      const float unit_of_o = fast_exp2(R);
       float* P = part_of(warp, slot);
       if (!whole && lane == 0) ids[warp * 2 + slot] = make_int4(u.start, u.seq, u.k, u.end <= c1 ? 1 : 0);
 #pragma unroll
@@ -358,7 +390,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
           if (h >= nh) continue;
           // this lane's D / 8 contiguous dims of head h: element 2i + half of o[i][c + 2 half]
           if (whole) {
-            const float inv = s == 0.f ? 0.f : 1.f / s;
+            const float inv = s == 0.f ? 0.f : unit_of_o / s;
             T* p = out + (int64_t)u.seq * a.o_s0 + (int64_t)(h0 + h) * a.o_s1 + (D / 8) * g;
             uint32_t w[MT];
 #pragma unroll
@@ -374,7 +406,8 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
 #pragma unroll
             for (int i = 0; i < MT / 2; ++i)
               *reinterpret_cast<float4*>(p + 4 * i) =
-                  make_float4(o[n][2 * i][c], o[n][2 * i][c + 2], o[n][2 * i + 1][c], o[n][2 * i + 1][c + 2]);
+                  make_float4(o[n][2 * i][c] * unit_of_o, o[n][2 * i][c + 2] * unit_of_o,
+                              o[n][2 * i + 1][c] * unit_of_o, o[n][2 * i + 1][c + 2] * unit_of_o);
             if (g == 0) *reinterpret_cast<float2*>(P + HR * D + 2 * h) = make_float2(m[n][c], s);
           }
         }
@@ -388,141 +421,210 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       v_at[i] = KW == 1 ? chunk_at<D>(token_of(2 * t4 + i), g >> 1) + 8 * (g & 1) : chunk_at<D>(token_of(2 * t4 + i), g);
-    int j = 0, get = 0;  // the tile's place in the current 32; its stage
-    for (int tile = r0; tile < r1; ++tile) {
+    // Tiles [tile, tile + NT) of one unit (their places j and on are in the current 32).
+    auto attend = [&](int tile, auto count) {
+      constexpr int NT = decltype(count)::value, WR = D / 32;  // WR: words of one V row in this lane
+      cp_async_wait<AHEAD - NT>();  // these tiles are here
+      __syncwarp();                 // for all lanes, and they are done with the tiles before
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        if (tile + AHEAD + b < r1) issue(j + AHEAD + b);
+        cp_async_commit();
+      }
+      uint32_t stage[NT];
+      float ks[NT], ve[NT];
+      bool edge = false;
+      int valid[NT];  // tokens of the tile that count
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        stage[b] = (uint32_t)((warp * ST + get) * Sm::TILE);
+        get = get + 1 == ST ? 0 : get + 1;
+        ks[b] = __shfl_sync(0xffffffffu, sc.x, j + b);
+        ve[b] = __shfl_sync(0xffffffffu, sc.y, j + b) - R;
+        valid[b] = (bad >> (j + b)) & 1 ? 0 : u.ctx - (tile + b - u.start) * kFp8Tile;
+        edge |= valid[b] < kFp8Tile;
+      }
+      // value scales that R does not serve
+      float rest[NT];
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        rest[b] = 1.f;
+        if (!(ve[b] >= kMinValueExp && ve[b] <= kMaxValueExp) || !have_r) {
+          if ((ve[b] > kMaxValueExp || !have_r) && ve[b] > -INFINITY) {  // R moves, and O with it
+            const float up = floorf(ve[b]), f = fast_exp2(-up);
+            R += up;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) ve[i] -= up;
+            if (have_r) {
+#pragma unroll
+              for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[n][i][e] *= f;
+            }
+            have_r = true;
+          }
+          if (ve[b] < kMinValueExp) {
+            rest[b] = fast_exp2(ve[b] - kMinValueExp);
+            ve[b] = kMinValueExp;
+          }
+        }
+      }
+      // S^T = K Q^T
+      float s[NT][NG][4];
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KW; ++c) {
+          const uint8_t* p = smem + stage[b] + (k_at ^ (c << 6));
+          const uint4 x4 = *reinterpret_cast<const uint4*>(p), y4 = *reinterpret_cast<const uint4*>(p + 8 * D);
+          const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16(x[k], a0, a2);
+            e4m3x4_to_f16(y[k], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma_f16(s[b][n], a0, a1, a2, a3, qf[n][4 * c + k][0], qf[n][4 * c + k][1]);
+          }
+        }
+      }
+      uint32_t v[NT][4 * WR];
+#pragma unroll
+      for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* p = smem + stage[b] + 16 * D + v_at[i & 1] + (i >> 1) * 8 * D;
+          if constexpr (KW == 1) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            v[b][2 * i] = x.x, v[b][2 * i + 1] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(p);
+            v[b][4 * i] = x.x, v[b][4 * i + 1] = x.y, v[b][4 * i + 2] = x.z, v[b][4 * i + 3] = x.w;
+          }
+        }
+      // P against the maximum of earlier tiles; taken anew where a lane's P add up to more than 2^14
+      uint32_t pb[NT][NG][2];
+      for (bool anew = fresh;;) {
+        if (anew) {
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = m[n][c];
+#pragma unroll
+              for (int b = 0; b < NT; ++b) {
+                if (tok_g < valid[b]) mx = fmaxf(mx, s[b][n][c] * (qs[n][c] * ks[b]));
+                if (tok_g + 8 < valid[b]) mx = fmaxf(mx, s[b][n][c + 2] * (qs[n][c] * ks[b]));
+              }
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float al = m[n][c] == mx ? 1.f : fast_exp2(m[n][c] - mx);
+              m[n][c] = mx;
+              l[n][c] *= al;
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                o[n][i][c] *= al;
+                o[n][i][c + 2] *= al;
+              }
+            }
+        }
+        float t[NT][NG][2];
+        bool over = false;
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fmaf(s[b][n][i], qs[n][i & 1] * ks[b], ve[b] - m[n][i & 1]);
+            if (edge) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (tok_g + (i >> 1) * 8 >= valid[b]) y[i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fast_exp2(y[i]);
+            t[b][n][0] = y[0] + y[2];
+            t[b][n][1] = y[1] + y[3];
+            over |= fmaxf(t[b][n][0], t[b][n][1]) > 16384.f;
+            pb[b][n][0] = pack_h2(y[0], y[1]);
+            pb[b][n][1] = pack_h2(y[2], y[3]);
+          }
+        anew = __any_sync(0xffffffffu, over);
+        if (anew) continue;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+          const float vu = fast_exp2(-ve[b]);
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            l[n][0] = fmaf(t[b][n][0], vu, l[n][0]);
+            l[n][1] = fmaf(t[b][n][1], vu, l[n][1]);
+            pb[b][n][0] = movmatrix(pb[b][n][0]);
+            pb[b][n][1] = movmatrix(pb[b][n][1]);
+          }
+        }
+        break;
+      }
+      if (fresh) fresh = __any_sync(0xffffffffu, m[0][0] == -INFINITY);  // (nothing but bad blocks so far)
+      // O^T += V^T P^T; rows past the last token may hold any bits
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (token_of(2 * t4 + (i & 1)) + (i >> 1) * 8 >= valid[b])
+#pragma unroll
+              for (int w = 0; w < WR; ++w) v[b][i * WR + w] = 0u;
+        }
+#pragma unroll
+        for (int w = 0; w < WR; ++w) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362 : 0x5140;  // bytes (A0 B0 A1 B1) or (A2 B2 A3 B3)
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16(__byte_perm(v[b][w], v[b][WR + w], sel), a0, a1);
+            e4m3x4_to_f16(__byte_perm(v[b][2 * WR + w], v[b][3 * WR + w], sel), a2, a3);
+            if (rest[b] != 1.f) {
+              const __half2 f = __float2half2_rn(rest[b]);
+              a0 = mul_h2(a0, f), a1 = mul_h2(a1, f), a2 = mul_h2(a2, f), a3 = mul_h2(a3, f);
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + half], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
+          }
+        }
+      }
+      j += NT;
+    };
+    for (int tile = r0; tile < r1;) {
       if (tile == u.end) {
         end_unit();
         u = unit_at(tile);
         begin_unit();
       }
-      cp_async_wait<ST - 2>();  // this tile is here
-      __syncwarp();             // for all lanes, and they are done with the last one
-      if (tile + ST - 1 < r1) issue(j + ST - 1);
-      cp_async_commit();
-      const uint8_t* stage = smem + Sm::RING + (warp * ST + get) * Sm::TILE;
-      get = get + 1 == ST ? 0 : get + 1;
-      const float ks = __shfl_sync(0xffffffffu, sc.x, j), vs = __shfl_sync(0xffffffffu, sc.y, j);
-      // tokens of the tile that count
-      const int valid = __shfl_sync(0xffffffffu, grp, j) == NONE ? 0 : u.ctx - (tile - u.start) * kFp8Tile;
-      uint4 kr[2 * KW];
-#pragma unroll
-      for (int c = 0; c < KW; ++c) {
-        kr[2 * c] = *reinterpret_cast<const uint4*>(stage + (k_at ^ (c << 6)));
-        kr[2 * c + 1] = *reinterpret_cast<const uint4*>(stage + (k_at ^ (c << 6)) + 8 * D);
+      const int before = j;
+      // two tiles at once where the unit, the range and the 32 places have them: half the bookkeeping, twice the
+      // independent work (D = 128 has that in one)
+      if (D == 64 && min(u.end, r1) - tile >= 2 && j < 31) {
+        attend(tile, std::integral_constant<int, D == 64 ? 2 : 1>());
+        tile += 2;
+      } else {
+        attend(tile, std::integral_constant<int, 1>());
+        ++tile;
       }
-      constexpr int WR = D / 32;  // words of one V row in this lane
-      uint32_t v[4 * WR];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = stage + 16 * D + v_at[i & 1] + (i >> 1) * 8 * D;
-        if constexpr (KW == 1) {
-          const uint2 x = *reinterpret_cast<const uint2*>(p);
-          v[2 * i] = x.x, v[2 * i + 1] = x.y;
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(p);
-          v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
-        }
-      }
-      {
-          // S^T = K Q^T
-          float s[NG][4];
-#pragma unroll
-          for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-          for (int c = 0; c < KW; ++c) {
-            const uint32_t* x = reinterpret_cast<const uint32_t*>(&kr[2 * c]);
-            const uint32_t* y = reinterpret_cast<const uint32_t*>(&kr[2 * c + 1]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t a0, a1, a2, a3;
-              e4m3x4_to_f16(x[k], a0, a2);
-              e4m3x4_to_f16(y[k], a1, a3);
-#pragma unroll
-              for (int n = 0; n < NG; ++n) mma_f16(s[n], a0, a1, a2, a3, qf[n][4 * c + k][0], qf[n][4 * c + k][1]);
-            }
-          }
-          // logits (powers of two) above the running maximum; rows g and g + 8
-          float y[NG][4];
-          bool jump = false;
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              y[n][i] = fmaf(s[n][i], qs[n][i & 1] * ks, -m[n][i & 1]);
-              if (tok_g + (i >> 1) * 8 >= valid) y[n][i] = -INFINITY;
-              jump |= y[n][i] > 8.f;
-            }
-          }
-          if (__any_sync(0xffffffffu, jump)) {
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float f = qs[n][c] * ks;
-                float mx = m[n][c];
-                if (tok_g < valid) mx = fmaxf(mx, s[n][c] * f);
-                if (tok_g + 8 < valid) mx = fmaxf(mx, s[n][c + 2] * f);
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float al = m[n][c] == mx ? 1.f : fast_exp2(m[n][c] - mx);
-                m[n][c] = mx;
-                l[n][c] *= al;
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                  o[n][i][c] *= al;
-                  o[n][i][c + 2] *= al;
-                }
-                y[n][c] = tok_g < valid ? fmaf(s[n][c], f, -mx) : -INFINITY;
-                y[n][c + 2] = tok_g + 8 < valid ? fmaf(s[n][c + 2], f, -mx) : -INFINITY;
-              }
-          }
-          uint32_t pb[NG][2];
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              y[n][i] = fast_exp2(y[n][i]);
-              l[n][i & 1] += y[n][i];
-            }
-            pb[n][0] = movmatrix(pack_h2(y[n][0], y[n][1]));
-            pb[n][1] = movmatrix(pack_h2(y[n][2], y[n][3]));
-          }
-          // O^T += vs * (V^T P^T); rows past the last token may hold any bits
-          if (valid < kFp8Tile) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (token_of(2 * t4 + (i & 1)) + (i >> 1) * 8 >= valid)
-#pragma unroll
-                for (int w = 0; w < WR; ++w) v[i * WR + w] = 0u;
-          }
-#pragma unroll
-          for (int w = 0; w < WR; ++w) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t sel = half ? 0x7362 : 0x5140;  // bytes (A0 B0 A1 B1) or (A2 B2 A3 B3)
-              uint32_t a0, a1, a2, a3;
-              e4m3x4_to_f16(__byte_perm(v[w], v[WR + w], sel), a0, a1);
-              e4m3x4_to_f16(__byte_perm(v[2 * WR + w], v[3 * WR + w], sel), a2, a3);
-              const int i = 2 * w + half;
-#pragma unroll
-              for (int n = 0; n < NG; ++n) {
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(x, a0, a1, a2, a3, pb[n][0], pb[n][1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][i][e] = fmaf(x[e], vs, o[n][i][e]);
-              }
-            }
-          }
-        if (++j == 32) {
-          j = 0;
-          grp = grp_n;
-          sc = sc_n;
-          grp_n = NONE;
-          if (tile + 33 + lane < r1) grp_n = find_tile(tile + 33 + lane);
-        } else if (j == 16) {
-          sc_n = grp_n != NONE ? __ldg(a.scale + (grp_n >> gshift)) : make_float2(0.f, 0.f);
-        }
+      if (j == 32) {
+        j = 0;
+        grp = grp_n;
+        sc = sc_n;
+        bad = __ballot_sync(0xffffffffu, grp == NONE);
+        grp_n = NONE;
+        if (tile + 32 + lane < r1) grp_n = find_tile(tile + 32 + lane);
+      } else if (before < 16 && j >= 16) {
+        sc_n = scales(grp_n);
       }
     }
     __syncwarp();  // the ring has been read, and no copy is on its way: the last piece may lie in it

@@ -628,3 +628,36 @@ def test_prefill_value_scales_that_grow():
     out = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, [0], [0], [n], bs)
     # rows of the first 128 positions attend small values only, and are not lost beside what comes later
     check_prefill(out, q, kc, vc, sc, table, [0], [n], bs)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 8, 128)])
+def test_value_scales_that_jump_about(heads):
+    """Value scales far apart in both directions, zeros (a block never written, a block of zeros) and small ones that
+    count: decode, and prefill of the same queries."""
+    lens = [700, 90]
+    q, kc, vc, sc, table, kvl = decode_case(31, lens, heads, 16, torch.bfloat16)
+    r = np.random.RandomState(5)
+    for i, n in enumerate(lens):
+        for b in range(-(-n // 16)):
+            sc[table[i, b], :, 1] *= 2.0 ** float(r.randint(-14, 15))
+    sc[table[0, 0], :, 1] = 0.0        # the first tile gives no reference
+    sc[table[1, 0], :, 1] = 2.0 ** -100
+    bits(vc)[table[1, 0]] = 0
+    check_decode(M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16), q, kc, vc, sc, table, lens, 16)
+    one = torch.ones(2, dtype=torch.int64, device=DEV)
+    out = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, one.cumsum(0) - 1, kvl.long() - 1, one, 16)
+    check_decode(out, q, kc, vc, sc, table, lens, 16)
+
+
+def test_decode_one_head_of_nan_leaves_the_others():
+    lens = [600]
+    q, kc, vc, sc, table, kvl = decode_case(32, lens, (14, 2, 64), 16, torch.bfloat16)
+    sc[table[0, 20], :, 1] *= 2.0 ** 12
+    q[0, 3] = math.nan
+    out = M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16)
+    assert torch.isnan(out[0, 3]).all()
+    keep = [h for h in range(14) if h != 3]
+    k, v = (F.dequant(c, sc, w, table[0, :38], 600) for w, c in enumerate((kc, vc)))
+    q[0, 3] = 0
+    ref, tol = F.attend(q, k, v, 600, 0.125)
+    F.check(out[:, keep], ref[:, keep], tol[:, keep])
