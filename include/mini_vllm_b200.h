@@ -427,7 +427,7 @@ int mvb_rope_kv_cache_write_fp8(const void* query, int64_t q_stride_token, int64
                                 void* stream);
 
 /* Paged decode attention over the 8-bit cache, one query token per sequence;
- * arguments, zero rows and device errors as in mvb_paged_decode (at most 8192
+ * arguments, zero rows and device errors as in mvb_paged_decode (at most 6144
  * sequences).  `workspace` holds mvb_paged_decode_fp8_workspace bytes (same
  * arguments; 256-byte aligned, contents arbitrary before and after); calls
  * that may overlap on the GPU need one each. */

@@ -293,7 +293,7 @@ def paged_decode_attention_fp8(
     Arguments, result and errors are ``paged_decode_attention``'s, with ``kv_scale`` beside the caches.  The
     query enters the tensor cores as f16 (a bf16 row by a power of two, exact but for elements below 2**-14 of
     its largest), probabilities as f16; logits, sums and the output are accumulated in float32.  The result does
-    not depend on timing.  At most 8192 sequences.  The call keeps no state between calls and may be captured.
+    not depend on timing.  At most 6144 sequences.  The call keeps no state between calls and may be captured.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5

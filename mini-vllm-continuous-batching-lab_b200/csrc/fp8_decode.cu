@@ -9,11 +9,11 @@
 // heads as rows would waste 9 of 16:
 //   S^T[16 tokens, 8 heads] = K_codes Q^T,   O^T[D, 8 heads] = V_codes^T P^T.
 // * A tile is 16 D contiguous bytes of K and of V.  Each warp copies its tiles
-//   into a ring of its own (cp.async, Fp8Geo::STAGES tiles) and turns codes into
-//   f16 (exact) in registers: the sum over D may run in any order, so a lane's 16
-//   contiguous bytes of a K row serve four k-steps, and its 8 (D = 64) or 16
-//   contiguous bytes of four V rows are D/8 rows of O^T.  The tiles held in
-//   registers instead, two ahead, reached 59 % of the memory's rate.
+//   into a ring of its own (Fp8Geo::STAGES tiles, TMA, one mbarrier a stage) and
+//   turns codes into f16 (exact) in registers: the sum over D may run in any
+//   order, so a lane's 16 contiguous bytes of a K row serve four k-steps, and its
+//   8 (D = 64) or 16 contiguous bytes of four V rows are D/8 rows of O^T.  The
+//   same ring filled by cp.async stayed at 5.1 TB/s with no arithmetic at all.
 // * The query enters as f16, each head's row times a power of two that brings
 //   its largest element into [1, 2): exact for f16 queries and for bf16 ones but
 //   for elements below 2^-14 of the row's largest, which lose bits under 2^-24
@@ -38,11 +38,15 @@
 // fp8_decode_merge_kernel joins in CTA order.  The workspace holds nothing from
 // one call to the next and needs no initialisation.
 // Bound: memory (1 byte per element; 28 operations per byte at 7 heads).
+#include <cudaTypedefs.h>
+
 #include <type_traits>
 
 #include "fp8_common.cuh"
 
 namespace mvb {
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // capi.cu
 
 struct Fp8DecodeArgs {
   const void* q;
@@ -66,7 +70,7 @@ struct Fp8DecodeArgs {
 namespace {
 
 constexpr int kFp8Tile = 16;
-constexpr int kFp8DecodeMaxSeqs = 8192;
+constexpr int kFp8DecodeMaxSeqs = 6144;  // the tile prefix lies in shared memory
 // log2 of (value scale / reference) that P takes up.
 constexpr float kMinValueExp = -4.f, kMaxValueExp = 7.f;
 // A warp gets at least this many tiles where the batch has few.
@@ -85,30 +89,28 @@ template <int D, int NG> struct Fp8Smem {
   static constexpr int NW = Fp8Geo<D, NG>::NW, TILE = 2 * 16 * D;  // K, then V
   static constexpr int PIECE = 8 * NG * (D + 2) * 4;  // bytes of one partial state: O [8 NG][D], then (m, l) [8 NG]
   static constexpr int RING = 0, PARTS = RING + NW * Fp8Geo<D, NG>::STAGES * TILE, IDS = PARTS + NW * PIECE;
-  static constexpr int PRE = IDS + NW * 2 * 16;
-  static constexpr int bytes(int num_seqs) { return PRE + (num_seqs + 1) * 4; }
+  static constexpr int BARS = IDS + NW * 2 * 16, PRE = BARS + NW * Fp8Geo<D, NG>::STAGES * 8;
+  // (the prefix gives way to the list of cut units at the end; 1024 for the alignment)
+  static constexpr int bytes(int num_seqs) { return PRE + (num_seqs < 64 ? 64 : num_seqs + 1) * 4 + 1024; }
+  static_assert(2 * (NW + 1) <= 64, "the list fits");
   static_assert(Fp8Geo<D, NG>::STAGES * TILE >= PIECE, "a warp's second piece lies in its ring");
   static_assert(bytes(kFp8DecodeMaxSeqs) + 128 <= 227 * 1024, "shared memory of one CTA");
 };
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// 16-byte chunk c of token r of a tile in shared memory: the chunks that eight
-// lanes (K) or sixteen lanes (V, 8 bytes each at D = 64) read at once lie in
-// different banks, for the token order of the rows below.
+// Byte offset of 16-byte chunk c of token r of a tile as the TMA load leaves it: rows of 128 bytes (two tokens at
+// D = 64: boxes of 64-byte rows stayed at 4.6 TB/s), chunks swizzled by the row.
 template <int D>
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  if constexpr (D == 64) return (uint32_t)(r * 64 + ((c ^ ((r >> 2 & 1) << 1)) << 4));
-  else return (uint32_t)(r * 128 + ((c ^ ((r >> 1 & 3) << 1) ^ ((r & 1) << 2)) << 4));
+  const int b = r * D + c * 16, row = b >> 7;
+  return (uint32_t)(row * 128 + ((b & 127) ^ ((row & 7) << 4)));
 }
-// Token of row r (0-7, and 8 more) of a tile's product.
-__device__ __forceinline__ int token_of(int r) { return r ^ (r >> 1 & 1); }
+// The same chunk 8 tokens on.
+template <int D>
+__device__ __forceinline__ uint32_t on8(uint32_t at) { return D == 64 ? (at ^ 64) + 512 : at + 1024; }
+// Token of row r (0-7, and 8 more) of a tile's product: an order in which the chunks that eight lanes (K, and V at
+// D = 128) or sixteen lanes (V at D = 64, 8 bytes each) read at once lie in different banks.
+template <int D>
+__device__ __forceinline__ int token_of(int r) { return D == 64 ? r ^ (r >> 1 & 1) : r ^ ((r & 1) << 2); }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -134,42 +136,17 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 struct Unit {
   int start, end;  // its tiles [start, end) of the stream
   int seq, k;      // sequence, unit of the sequence
-  int ctx;         // tokens
 };
 
-// Weighted sum of the pieces' states of one head row: lane i < n holds piece
-// i's (m, l) and calls `o(i, d)` for its sums.  Writes O to dst(d, value) with
-// the factor `norm ? 1 / L : 1` and returns (M, L).
-template <int D, typename LoadO, typename Store>
-__device__ __forceinline__ float2 merge_row(int n, float m, float l, bool norm, LoadO o, Store st) {
-  const int lane = threadIdx.x & 31;
-  float M = m;
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-  const float w = m == -INFINITY ? 0.f : fast_exp2(m - M);
-  float L = w * l;
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) L += __shfl_xor_sync(0xffffffffu, L, s);
-  float acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  for (int p = 0; p < n; ++p) {
-    const float wp = __shfl_sync(0xffffffffu, w, p);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(wp, o(p, lane + 32 * i), acc[i]);
-  }
-  const float f = !norm ? 1.f : L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) st(lane + 32 * i, acc[i] * f);
-  return make_float2(M, L);
-}
-
 template <typename T, int D, int NG>
-__global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(const Fp8DecodeArgs a) {
+__global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1)
+fp8_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                  const Fp8DecodeArgs a) {
   using Sm = Fp8Smem<D, NG>;
   constexpr int NW = Fp8Geo<D, NG>::NW, ST = Fp8Geo<D, NG>::STAGES;
   constexpr int HR = 8 * NG, MT = D / 16, KS = D / 16, KW = D / 64;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   int4* ids = reinterpret_cast<int4*>(smem + Sm::IDS);  // [NW][2] {unit, seq, k, ends in this CTA}
   int* pre = reinterpret_cast<int*>(smem + Sm::PRE);    // [Nd + 1] tile prefix
   __shared__ int sums[NW];
@@ -183,6 +160,10 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
   const int g = lane >> 2, t4 = lane & 3;
   const int Nd = a.num_seqs, KHG = a.num_kv_heads * a.head_groups;
   T* const out = static_cast<T*>(a.out);
+  if (tid == 0) {
+    prefetch_tensormap(&tmk);
+    prefetch_tensormap(&tmv);
+  }
   grid_dependency_wait();
   grid_launch_dependents();
 
@@ -233,7 +214,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
 
   const int T_all = pre[Nd];
   const int ctas = min((int)gridDim.x, max(1, (T_all + NW * kFp8MinTiles - 1) / (NW * kFp8MinTiles)));
-  const int W = ctas * NW, wid = blockIdx.x * NW + warp;
+  const int W = min(ctas * NW, max(T_all, 1)), wid = blockIdx.x * NW + warp;
   auto bound = [&](int w) { return (int)((int64_t)min(w, W) * T_all / W); };
   const int r0 = bound(wid), r1 = bound(wid + 1);
   const int c0 = bound(blockIdx.x * NW), c1 = bound(blockIdx.x * NW + NW);
@@ -249,100 +230,123 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     }
     Unit u;
     u.seq = lo;
-    u.ctx = __ldg(a.kv_len + lo);
-    const int n = (u.ctx + kFp8Tile - 1) / kFp8Tile;
+    const int n = (pre[lo + 1] - pre[lo]) / KHG;
     u.k = (tile - pre[lo]) / n;
     u.start = pre[lo] + u.k * n;
     u.end = u.start + n;
     return u;
   };
   const int BSm = (1 << a.block_shift) - 1, gshift = a.block_shift - 4;
-  constexpr uint32_t NONE = 0xffffffffu;
-  // Lane-wise: tile `tile` of the stream, numbered among the cache's 16-token groups; NONE for a bad block id.
-  auto find_tile = [&](int tile) {
+  const uint64_t policy = l2_policy_evict_first();
+  // Lane-wise: tile `tile` of the stream, numbered among the cache's 16-token groups; for a bad block id group 0,
+  // which is read and not counted.
+  auto find_tile = [&](int tile, bool& missing) {
     const Unit u = unit_at(tile);
     const int tok = (tile - u.start) * kFp8Tile;
     const int64_t b = __ldg(a.bt + (int64_t)u.seq * a.bt_s0 + (tok >> a.block_shift));
     if (b >= 0 && b < a.num_blocks)
       return ((uint32_t)((int)b * a.num_kv_heads + u.k / a.head_groups) << gshift) + ((uint32_t)(tok & BSm) >> 4);
     atomicOr(a.err, MVB_DEV_BLOCK_ID);
-    return NONE;
+    missing = true;
+    return 0u;
   };
 
   if (r0 < r1) {
     // 32 tiles' places and scales at a time, one per lane; the next 32 are fetched ahead
-    uint32_t grp = NONE, grp_n = NONE;
-    if (r0 + lane < r1) grp = find_tile(r0 + lane);
-    // lane's chunks of a tile: 16 bytes each 512 bytes, and where they go
-    constexpr int NCH = D / 32;
-    uint32_t to[NCH];
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int c = i * 32 + lane;
-      to[i] = chunk_at<D>(c / (D / 16), c % (D / 16));
-    }
+    uint32_t grp = 0, grp_n = 0;
+    bool missing = false;
+    if (r0 + lane < r1) grp = find_tile(r0 + lane, missing);
     const uint32_t ring = smem_u32(smem + Sm::RING + warp * ST * Sm::TILE);
+    const uint32_t bars = smem_u32(smem + Sm::BARS + warp * ST * 8);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < ST; ++i) mbar_init(bars + 8 * i, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
     int put = 0;  // stage that is filled next
     // Start the copies of the tile `j` places into the current 32 (or the next 32's).
     auto issue = [&](int j) {
       const uint32_t g = __shfl_sync(0xffffffffu, j < 32 ? grp : grp_n, j & 31);
-      const uint64_t off = (uint64_t)(g == NONE ? 0u : g) * (16 * D) + lane * 16;
-      const uint32_t dst = ring + put * Sm::TILE;
-#pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        cp_async_16(dst + to[i], a.kc + off + 512 * i);
-        cp_async_16(dst + 16 * D + to[i], a.vc + off + 512 * i);
+      if (lane == 0) {
+        const uint32_t bar = bars + 8 * put, dst = ring + put * Sm::TILE;
+        mbar_arrive_expect_tx(bar, Sm::TILE);
+        tma_load_2d(dst, &tmk, 0, (int)(g * (D / 8)), bar, policy);
+        tma_load_2d(dst + 16 * D, &tmv, 0, (int)(g * (D / 8)), bar, policy);
       }
       put = put + 1 == ST ? 0 : put + 1;
     };
-    // tiles on their way or at hand before each step, which takes one or two (D = 64) and starts as many
-    constexpr int AHEAD = D == 64 ? ST - 2 : ST - 1;
+    int next = r0;  // the tile that is started next
 #pragma unroll
-    for (int b = 0; b < AHEAD; ++b) {
-      if (r0 + b < r1) issue(b);
-      cp_async_commit();
-    }
+    for (int b = 0; b < ST; ++b)
+      if (next < r1) {
+        issue(b);
+        ++next;
+      }
+    // what else the first step needs, all on its way at once: scales, lengths, queries, the next places
+    auto scales_raw = [&](uint32_t group) {
+      float2 x;
+      asm volatile("ld.global.nc.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "l"(a.scale + (group >> gshift)));
+      return x;
+    };
     // a group's key scale and log2 of its value scale (exact for a power of two)
-    auto scales = [&](uint32_t group) {
-      if (group == NONE) return make_float2(0.f, 0.f);
-      float2 x = __ldg(a.scale + (group >> gshift));
+    auto scales = [&](float2 x) {
       const uint32_t bits = __float_as_uint(x.y);
       x.y = (bits & 0x7fffffu) == 0 && bits != 0 ? (float)((int)(bits >> 23) - 127) : log2f(x.y);
       return x;
     };
-    float2 sc = scales(grp), sc_n = sc;
-    uint32_t bad = __ballot_sync(0xffffffffu, grp == NONE);  // places of the current 32 without a block
-    if (r0 + 32 + lane < r1) grp_n = find_tile(r0 + 32 + lane);
-
+    float2 sc = scales_raw(grp), sc_n = make_float2(1.f, 1.f);
     Unit u = unit_at(r0);
-    int j = 0, get = 0;  // the current tile's place in the current 32, and its stage
+    int h0 = 0, nh = 0, ctx = 0;
+    uint4 qraw[NG][KW][2];
+    auto load_q = [&]() {
+      const int kvh = u.k / a.head_groups, hg = u.k - kvh * a.head_groups;
+      h0 = kvh * a.G + hg * HR;
+      nh = min(HR, a.G - hg * HR);
+      asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(ctx) : "l"(a.kv_len + u.seq));
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const int h = 8 * n + g;
+        const T* qp = static_cast<const T*>(a.q) + (int64_t)u.seq * a.q_s0 + (int64_t)(h0 + h) * a.q_s1 + 16 * t4;
+#pragma unroll
+        for (int c = 0; c < KW; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint4& r = qraw[n][c][i];
+            r = make_uint4(0, 0, 0, 0);
+            if (h < nh)
+              asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                           : "l"(qp + 64 * c + 8 * i));
+          }
+      }
+    };
+    load_q();
+    uint32_t bad = __ballot_sync(0xffffffffu, missing);  // places of the current 32 without a block
+    missing = false;
+    if (r0 + 32 + lane < r1) grp_n = find_tile(r0 + 32 + lane, missing);
+    sc = scales(sc);
+
+    int j = 0;           // the current tile's place in the current 32
+    int get = 0;         // its stage, and that one's phase
+    uint32_t phase = 0;
+    bool late = false;   // a bounded wait ran out: what was read is not the cache
     uint32_t qf[NG][KS][2];
     float qs[NG][2];  // per column (heads 2t, 2t + 1): softmax scale, log2 e, the query row's power of two
     float o[NG][MT][4], m[NG][2], l[NG][2];
-    int h0 = 0, nh = 0;
     float R = 0.f;       // log2 of the reference that O is in units of, once a tile has given it
     bool have_r = false;
     bool fresh = true;   // the unit has no maximum yet
     auto begin_unit = [&]() {
-      const int kvh = u.k / a.head_groups, hg = u.k - kvh * a.head_groups;
-      h0 = kvh * a.G + hg * HR;
-      nh = min(HR, a.G - hg * HR);
       R = 0.f;
       have_r = false;
       fresh = true;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const int h = 8 * n + g;
-        const T* qp = static_cast<const T*>(a.q) + (int64_t)u.seq * a.q_s0 + (int64_t)(h0 + h) * a.q_s1;
         float x[KW][16], amax = 0.f;
 #pragma unroll
         for (int c = 0; c < KW; ++c) {
-          uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-          if (h < nh) {
-            raw[0] = __ldg(reinterpret_cast<const uint4*>(qp + 64 * c + 16 * t4));
-            raw[1] = __ldg(reinterpret_cast<const uint4*>(qp + 64 * c + 16 * t4) + 1);
-          }
-          const T* e = reinterpret_cast<const T*>(raw);
+          const T* e = reinterpret_cast<const T*>(qraw[n][c]);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             x[c][i] = to_f32<T>(e[i]);
@@ -415,41 +419,49 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
     begin_unit();
 
     // rows g and g + 8 of K, and rows 2t, 2t + 1, 2t + 8, 2t + 9 of V, in a stage
-    const int tok_g = token_of(g);
-    const uint32_t k_at = chunk_at<D>(tok_g, t4);  // (8 tokens on: + 8 D; 64 columns on: the chunk's bit 2)
+    const int tok_g = token_of<D>(g);
+    const uint32_t k_at = chunk_at<D>(tok_g, t4);  // (64 columns on, at D = 128: bit 6)
     uint32_t v_at[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      v_at[i] = KW == 1 ? chunk_at<D>(token_of(2 * t4 + i), g >> 1) + 8 * (g & 1) : chunk_at<D>(token_of(2 * t4 + i), g);
+      v_at[i] = KW == 1 ? chunk_at<D>(token_of<D>(2 * t4 + i), g >> 1) + 8 * (g & 1) : chunk_at<D>(token_of<D>(2 * t4 + i), g);
     // Tiles [tile, tile + NT) of one unit (their places j and on are in the current 32).
     auto attend = [&](int tile, auto count) {
       constexpr int NT = decltype(count)::value, WR = D / 32;  // WR: words of one V row in this lane
-      cp_async_wait<AHEAD - NT>();  // these tiles are here
-      __syncwarp();                 // for all lanes, and they are done with the tiles before
+      __syncwarp();  // all lanes are done with the tiles before: their stages are free
 #pragma unroll
-      for (int b = 0; b < NT; ++b) {
-        if (tile + AHEAD + b < r1) issue(j + AHEAD + b);
-        cp_async_commit();
-      }
+      for (int b = 0; b < (D == 64 ? 2 : 1); ++b)
+        if (next < r1 && next < tile + ST) {
+          issue(j + next - tile);
+          ++next;
+        }
       uint32_t stage[NT];
-      float ks[NT], ve[NT];
-      bool edge = false;
-      int valid[NT];  // tokens of the tile that count
 #pragma unroll
       for (int b = 0; b < NT; ++b) {
-        stage[b] = (uint32_t)((warp * ST + get) * Sm::TILE);
-        get = get + 1 == ST ? 0 : get + 1;
+        if (!mbar_wait_bounded(bars + 8 * get, phase)) late = true;
+        stage[b] = (uint32_t)(Sm::RING + (warp * ST + get) * Sm::TILE);
+        if (++get == ST) {
+          get = 0;
+          phase ^= 1;
+        }
+      }
+      float ks[NT], ve[NT], rest[NT];
+      bool odd = !have_r;
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
         ks[b] = __shfl_sync(0xffffffffu, sc.x, j + b);
         ve[b] = __shfl_sync(0xffffffffu, sc.y, j + b) - R;
-        valid[b] = (bad >> (j + b)) & 1 ? 0 : u.ctx - (tile + b - u.start) * kFp8Tile;
-        edge |= valid[b] < kFp8Tile;
-      }
-      // value scales that R does not serve
-      float rest[NT];
-#pragma unroll
-      for (int b = 0; b < NT; ++b) {
         rest[b] = 1.f;
-        if (!(ve[b] >= kMinValueExp && ve[b] <= kMaxValueExp) || !have_r) {
+        odd |= !(fabsf(ve[b] - 0.5f * (kMinValueExp + kMaxValueExp)) <= 0.5f * (kMaxValueExp - kMinValueExp));
+      }
+      // the unit's last tile, or places without a block: some tokens do not count
+      const bool edge = tile + NT >= u.end || (bad >> j & ((1u << NT) - 1)) != 0;
+      int valid[NT];
+#pragma unroll
+      for (int b = 0; b < NT; ++b) valid[b] = (bad >> (j + b)) & 1 ? 0 : ctx - (tile + b - u.start) * kFp8Tile;
+      if (odd) {  // value scales that R does not serve
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
           if ((ve[b] > kMaxValueExp || !have_r) && ve[b] > -INFINITY) {  // R moves, and O with it
             const float up = floorf(ve[b]), f = fast_exp2(-up);
             R += up;
@@ -465,11 +477,15 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
             }
             have_r = true;
           }
+        }
+        odd = false;
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
           if (ve[b] < kMinValueExp) {
             rest[b] = fast_exp2(ve[b] - kMinValueExp);
             ve[b] = kMinValueExp;
+            odd = true;
           }
-        }
       }
       // S^T = K Q^T
       float s[NT][NG][4];
@@ -479,8 +495,8 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
         for (int n = 0; n < NG; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.f;
 #pragma unroll
         for (int c = 0; c < KW; ++c) {
-          const uint8_t* p = smem + stage[b] + (k_at ^ (c << 6));
-          const uint4 x4 = *reinterpret_cast<const uint4*>(p), y4 = *reinterpret_cast<const uint4*>(p + 8 * D);
+          const uint4 x4 = *reinterpret_cast<const uint4*>(smem + stage[b] + (k_at ^ (c << 6))),
+                      y4 = *reinterpret_cast<const uint4*>(smem + stage[b] + on8<D>(k_at ^ (c << 6)));
           const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -497,7 +513,7 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
       for (int b = 0; b < NT; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint8_t* p = smem + stage[b] + 16 * D + v_at[i & 1] + (i >> 1) * 8 * D;
+          const uint8_t* p = smem + stage[b] + 16 * D + (i < 2 ? v_at[i] : on8<D>(v_at[i & 1]));
           if constexpr (KW == 1) {
             const uint2 x = *reinterpret_cast<const uint2*>(p);
             v[b][2 * i] = x.x, v[b][2 * i + 1] = x.y;
@@ -572,38 +588,45 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
       }
       if (fresh) fresh = __any_sync(0xffffffffu, m[0][0] == -INFINITY);  // (nothing but bad blocks so far)
       // O^T += V^T P^T; rows past the last token may hold any bits
+      if (edge) {
 #pragma unroll
-      for (int b = 0; b < NT; ++b) {
-        if (edge) {
+        for (int b = 0; b < NT; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (token_of(2 * t4 + (i & 1)) + (i >> 1) * 8 >= valid[b])
+            if (token_of<D>(2 * t4 + (i & 1)) + (i >> 1) * 8 >= valid[b])
 #pragma unroll
               for (int w = 0; w < WR; ++w) v[b][i * WR + w] = 0u;
-        }
-#pragma unroll
-        for (int w = 0; w < WR; ++w) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t sel = half ? 0x7362 : 0x5140;  // bytes (A0 B0 A1 B1) or (A2 B2 A3 B3)
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_to_f16(__byte_perm(v[b][w], v[b][WR + w], sel), a0, a1);
-            e4m3x4_to_f16(__byte_perm(v[b][2 * WR + w], v[b][3 * WR + w], sel), a2, a3);
-            if (rest[b] != 1.f) {
-              const __half2 f = __float2half2_rn(rest[b]);
-              a0 = mul_h2(a0, f), a1 = mul_h2(a1, f), a2 = mul_h2(a2, f), a3 = mul_h2(a3, f);
-            }
-#pragma unroll
-            for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + half], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
-          }
-        }
       }
+      auto values = [&](auto scaled) {
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+          for (int w = 0; w < WR; ++w)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t sel = half ? 0x7362 : 0x5140;  // bytes (A0 B0 A1 B1) or (A2 B2 A3 B3)
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16(__byte_perm(v[b][w], v[b][WR + w], sel), a0, a1);
+              e4m3x4_to_f16(__byte_perm(v[b][2 * WR + w], v[b][3 * WR + w], sel), a2, a3);
+              if constexpr (decltype(scaled)::value) {
+                const __half2 f = __float2half2_rn(rest[b]);
+                a0 = mul_h2(a0, f), a1 = mul_h2(a1, f), a2 = mul_h2(a2, f), a3 = mul_h2(a3, f);
+              }
+#pragma unroll
+              for (int n = 0; n < NG; ++n) mma_f16(o[n][2 * w + half], a0, a1, a2, a3, pb[b][n][0], pb[b][n][1]);
+            }
+      };
+      if (odd)
+        values(std::true_type());
+      else
+        values(std::false_type());
       j += NT;
     };
     for (int tile = r0; tile < r1;) {
       if (tile == u.end) {
         end_unit();
         u = unit_at(tile);
+        load_q();
         begin_unit();
       }
       const int before = j;
@@ -620,53 +643,82 @@ __global__ void __launch_bounds__(Fp8Geo<D, NG>::NW * 32, 1) fp8_decode_kernel(c
         j = 0;
         grp = grp_n;
         sc = sc_n;
-        bad = __ballot_sync(0xffffffffu, grp == NONE);
-        grp_n = NONE;
-        if (tile + 32 + lane < r1) grp_n = find_tile(tile + 32 + lane);
+        bad = __ballot_sync(0xffffffffu, missing);
+        missing = false;
+        grp_n = 0;
+        if (tile + 32 + lane < r1) grp_n = find_tile(tile + 32 + lane, missing);
       } else if (before < 16 && j >= 16) {
-        sc_n = scales(grp_n);
+        sc_n = scales(scales_raw(grp_n));
       }
     }
+    if (late) atomicOr(a.err, MVB_DEV_TIMEOUT);
     __syncwarp();  // the ring has been read, and no copy is on its way: the last piece may lie in it
     end_unit();
   }
   __syncthreads();
 
-  // ---- units cut inside this CTA: candidates w < NW begin in warp w, candidate
-  // NW began in an earlier CTA; one head row per warp and step ----
-  if (tid < 2) a.desc[blockIdx.x * 2 + tid] = make_int4(-1, 0, 0, 0);
+  // ---- units cut inside this CTA: candidate w < NW began in warp w (pieces: its
+  // slot 1, then slot 0 of the warps after it that hold the unit), candidate NW
+  // began in an earlier CTA (pieces: slot 0 from warp 0 on) ----
+  int* list = reinterpret_cast<int*>(pre);  // (the prefix is not needed any more) candidates, their numbers of pieces
+  __shared__ int count;
+  if (warp == 0) {
+    const int4 id = lane < NW ? ids[lane * 2 + 1] : lane == NW ? ids[0] : make_int4(-1, 0, 0, 0);
+    const int first = lane < NW ? lane + 1 : 0;  // slot 0 pieces from here on
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) n += w >= first && ids[w * 2].x == id.x;
+    const uint32_t live = __ballot_sync(0xffffffffu, id.x >= 0);
+    if (id.x >= 0) {
+      const int at = __popc(live & ((1u << lane) - 1));
+      list[2 * at] = lane;
+      list[2 * at + 1] = n;
+    }
+    if (lane == 0) count = __popc(live);
+    if (lane < 2) a.desc[blockIdx.x * 2 + lane] = make_int4(-1, 0, 0, 0);
+  }
   __syncthreads();
-  for (int item = warp; item < (NW + 1) * HR; item += NW) {
-    const int cand = item / HR, h = item - cand * HR;
-    const int4 id = cand < NW ? ids[cand * 2 + 1] : ids[0];
-    if (id.x < 0) continue;
+  // D / 4 threads per head row, four columns each; pieces in warp order
+  constexpr int TPR = D / 4, STEP = NW * 32 / TPR;
+  for (int row = tid / TPR; row < count * HR; row += STEP) {
+    const int at = row / HR, h = row - at * HR, d = (tid % TPR) * 4;
+    const int cand = list[2 * at], n0 = list[2 * at + 1];
+    const bool own = cand < NW;  // it has a slot 1
+    const int4 id = own ? ids[cand * 2 + 1] : ids[0];
     const int kvh = id.z / a.head_groups, hg = id.z - kvh * a.head_groups;
     const int hb = kvh * a.G + hg * HR, n_h = min(HR, a.G - hg * HR);
     if (h >= n_h) continue;
-    // pieces: the first warp's slot 1 (or warp 0's slot 0), then slot 0 of the warps after it
-    const int first = cand < NW ? cand : 0;
-    const int mine = first + lane;  // lane i: warp first + i
-    const bool has = mine < NW && (lane == 0 || ids[mine * 2].x == id.x);
-    const uint32_t mask = __ballot_sync(0xffffffffu, has);
-    const int n = 32 - __clz(mask);
-    auto piece = [&](int i) { return part_of(first + i, i == 0 && cand < NW ? 1 : 0); };
-    float pm = -INFINITY, pl = 0.f;
-    if (has) {
-      const float2 ml = *reinterpret_cast<const float2*>(piece(lane) + HR * D + 2 * h);
-      pm = ml.x;
-      pl = ml.y;
-    }
-    const bool whole = cand < NW && id.w != 0;
-    auto load_o = [&](int i, int d) { return (mask >> i) & 1 ? piece(i)[h * D + d] : 0.f; };
-    if (whole) {
-      T* p = out + (int64_t)id.y * a.o_s0 + (int64_t)(hb + h) * a.o_s1;
-      merge_row<D>(n, pm, pl, true, load_o, [&](int d, float x) { p[d] = from_f32<T>(x); });
+    const float* p1 = part_of(own ? cand : 0, own ? 1 : 0);
+    const float* p0 = part_of(own ? cand + 1 : 0, 0);
+    constexpr int STRIDE = Sm::PIECE / 4;
+    float M = own ? p1[HR * D + 2 * h] : -INFINITY;
+#pragma unroll 4
+    for (int w = 0; w < n0; ++w) M = fmaxf(M, p0[w * STRIDE + HR * D + 2 * h]);
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float* p) {
+      const float2 ml = *reinterpret_cast<const float2*>(p + HR * D + 2 * h);
+      const float4 o = *reinterpret_cast<const float4*>(p + h * D + d);
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+      L = fmaf(w, ml.y, L);
+      acc = make_float4(fmaf(w, o.x, acc.x), fmaf(w, o.y, acc.y), fmaf(w, o.z, acc.z), fmaf(w, o.w, acc.w));
+    };
+    if (own) add(p1);
+#pragma unroll 4
+    for (int w = 0; w < n0; ++w) add(p0 + w * STRIDE);
+    if (own && id.w != 0) {
+      const float f = L == 0.f ? 0.f : 1.f / L;
+      uint2 w;
+      T* e = reinterpret_cast<T*>(&w);
+      e[0] = from_f32<T>(acc.x * f), e[1] = from_f32<T>(acc.y * f);
+      e[2] = from_f32<T>(acc.z * f), e[3] = from_f32<T>(acc.w * f);
+      *reinterpret_cast<uint2*>(out + (int64_t)id.y * a.o_s0 + (int64_t)(hb + h) * a.o_s1 + d) = w;
     } else {
-      const int slot = cand < NW ? 1 : 0;
+      const int slot = own ? 1 : 0;
       float* p = a.part + ((int64_t)blockIdx.x * 2 + slot) * 16 * (D + 2);
-      const float2 ml = merge_row<D>(n, pm, pl, false, load_o, [&](int d, float x) { p[h * D + d] = x; });
-      if (lane == 0) {
-        *reinterpret_cast<float2*>(p + HR * D + 2 * h) = ml;
+      *reinterpret_cast<float4*>(p + h * D + d) = acc;
+      if (d == 0) {
+        *reinterpret_cast<float2*>(p + HR * D + 2 * h) = make_float2(M, L);
         if (h == 0) a.desc[blockIdx.x * 2 + slot] = make_int4(id.x, id.y, hb, n_h);
       }
     }
@@ -756,10 +808,9 @@ int plan_decode(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int
   pl->nw = head_dim == 64 ? (pl->ng == 1 ? Fp8Geo<64, 1>::NW : Fp8Geo<64, 2>::NW)
                           : (pl->ng == 1 ? Fp8Geo<128, 1>::NW : Fp8Geo<128, 2>::NW);
   const int units = num_kv_heads * pl->head_groups;
-  // tile, (block, KV head) and 16-token group numbers are 32-bit
+  // tile and cache row numbers are 32-bit
   if ((int64_t)num_seqs * units * ((int64_t)max_blocks * block_size / kFp8Tile + 1) >= ((int64_t)1 << 31) ||
-      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31) ||
-      (int64_t)num_blocks * num_kv_heads * (block_size / 16) >= 0xffffffffll)
+      (int64_t)num_blocks * num_kv_heads * block_size >= ((int64_t)1 << 31))
     return MVB_ERR_INVALID_ARG;
   pl->grid = decode_grid(num_seqs, units, max_blocks, block_size, pl->nw);
   pl->off_part = ((int64_t)pl->grid * 32 + 255) / 256 * 256;
@@ -767,13 +818,29 @@ int plan_decode(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int
   return MVB_OK;
 }
 
+// A cache of `bytes` bytes as rows of 128, a 16-token tile a box.
+bool cache_map(const void* base, int64_t bytes, int head_dim, CUtensorMap* map) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {128, (cuuint64_t)(bytes / 128)};
+  const cuuint64_t strides[1] = {128};
+  const cuuint32_t box[2] = {128, (cuuint32_t)(kFp8Tile * head_dim / 128)};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, int NG>
 int launch_decode(const Fp8DecodeArgs& a, int grid, cudaStream_t stream) {
+  CUtensorMap tmk, tmv;
+  const int64_t bytes = (((int64_t)a.num_blocks * a.num_kv_heads) << a.block_shift) * D;
+  if (!cache_map(a.kc, bytes, D, &tmk) || !cache_map(a.vc, bytes, D, &tmv)) return MVB_ERR_TENSOR_MAP;
   auto kern = fp8_decode_kernel<T, D, NG>;
   const int smem = Fp8Smem<D, NG>::bytes(a.num_seqs);
   // the largest batch's size at once: the attribute is set on the first call only
   if (ensure_kernel_attrs(kern, Fp8Smem<D, NG>::bytes(kFp8DecodeMaxSeqs)) != cudaSuccess) return MVB_ERR_CUDA;
-  if (launch_pdl(kern, dim3(grid), dim3(Fp8Geo<D, NG>::NW * 32), smem, stream, a) != cudaSuccess) return MVB_ERR_CUDA;
+  if (launch_pdl(kern, dim3(grid), dim3(Fp8Geo<D, NG>::NW * 32), smem, stream, tmk, tmv, a) != cudaSuccess) return MVB_ERR_CUDA;
   if (grid == 1) return MVB_OK;  // no unit is cut between CTAs
   auto merge = fp8_decode_merge_kernel<T, D, 8 * NG>;
   if (ensure_kernel_attrs(merge, 0) != cudaSuccess) return MVB_ERR_CUDA;

@@ -93,12 +93,12 @@ def test_library_checks_without_a_gpu():
         return lib.mvb_paged_decode_fp8(ptr, 64, 64, ptr, ptr, ptr, ptr, 8, maxb, ptr, ptr, 64, 64, seqs, heads, kv, dim,
                                         bs, 100, 0.1, dtype, ws, wsb, ptr, None)
 
-    assert d(0) == _native.OK and d(1) == _native.ERR_INVALID_ARG and d(8193) == _native.ERR_INVALID_ARG
+    assert d(0) == _native.OK and d(1) == _native.ERR_INVALID_ARG and d(6145) == _native.ERR_INVALID_ARG
     assert d(1, heads=15) == _native.ERR_HEADS and d(1, dim=80) == _native.ERR_HEAD_DIM
     assert d(1, bs=8) == _native.ERR_BLOCK_SIZE and d(1, dtype=_native.DTYPE_F32) == _native.ERR_DTYPE
     assert d(1, ptr=4096, maxb=9) == _native.ERR_INVALID_ARG  # the table's rows are shorter
     assert d(1, ptr=8) == _native.ERR_ALIGNMENT and d(1, ptr=4096) == _native.ERR_WORKSPACE
-    assert d(8192, maxb=1 << 26) == _native.ERR_INVALID_ARG  # tile numbers are 32-bit
+    assert d(6144, maxb=1 << 26) == _native.ERR_INVALID_ARG  # tile numbers are 32-bit
     assert lib.mvb_paged_decode_fp8_workspace(256, 14, 2, 64, 16, 100, 128, BF16, ctypes.byref(n)) == _native.OK
     assert n.value >= 148 * 2 * (16 + 8 * 66 * 4)
 
