@@ -20,17 +20,21 @@
 // turns by less than a float32 ulp (low frequencies), and a value beside
 // 448 * 2^k decides about the scale.
 //
-// Work split.  A block's scale needs the maximum over all the call's rows of
-// the block, so one warp owns (block, KV head, keys or values).  It belongs to
-// the CTA of the block's leader: the token that writes the block's lowest slot
-// of the call.  Leaders are found in one of two ways:
-//   * up to kFp8ScanTokens tokens, each token's CTA reads every slot of the
-//     call and keeps the rows of its own block in shared memory: one launch;
+// Work split.  A block's scale needs the maximum over all the call's rows of the
+// block, so its rows belong together, with the CTA of the block's leader: the
+// token that writes the block's lowest slot of the call.  A warp takes one (KV
+// head, keys or values) and all of the block's rows at once, D / 16 lanes a row;
+// where the call writes a single row (a decode step), each D / 16 lanes take a
+// (KV head, keys or values) of their own.  Leaders are found in one of two ways:
+//   * up to kFp8ScanTokens tokens, each token's CTA reads every slot of the call
+//     and keeps the rows of its block in shared memory: one launch;
 //   * more tokens: a first kernel stores writer[slot] = token, and a CTA reads
-//     its block's entries.  An entry is believed only if slot_mapping[entry]
-//     is that slot, so the array needs no initialisation and keeps nothing from
-//     one call to the next.
-// Each token's CTA also rotates the token's query rows.
+//     the entries of its eight tokens' blocks.  An entry is believed only if
+//     slot_mapping[entry] is that slot, so the array needs no initialisation and
+//     keeps nothing from one call to the next.
+// The query rows are rotated by CTAs of their own, behind the others in the same
+// launch or, for many tokens, by a kernel of their own: a thread holds 8 + 8
+// columns of two heads of one token, so the cos and sin rows are read once for two.
 // Bound: memory for long chunks; for a decode step the latency of slots ->
 // rows -> maximum -> codes.
 #include "fp8_common.cuh"
@@ -62,7 +66,7 @@ struct Fp8WriteArgs {
 
 namespace {
 
-constexpr int kFp8ScanTokens = 1024;
+constexpr int kFp8ScanTokens = 2048;
 constexpr int kFp8WriteThreads = 256;
 
 // x c + y s (y the signed partner) rounded once to float32.  16-bit tables: the
@@ -83,49 +87,19 @@ __device__ __forceinline__ float rope_exact(float x, float c, float y, float s) 
   }
 }
 
-// 8 consecutive elements as floats (16-byte aligned for 16-bit types, 32 for float).
+// 4 consecutive elements as floats.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+__device__ __forceinline__ void load4(const T* p, float (&f)[4]) {
   if constexpr (sizeof(T) == 2) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
     const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(e[i]);
+    for (int i = 0; i < 4; ++i) f[i] = to_f32<T>(e[i]);
   } else {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  uint4 r;
-  T* e = reinterpret_cast<T*>(&r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
-  *reinterpret_cast<uint4*>(p) = r;
-}
-
-// Elements [d0, d0 + 8) and [d0 + D/2, d0 + D/2 + 8) of one row, rotated when ROT.
-template <typename T, typename TAB, int D, bool ROT>
-__device__ __forceinline__ void load_row(const T* row, const TAB* cs, const TAB* sn, int d0, float (&lo)[8],
-                                         float (&hi)[8]) {
-  load8<T>(row + d0, lo);
-  load8<T>(row + D / 2 + d0, hi);
-  if constexpr (ROT) {
-    float cl[8], ch[8], sl[8], sh[8];
-    load8<TAB>(cs + d0, cl);
-    load8<TAB>(cs + D / 2 + d0, ch);
-    load8<TAB>(sn + d0, sl);
-    load8<TAB>(sn + D / 2 + d0, sh);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = lo[i], b = hi[i];
-      lo[i] = rope_exact<TAB>(a, cl[i], -b, sl[i]);
-      hi[i] = rope_exact<TAB>(b, ch[i], a, sh[i]);
-    }
-  }
-}
-
 // The token's slot if the token is written at all, else -1.
 template <bool ROT>
 __device__ __forceinline__ int64_t live_slot(const Fp8WriteArgs& a, int64_t total_slots, int t) {
@@ -138,6 +112,18 @@ __device__ __forceinline__ int64_t live_slot(const Fp8WriteArgs& a, int64_t tota
   return s < 0 ? -1 : s;
 }
 
+// What of token t only the device can see to be wrong.
+template <bool ROT>
+__device__ __forceinline__ void flag_token(const Fp8WriteArgs& a, int64_t total_slots, int t) {
+  const int64_t raw = __ldg(a.slots + t);
+  int bad = raw < -1 || raw >= total_slots ? MVB_DEV_SLOT_RANGE : 0;
+  if constexpr (ROT) {
+    const int64_t p = __ldg(a.pos + t);
+    if (p < 0 || p >= a.table_rows) bad |= MVB_DEV_POSITION;
+  }
+  if (bad) atomicOr(a.err, bad);
+}
+
 template <bool ROT>
 __global__ void __launch_bounds__(256) fp8_writer_kernel(const Fp8WriteArgs a) {
   grid_dependency_wait();
@@ -148,177 +134,310 @@ __global__ void __launch_bounds__(256) fp8_writer_kernel(const Fp8WriteArgs a) {
   if (s >= 0) a.writer[s] = t;
 }
 
-template <typename T, typename TAB, int D, bool ROT>
-__global__ void __launch_bounds__(kFp8WriteThreads) fp8_write_kernel(const Fp8WriteArgs a) {
-  extern __shared__ int map[];  // [block_size] the call's token at each slot of this block, -1: none
-  constexpr int LPR = D / 16, RPP = 32 / LPR, NWARP = kFp8WriteThreads / 32;
+
+// Query rows, and key rows where the caller wants them: CTA `cta` of them, HPT
+// rows of one token per thread.  Rounded to 16 bits, they need no exact sum.
+template <typename T, typename TAB, int D, int HPT>
+__device__ __forceinline__ void rotate_rows(const Fp8WriteArgs& a, int cta) {
+  constexpr int LPR = D / 16;
+  const int H = a.num_heads, rows = H + (a.k_out != nullptr ? a.num_kv_heads : 0);
+  const int groups = (rows + HPT - 1) / HPT, d0 = (threadIdx.x % LPR) * 8;
+  const int64_t tg = (int64_t)cta * (kFp8WriteThreads / LPR) + threadIdx.x / LPR;
+  if (tg >= (int64_t)a.num_tokens * groups) return;
+  const int t = (int)(tg / groups), r0 = (int)(tg - (int64_t)t * groups) * HPT;
+  uint4 raw[HPT][2];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int r = min(r0 + i, rows - 1);
+    const T* x = (r < H ? static_cast<const T*>(a.q) + (int64_t)t * a.q_s0 + (int64_t)r * a.q_s1
+                        : static_cast<const T*>(a.k) + (int64_t)t * a.k_s0 + (int64_t)(r - H) * a.k_s1) + d0;
+    // (plain loads: query_out may be query)
+    raw[i][0] = *reinterpret_cast<const uint4*>(x);
+    raw[i][1] = *reinterpret_cast<const uint4*>(x + D / 2);
+  }
+  const int64_t at = __ldg(a.pos + t);
+  if (at < 0 || at >= a.table_rows) return;
+  const TAB *cs = static_cast<const TAB*>(a.cos) + at * D + d0, *sn = static_cast<const TAB*>(a.sin) + at * D + d0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {  // four columns of each half at a time
+    float cl[4], ch[4], sl[4], sh[4];
+    load4<TAB>(cs + 4 * half, cl);
+    load4<TAB>(cs + D / 2 + 4 * half, ch);
+    load4<TAB>(sn + 4 * half, sl);
+    load4<TAB>(sn + D / 2 + 4 * half, sh);
+#pragma unroll
+    for (int i = 0; i < HPT; ++i) {
+      T *x = reinterpret_cast<T*>(&raw[i][0]) + 4 * half, *y = reinterpret_cast<T*>(&raw[i][1]) + 4 * half;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float u = to_f32<T>(x[k]), v = to_f32<T>(y[k]);
+        x[k] = from_f32<T>(__fmaf_rn(u, cl[k], -__fmul_rn(v, sl[k])));
+        y[k] = from_f32<T>(__fmaf_rn(v, ch[k], __fmul_rn(u, sh[k])));
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const int r = r0 + i;
+    if (r >= rows) break;
+    T* dst = (r < H ? static_cast<T*>(a.q_out) + (int64_t)t * a.qo_s0 + (int64_t)r * a.qo_s1
+                    : static_cast<T*>(a.k_out) + ((int64_t)t * a.num_kv_heads + (r - H)) * D) + d0;
+    *reinterpret_cast<uint4*>(dst) = raw[i][0];
+    *reinterpret_cast<uint4*>(dst + D / 2) = raw[i][1];
+  }
+}
+
+template <typename T, typename TAB, int D>
+__global__ void __launch_bounds__(kFp8WriteThreads, 4) fp8_rotate_kernel(const Fp8WriteArgs a) {
   grid_dependency_wait();
   grid_launch_dependents();
-  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int KH = a.num_kv_heads, BS = a.block_size;
-  const int64_t total_slots = (int64_t)a.num_blocks * BS;
-  const int64_t slot = live_slot<ROT>(a, total_slots, t);
-  const int64_t b0 = slot & ~(int64_t)(BS - 1);  // first slot of the block (BS is a power of two)
-  const int off = (int)(slot - b0);
-  if (tid == 0) {
-    const int64_t raw = __ldg(a.slots + t);
-    int bad = raw < -1 || raw >= total_slots ? MVB_DEV_SLOT_RANGE : 0;
-    if constexpr (ROT) {
-      const int64_t p = __ldg(a.pos + t);
-      if (p < 0 || p >= a.table_rows) bad |= MVB_DEV_POSITION;
-    }
-    if (bad) atomicOr(a.err, bad);
-  }
+  rotate_rows<T, TAB, D, 2>(a, blockIdx.x);
+}
 
-  // ---- is this token its block's leader, and which tokens write the block ----
-  bool leader = false;
-  if (slot >= 0) {  // the same for all threads of the CTA
-    bool other;     // some lower slot of the block is written, or this slot by another token
-    if (a.writer == nullptr) {
-      for (int i = tid; i < BS; i += kFp8WriteThreads) map[i] = -1;
-      __syncthreads();
-      for (int u = tid; u < a.num_tokens; u += kFp8WriteThreads) {
-        const int64_t s = live_slot<ROT>(a, total_slots, u);
-        // two tokens of one slot: the later one is written, and the call is flagged
-        if (s >= 0 && (s & ~(int64_t)(BS - 1)) == b0 && atomicMax(map + (s - b0), u) >= 0)
-          atomicOr(a.err, MVB_DEV_DUP_SLOT);
-      }
-      __syncthreads();
-      other = map[off] != t;
-      for (int i = tid; i < off; i += kFp8WriteThreads) other |= map[i] >= 0;
-      leader = __syncthreads_or(other) == 0;
-    } else {
-      // a chunk's next token: its left neighbour writes the slot before it
-      bool next = false;
-      if (off > 0 && t > 0) next = live_slot<ROT>(a, total_slots, t - 1) == slot - 1;
-      other = false;
-      if (tid == 0) {
-        const int w = __ldcg(a.writer + slot);
-        other = w != t;  // this slot's entry is some token's of this call: another one wrote it last
-        if (other) atomicOr(a.err, MVB_DEV_DUP_SLOT);
-      }
-      if (!next) {
-        for (int i = tid; i < BS; i += kFp8WriteThreads) {
-          const int w = __ldcg(a.writer + b0 + i);
-          const bool ok = w >= 0 && w < a.num_tokens && live_slot<ROT>(a, total_slots, w) == b0 + i;
-          map[i] = ok ? w : -1;
-          other |= ok && i < off;
-        }
-      }
-      leader = __syncthreads_or(other || next) == 0;
+// One block's rows: the call's token at each of its slots is in map (-1: none).
+template <typename T, typename TAB, int D, bool ROT>
+__device__ __forceinline__ void write_block(const Fp8WriteArgs& a, const int* map, int64_t b0) {
+  constexpr int LPR = D / 16, RPP = 32 / LPR, NWARP = kFp8WriteThreads / 32, NP = 16 / RPP;  // NP: passes at once
+  const int KH = a.num_kv_heads, BS = a.block_size, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane % LPR, place = lane / LPR, d0 = sub * 8;
+  int rows = 0, only = 0;  // rows of the call, the last of them
+  for (int r = lane; r < BS; r += 32)
+    if (map[r] >= 0) {
+      ++rows;
+      only = r;
     }
-  }
-
-  // ---- the block's rows: one warp per (KV head, keys / values) ----
-  const int kv_items = leader ? 2 * KH : 0;
-  for (int it = warp; it < kv_items; it += NWARP) {
-    const int kvh = it >> 1, which = it & 1;
+  rows = __reduce_add_sync(0xffffffffu, rows);
+  only = __reduce_max_sync(0xffffffffu, only);
+  const bool single = rows == 1;  // each place of a warp has a (KV head, keys / values) of its own
+  const int items = 2 * KH, per = single ? RPP : 1;
+  for (int i0 = warp * per; i0 < items; i0 += NWARP * per) {
+    const int it = single ? i0 + place : i0;
+    const bool live = it < items;
+    const int which = it < KH ? 0 : 1, kvh = live ? it - which * KH : 0;  // (keys, which are rotated, first)
     const int64_t bh = (b0 / BS) * KH + kvh;
     float* sp = a.scale + bh * 2 + which;
     const float old = map[0] >= 0 ? 0.f : *sp;
-    const float base = old > 0.f && old < INFINITY ? old : 0.f;  // not a scale yet (or never): nothing to keep
     uint8_t* codes = (which ? a.vc : a.kc) + bh * BS * D;
     const T* src = static_cast<const T*>(which ? a.v : a.k);
     const int64_t s0 = which ? a.v_s0 : a.k_s0;
-    src += (int64_t)kvh * (which ? a.v_s1 : a.k_s1);
-    const int d0 = (lane % LPR) * 8;
-    const TAB* cs = static_cast<const TAB*>(a.cos);
-    const TAB* sn = static_cast<const TAB*>(a.sin);
-    auto row = [&](int r, float (&lo)[8], float (&hi)[8]) {
-      const int u = map[r];
-      if (u < 0) return false;
-      const T* p = src + (int64_t)u * s0;
-      if (ROT && which == 0) {
-        const int64_t at = __ldg(a.pos + u) * D;
-        load_row<T, TAB, D, ROT>(p, cs + at, sn + at, d0, lo, hi);
-      } else {
-        load_row<T, TAB, D, false>(p, cs, sn, d0, lo, hi);
+    src += (int64_t)kvh * (which ? a.v_s1 : a.k_s1) + d0;
+    // rows r0 + p RPP + place (or the only one) and their table rows
+    uint4 raw[NP][2];
+    int at[NP], pos[NP];
+    auto load_rows = [&](int r0) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const int r = single ? (p == 0 ? only : BS) : r0 + p * RPP + place;
+        const int u = r < BS && live ? map[r] : -1;
+        at[p] = u >= 0 ? r : -1;
+        if (u < 0) continue;
+        raw[p][0] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)u * s0));
+        raw[p][1] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)u * s0 + D / 2));
+        if (ROT && which == 0) pos[p] = (int)__ldg(a.pos + u);
       }
-      return true;
+    };
+    // pass p's row as float32, rotated: four columns of the lower and of the upper half at a time (rotated again where
+    // it is coded: sixteen float32 values a row in registers spilled)
+    auto row = [&](int p, auto use) {
+      const T *x = reinterpret_cast<const T*>(&raw[p][0]), *y = reinterpret_cast<const T*>(&raw[p][1]);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = to_f32<T>(x[4 * half + i]);
+          hi[i] = to_f32<T>(y[4 * half + i]);
+        }
+        if (ROT && which == 0) {
+          const int64_t o = (int64_t)pos[p] * D + d0 + 4 * half;
+          const TAB *cs = static_cast<const TAB*>(a.cos) + o, *sn = static_cast<const TAB*>(a.sin) + o;
+          float cl[4], ch[4], sl[4], sh[4];
+          load4<TAB>(cs, cl);
+          load4<TAB>(cs + D / 2, ch);
+          load4<TAB>(sn, sl);
+          load4<TAB>(sn + D / 2, sh);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float u = lo[i], v = hi[i];
+            lo[i] = rope_exact<TAB>(u, cl[i], -v, sl[i]);
+            hi[i] = rope_exact<TAB>(v, ch[i], u, sh[i]);
+          }
+        }
+        use(half, lo, hi);
+      }
     };
     float amax = 0.f;
-    for (int r = lane / LPR; r < BS; r += RPP) {
-      float lo[8], hi[8];
-      if (!row(r, lo, hi)) continue;
+    for (int r0 = 0; r0 < BS; r0 += NP * RPP) {
+      load_rows(r0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = fabsf(lo[i]), y = fabsf(hi[i]);
-        amax = fmaxf(amax, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+      for (int p = 0; p < NP; ++p) {
+        if (at[p] < 0) continue;
+        row(p, [&](int, const float (&lo)[4], const float (&hi)[4]) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = fabsf(lo[i]), y = fabsf(hi[i]);
+            amax = fmaxf(amax, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+          }
+        });
       }
+      if (single) break;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = 1; o < LPR; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (!single) {
+#pragma unroll
+      for (int o = LPR; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
+    const float base = old > 0.f && old < INFINITY ? old : 0.f;  // not a scale yet (or never): nothing to keep
     const float s = fmaxf(base, fp8_scale_for(amax));
-    if (base > 0.f && s > base) {  // the scale has grown: the rows already there, 16 codes a lane
+    if (live && base > 0.f && s > base) {  // the scale has grown: the rows already there, 16 codes a lane
       const float ratio = __fdiv_rn(base, s);
-      for (int c = lane; c < BS * (D / 16); c += 32) {
-        if (map[c / (D / 16)] >= 0) continue;
-        uint4* p = reinterpret_cast<uint4*>(codes) + c;
+#pragma unroll 4
+      for (int r = single ? 0 : place; r < BS; r += single ? 1 : RPP) {
+        if (map[r] >= 0) continue;
+        uint4* p = reinterpret_cast<uint4*>(codes + (int64_t)r * D) + sub;
         uint4 w = *p;
         uint32_t* e = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t lo, hi;
-          e4m3x4_to_f16(e[i], lo, hi);
-          const float2 x = __half22float2(*reinterpret_cast<__half2*>(&lo));
-          const float2 y = __half22float2(*reinterpret_cast<__half2*>(&hi));
+          uint32_t l, h;
+          e4m3x4_to_f16(e[i], l, h);
+          const float2 x = __half22float2(*reinterpret_cast<__half2*>(&l));
+          const float2 y = __half22float2(*reinterpret_cast<__half2*>(&h));
           e[i] = f32x4_to_e4m3(x.x * ratio, x.y * ratio, y.x * ratio, y.y * ratio);
         }
         *p = w;
       }
     }
     const float inv = __frcp_rn(s);
-    for (int r = lane / LPR; r < BS; r += RPP) {
-      float lo[8], hi[8];
-      if (!row(r, lo, hi)) continue;
-      uint2 l, h;
-      l.x = f32x4_to_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv);
-      l.y = f32x4_to_e4m3(lo[4] * inv, lo[5] * inv, lo[6] * inv, lo[7] * inv);
-      h.x = f32x4_to_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv);
-      h.y = f32x4_to_e4m3(hi[4] * inv, hi[5] * inv, hi[6] * inv, hi[7] * inv);
-      uint8_t* p = codes + (int64_t)r * D + d0;
-      *reinterpret_cast<uint2*>(p) = l;
-      *reinterpret_cast<uint2*>(p + D / 2) = h;
+    for (int r0 = 0; r0 < BS; r0 += NP * RPP) {
+      if (!single && BS > NP * RPP) load_rows(r0);  // (else they are still at hand)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        if (at[p] < 0) continue;
+        uint2 l, h;
+        row(p, [&](int half, const float (&lo)[4], const float (&hi)[4]) {
+          (half ? l.y : l.x) = f32x4_to_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv);
+          (half ? h.y : h.x) = f32x4_to_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv);
+        });
+        uint8_t* to = codes + (int64_t)at[p] * D + d0;
+        *reinterpret_cast<uint2*>(to) = l;
+        *reinterpret_cast<uint2*>(to + D / 2) = h;
+      }
+      if (single) break;
     }
-    __syncwarp();
-    if (lane == 0) *sp = s;
+    __syncwarp();  // all lanes have read the old scale
+    if (live && sub == 0 && (single || place == 0)) *sp = s;
   }
+}
 
-  // ---- this token's query rows, and its key rows where the caller wants them ----
+// Up to kFp8ScanTokens tokens: CTA t < num_tokens takes token t's block if the token is its leader, the CTAs behind
+// them rotate the query rows.
+template <typename T, typename TAB, int D, bool ROT>
+__global__ void __launch_bounds__(kFp8WriteThreads, 2) fp8_write_kernel(const Fp8WriteArgs a) {
+  extern __shared__ int map[];  // [block_size]
+  grid_dependency_wait();
+  grid_launch_dependents();
   if constexpr (ROT) {
-    const int64_t p = __ldg(a.pos + t);
-    if (p < 0 || p >= a.table_rows) return;
-    const TAB* cs = static_cast<const TAB*>(a.cos) + p * D;
-    const TAB* sn = static_cast<const TAB*>(a.sin) + p * D;
-    const int H = a.num_heads, rows = H + (a.k_out != nullptr ? KH : 0);
-    // warps take these from the last one down: the first ones may still be at the block's rows
-    for (int it = (NWARP - 1 - warp) * 32 + lane; it < rows * LPR; it += kFp8WriteThreads) {
-      const int r = it / LPR, d0 = (it - r * LPR) * 8;
-      const T* src = r < H ? static_cast<const T*>(a.q) + (int64_t)t * a.q_s0 + (int64_t)r * a.q_s1
-                           : static_cast<const T*>(a.k) + (int64_t)t * a.k_s0 + (int64_t)(r - H) * a.k_s1;
-      T* dst = r < H ? static_cast<T*>(a.q_out) + (int64_t)t * a.qo_s0 + (int64_t)r * a.qo_s1
-                     : static_cast<T*>(a.k_out) + ((int64_t)t * KH + (r - H)) * D;
-      float lo[8], hi[8];
-      load_row<T, TAB, D, true>(src, cs, sn, d0, lo, hi);
-      store8<T>(dst + d0, lo);
-      store8<T>(dst + D / 2 + d0, hi);
+    if ((int)blockIdx.x >= a.num_tokens) {
+      rotate_rows<T, TAB, D, 2>(a, (int)blockIdx.x - a.num_tokens);
+      return;
     }
+  }
+  const int t = blockIdx.x, tid = threadIdx.x, BS = a.block_size;
+  const int64_t total_slots = (int64_t)a.num_blocks * BS;
+  const int64_t slot = live_slot<ROT>(a, total_slots, t);
+  const int64_t b0 = slot & ~(int64_t)(BS - 1);  // first slot of the block (BS is a power of two)
+  const int off = (int)(slot - b0);
+  if (tid == 0) flag_token<ROT>(a, total_slots, t);
+  if (slot < 0) return;  // the same for all threads of the CTA
+  for (int i = tid; i < BS; i += kFp8WriteThreads) map[i] = -1;
+  __syncthreads();
+  for (int u = tid; u < a.num_tokens; u += kFp8WriteThreads) {
+    const int64_t s = live_slot<ROT>(a, total_slots, u);
+    // two tokens of one slot: the later one is written, and the call is flagged
+    if (s >= 0 && (s & ~(int64_t)(BS - 1)) == b0 && atomicMax(map + (s - b0), u) >= 0)
+      atomicOr(a.err, MVB_DEV_DUP_SLOT);
+  }
+  __syncthreads();
+  bool other = map[off] != t;  // some lower slot of the block is written, or this slot by another token
+  for (int i = tid; i < off; i += kFp8WriteThreads) other |= map[i] >= 0;
+  if (__syncthreads_or(other)) return;
+  write_block<T, TAB, D, ROT>(a, map, b0);
+}
+
+// More tokens, behind fp8_writer_kernel: kFp8Chunk tokens a CTA.
+constexpr int kFp8Chunk = 8;
+template <typename T, typename TAB, int D, bool ROT>
+__global__ void __launch_bounds__(kFp8WriteThreads, 2) fp8_write_many_kernel(const Fp8WriteArgs a) {
+  extern __shared__ int map[];  // [block_size]
+  __shared__ int64_t slots[kFp8Chunk];  // -1: not a leader
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x, BS = a.block_size;
+  const int64_t total_slots = (int64_t)a.num_blocks * BS;
+  if (tid < kFp8Chunk) {
+    const int t = blockIdx.x * kFp8Chunk + tid;
+    int64_t slot = -1;
+    if (t < a.num_tokens) {
+      flag_token<ROT>(a, total_slots, t);
+      slot = live_slot<ROT>(a, total_slots, t);
+      if (slot >= 0) {
+        // this slot's entry is some token's of this call: if another's, that one wrote it last
+        const bool dup = __ldcg(a.writer + slot) != t;
+        if (dup) atomicOr(a.err, MVB_DEV_DUP_SLOT);
+        // a chunk's next token: its left neighbour writes the slot before it
+        if (dup || ((slot & (BS - 1)) != 0 && t > 0 && live_slot<ROT>(a, total_slots, t - 1) == slot - 1)) slot = -1;
+      }
+    }
+    slots[tid] = slot;
+  }
+  __syncthreads();
+  for (int k = 0; k < kFp8Chunk; ++k) {
+    const int64_t slot = slots[k];
+    if (slot < 0) continue;  // the same for all threads of the CTA
+    const int64_t b0 = slot & ~(int64_t)(BS - 1);
+    bool other = false;  // some lower slot of the block is written
+    for (int i = tid; i < BS; i += kFp8WriteThreads) {
+      const int w = __ldcg(a.writer + b0 + i);
+      const bool ok = w >= 0 && w < a.num_tokens && live_slot<ROT>(a, total_slots, w) == b0 + i;
+      map[i] = ok ? w : -1;
+      other |= ok && b0 + i < slot;
+    }
+    if (!__syncthreads_or(other)) write_block<T, TAB, D, ROT>(a, map, b0);
+    __syncthreads();
   }
 }
 
 template <typename T, typename TAB, int D, bool ROT>
 int launch_write(const Fp8WriteArgs& a, cudaStream_t stream) {
-  auto kern = fp8_write_kernel<T, TAB, D, ROT>;
-  if (ensure_kernel_attrs(kern, a.block_size * 4) != cudaSuccess) return MVB_ERR_CUDA;
-  if (a.writer != nullptr) {
-    auto first = fp8_writer_kernel<ROT>;
-    if (ensure_kernel_attrs(first, 0) != cudaSuccess) return MVB_ERR_CUDA;
-    if (launch_pdl(first, dim3((a.num_tokens + 255) / 256), dim3(256), 0, stream, a) != cudaSuccess)
+  const int smem = a.block_size * 4;
+  const int rows = a.num_heads + (a.k_out != nullptr ? a.num_kv_heads : 0);
+  const int64_t fill = ((int64_t)a.num_tokens * ((rows + 1) / 2) * (D / 16) + kFp8WriteThreads - 1) / kFp8WriteThreads;
+  const int64_t rotate_ctas = ROT ? fill : 0;
+  if (a.num_tokens + rotate_ctas >= ((int64_t)1 << 31)) return MVB_ERR_INVALID_ARG;
+  if (a.writer == nullptr) {
+    auto kern = fp8_write_kernel<T, TAB, D, ROT>;
+    if (ensure_kernel_attrs(kern, smem) != cudaSuccess) return MVB_ERR_CUDA;
+    return launch_pdl(kern, dim3((unsigned)(a.num_tokens + rotate_ctas)), dim3(kFp8WriteThreads), smem, stream, a) ==
+                   cudaSuccess
+               ? MVB_OK
+               : MVB_ERR_CUDA;
+  }
+  auto first = fp8_writer_kernel<ROT>;
+  auto kern = fp8_write_many_kernel<T, TAB, D, ROT>;
+  if (ensure_kernel_attrs(first, 0) != cudaSuccess || ensure_kernel_attrs(kern, smem) != cudaSuccess) return MVB_ERR_CUDA;
+  if (launch_pdl(first, dim3((a.num_tokens + 255) / 256), dim3(256), 0, stream, a) != cudaSuccess) return MVB_ERR_CUDA;
+  if (launch_pdl(kern, dim3((a.num_tokens + kFp8Chunk - 1) / kFp8Chunk), dim3(kFp8WriteThreads), smem, stream, a) !=
+      cudaSuccess)
+    return MVB_ERR_CUDA;
+  if constexpr (ROT) {
+    auto rotate = fp8_rotate_kernel<T, TAB, D>;
+    if (ensure_kernel_attrs(rotate, 0) != cudaSuccess) return MVB_ERR_CUDA;
+    if (launch_pdl(rotate, dim3((unsigned)rotate_ctas), dim3(kFp8WriteThreads), 0, stream, a) != cudaSuccess)
       return MVB_ERR_CUDA;
   }
-  return launch_pdl(kern, dim3(a.num_tokens), dim3(kFp8WriteThreads), a.block_size * 4, stream, a) == cudaSuccess
-             ? MVB_OK
-             : MVB_ERR_CUDA;
+  return MVB_OK;
 }
 
 template <typename T>
@@ -345,6 +464,7 @@ int write_fp8(Fp8WriteArgs a, int head_dim, int dtype, int table_dtype, void* wo
   if (!al(a.k, 16) || !al(a.v, 16) || !al(a.kc, 16) || !al(a.vc, 16) || !al(a.scale, 4) || !al_s(a.k_s0) ||
       !al_s(a.k_s1) || !al_s(a.v_s0) || !al_s(a.v_s1) || !al(a.k_out, 16))
     return MVB_ERR_ALIGNMENT;
+  if (a.pos != nullptr && a.table_rows >= ((int64_t)1 << 31)) return MVB_ERR_INVALID_ARG;
   if (a.pos != nullptr &&
       (!al(a.q, 16) || !al(a.q_out, 16) || !al(a.cos, 16) || !al(a.sin, 16) || !al_s(a.q_s0) || !al_s(a.q_s1) ||
        !al_s(a.qo_s0) || !al_s(a.qo_s1)))

@@ -85,9 +85,9 @@ def test_library_checks_without_a_gpu():
     assert w(1, bs=8) == _native.ERR_BLOCK_SIZE and w(1, bs=24) == _native.ERR_BLOCK_SIZE
     assert w(1, d=32) == _native.ERR_HEAD_DIM and w(1, dtype=_native.DTYPE_F32) == _native.ERR_DTYPE
     assert w(1, ptr=8) == _native.ERR_ALIGNMENT and w(5000, ptr=4096) == _native.ERR_WORKSPACE
-    assert lib.mvb_kv_cache_write_fp8_workspace(1024, 10, 16, ctypes.byref(n)) == _native.OK and n.value == 0
-    assert lib.mvb_kv_cache_write_fp8_workspace(1025, 10, 16, ctypes.byref(n)) == _native.OK and n.value == 640
-    assert lib.mvb_kv_cache_write_fp8_workspace(1025, 0, 16, ctypes.byref(n)) == _native.ERR_INVALID_ARG
+    assert lib.mvb_kv_cache_write_fp8_workspace(2048, 10, 16, ctypes.byref(n)) == _native.OK and n.value == 0
+    assert lib.mvb_kv_cache_write_fp8_workspace(2049, 10, 16, ctypes.byref(n)) == _native.OK and n.value == 640
+    assert lib.mvb_kv_cache_write_fp8_workspace(2049, 0, 16, ctypes.byref(n)) == _native.ERR_INVALID_ARG
 
     def d(seqs, heads=14, kv=2, dim=64, bs=16, maxb=8, dtype=BF16, ptr=None, ws=None, wsb=0):
         return lib.mvb_paged_decode_fp8(ptr, 64, 64, ptr, ptr, ptr, ptr, 8, maxb, ptr, ptr, 64, 64, seqs, heads, kv, dim,

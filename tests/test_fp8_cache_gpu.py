@@ -74,10 +74,12 @@ def write_case(g, tokens, heads, dtype, table_dtype, rows=512):
 
 
 def check_write(heads, bs, dtype, table_dtype, slots, num_blocks, seed=0, calls=1):
-    """`calls` writes into one cache, each of new rows into `slots`; everything compared bit for bit.
+    """`calls` writes into one cache, each of new rows into `slots`; the cache is compared bit for bit.
 
-    The model rounds the exact rotation to float32 once, as the kernel does up to a float32 rounding in
-    about 2^25, and every further step is exact or the same rounding."""
+    The model rounds the exact rotation to float32 once, as the kernel does for the keys it codes up to a
+    float32 rounding in about 2^25, and every further step is exact or the same rounding.  Query rows and
+    returned keys are a product and a fused multiply-add in float32 (two roundings, of terms that add up to
+    at most |x c| + |y s|), rounded to 16 bits."""
     g = gen(seed)
     H, KH, D = heads
     kc, vc, sc = make_cache(g, num_blocks, KH, bs, D)
@@ -87,7 +89,11 @@ def check_write(heads, bs, dtype, table_dtype, slots, num_blocks, seed=0, calls=
         q, k, v, pos, cos, sin = write_case(g, len(slots), heads, dtype, table_dtype)
         qo, ko = M.rope_cache_write_fp8(q, k, v, pos, cos, sin, kc, vc, sc, slots, bs, return_key=True)
         rq, rk = (F.rotate(x, cos, sin, pos) for x in (q, k))
-        assert torch.equal(qo, rq.to(dtype)) and torch.equal(ko, rk.to(dtype))
+        for got, ref, x in ((qo, rq, q), (ko, rk, k)):
+            ref, terms = ref.double(), F.rotate(x.abs(), cos.abs(), -sin.abs(), pos).abs().double()
+            terms = torch.maximum(terms, F.rotate(x.abs(), cos.abs(), sin.abs(), pos).abs().double())
+            limit = F.UNIT[dtype] * ref.abs() + 2.0 ** -22 * terms + 2.0 ** -25
+            assert ((got.double() - ref).abs() <= limit).all()
         F.write(rk.cpu(), v.float().cpu(), mk, mv, ms, slots.cpu(), bs)
     assert torch.equal(sc.cpu(), ms)
     assert torch.equal(bits(kc).cpu(), bits(mk)) and torch.equal(bits(vc).cpu(), bits(mv))
@@ -114,12 +120,13 @@ def test_write_block_sizes_and_orders(bs, tokens):
 
 @pytest.mark.parametrize("shuffled", [False, True])
 def test_write_many_tokens(shuffled):
-    """Past the size up to which a token's CTA looks at every slot (1024)."""
+    """Past the size up to which a token's CTA looks at every slot (2048)."""
     r = np.random.RandomState(3)
-    slots = np.concatenate([np.arange(7, 900), np.arange(1024, 1500), np.full(9, -1)])
+    slots = np.concatenate([np.arange(7, 1900), np.arange(2048, 2500), np.full(9, -1)])
     if shuffled:
         r.shuffle(slots)
-    check_write((14, 2, 64), 16, torch.bfloat16, torch.float32, slots, 100, calls=2)
+    check_write((14, 2, 64), 16, torch.bfloat16, torch.float32, slots, 160, calls=2)
+    check_write((8, 8, 128), 64, torch.float16, torch.float16, slots, 40, calls=2)
 
 
 def test_write_token_by_token_is_the_write_at_once():
@@ -157,6 +164,14 @@ def test_write_zeros_infinities_and_nan():
     assert torch.equal(sc.cpu(), ms) and torch.equal(bits(kc).cpu(), bits(mk)) and torch.equal(bits(vc).cpu(), bits(mv))
     assert sc[0, 0, 0] == 2.0 ** -100 and torch.isnan(kc.float()[0, 0, 1, 5])
     assert kc.float()[0, 0, 1, 3] == 448 and kc.float()[0, 0, 1, 4] == -448
+
+
+@pytest.mark.parametrize("tokens", [1, 700, 2200])
+def test_write_one_row_per_block(tokens):
+    """A decode step: every block has one new row, in any place."""
+    r = np.random.RandomState(tokens)
+    slots = r.permutation(tokens) * 16 + r.randint(0, 16, tokens)
+    check_write((32, 8, 128), 16, torch.bfloat16, torch.bfloat16, slots, tokens, calls=2)
 
 
 def test_write_border_of_a_scale():
@@ -203,7 +218,7 @@ def test_write_strides_in_place_and_other_dtypes_of_indices():
 def test_write_device_errors():
     bs, KH, D = 16, 2, 64
     for many in (False, True):
-        n = 1100 if many else 3
+        n = 2100 if many else 3
         cache = make_cache(gen(8), 100, KH, bs, D)
         k = torch.ones(n, KH, D, device=DEV).half()
         slots = torch.full((n,), -1, dtype=torch.int64, device=DEV)
@@ -522,7 +537,7 @@ def test_captured_calls_and_two_streams():
 
 def test_captured_writes_with_new_rows():
     """A captured write replayed with other rows, slots and positions in the same tensors; many tokens too."""
-    for T in (30, 1500):
+    for T in (30, 2500):
         g = gen(22)
         bs, heads = 16, (14, 2, 64)
         num_blocks = 2 * T // bs + 2
