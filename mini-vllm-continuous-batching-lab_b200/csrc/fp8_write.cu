@@ -15,10 +15,12 @@
 // holds does not depend on how its tokens were split into calls but for those.
 // The maximum runs over the finite elements; an infinity is stored as +-448 s.
 //
-// A rotated key is the exact rotation x cos + rot(x) sin rounded once to
-// float32 (rope_exact): the largest value of a block is often a coordinate that
-// turns by less than a float32 ulp (low frequencies), and a value beside
-// 448 * 2^k decides about the scale.
+// A rotated row is a product and a fused multiply-add in float32: the exact
+// rotation rounded once but for the product's rounding, which matters only beside
+// a tie (about one code in 2^20 differs from the exact rotation's).  A maximum
+// within 4 ulps of 448 * 2^k decides about a scale, so there it is taken again
+// from exact sums (rope_exact); sums exact everywhere were half of the kernel's
+// instructions.
 //
 // Work split.  A block's scale needs the maximum over all the call's rows of the
 // block, so its rows belong together, with the CTA of the block's leader: the
@@ -37,6 +39,8 @@
 // columns of two heads of one token, so the cos and sin rows are read once for two.
 // Bound: memory for long chunks; for a decode step the latency of slots ->
 // rows -> maximum -> codes.
+#include <type_traits>
+
 #include "fp8_common.cuh"
 
 namespace mvb {
@@ -69,22 +73,20 @@ namespace {
 constexpr int kFp8ScanTokens = 2048;
 constexpr int kFp8WriteThreads = 256;
 
-// x c + y s (y the signed partner) rounded once to float32.  16-bit tables: the
-// product of two 16-bit floats is exact in float32, one fma rounds the sum.
-// float32 tables: the products and the sum with their rounding errors (exact by
-// fma and by Knuth's two-sum), added back at the end.
-template <typename TAB>
-__device__ __forceinline__ float rope_exact(float x, float c, float y, float s) {
-  if constexpr (sizeof(TAB) == 2) {
-    return __fmaf_rn(x, c, __fmul_rn(y, s));
-  } else {
-    const float p1 = __fmul_rn(x, c), e1 = __fmaf_rn(x, c, -p1);
-    const float p2 = __fmul_rn(y, s), e2 = __fmaf_rn(y, s, -p2);
-    const float t = __fadd_rn(p1, p2);
-    const float b = __fsub_rn(t, p1);
-    const float e3 = __fadd_rn(__fsub_rn(p1, __fsub_rn(t, b)), __fsub_rn(p2, b));
-    return __fadd_rn(t, __fadd_rn(e3, __fadd_rn(e1, e2)));
-  }
+// x c + y s, y the signed partner.  With 16-bit tables the product of two 16-bit
+// floats is exact, and this is the exact rotation rounded once.
+__device__ __forceinline__ float rope(float x, float c, float y, float s) {
+  return __fmaf_rn(x, c, __fmul_rn(y, s));
+}
+// The same rounded once for float32 tables: the products and the sum with their
+// rounding errors (exact by fma and by Knuth's two-sum), added back at the end.
+__device__ __noinline__ float rope_exact(float x, float c, float y, float s) {
+  const float p1 = __fmul_rn(x, c), e1 = __fmaf_rn(x, c, -p1);
+  const float p2 = __fmul_rn(y, s), e2 = __fmaf_rn(y, s, -p2);
+  const float t = __fadd_rn(p1, p2);
+  const float b = __fsub_rn(t, p1);
+  const float e3 = __fadd_rn(__fsub_rn(p1, __fsub_rn(t, b)), __fsub_rn(p2, b));
+  return __fadd_rn(t, __fadd_rn(e3, __fadd_rn(e1, e2)));
 }
 
 // 4 consecutive elements as floats.
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(256) fp8_writer_kernel(const Fp8WriteArgs a) {
 
 
 // Query rows, and key rows where the caller wants them: CTA `cta` of them, HPT
-// rows of one token per thread.  Rounded to 16 bits, they need no exact sum.
+// rows of one token per thread.
 template <typename T, typename TAB, int D, int HPT>
 __device__ __forceinline__ void rotate_rows(const Fp8WriteArgs& a, int cta) {
   constexpr int LPR = D / 16;
@@ -171,8 +173,8 @@ __device__ __forceinline__ void rotate_rows(const Fp8WriteArgs& a, int cta) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float u = to_f32<T>(x[k]), v = to_f32<T>(y[k]);
-        x[k] = from_f32<T>(__fmaf_rn(u, cl[k], -__fmul_rn(v, sl[k])));
-        y[k] = from_f32<T>(__fmaf_rn(v, ch[k], __fmul_rn(u, sh[k])));
+        x[k] = from_f32<T>(rope(u, cl[k], -v, sl[k]));
+        y[k] = from_f32<T>(rope(v, ch[k], u, sh[k]));
       }
     }
   }
@@ -238,7 +240,7 @@ __device__ __forceinline__ void write_block(const Fp8WriteArgs& a, const int* ma
     };
     // pass p's row as float32, rotated: four columns of the lower and of the upper half at a time (rotated again where
     // it is coded: sixteen float32 values a row in registers spilled)
-    auto row = [&](int p, auto use) {
+    auto row = [&](int p, auto exact, auto use) {
       const T *x = reinterpret_cast<const T*>(&raw[p][0]), *y = reinterpret_cast<const T*>(&raw[p][1]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -259,34 +261,49 @@ __device__ __forceinline__ void write_block(const Fp8WriteArgs& a, const int* ma
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float u = lo[i], v = hi[i];
-            lo[i] = rope_exact<TAB>(u, cl[i], -v, sl[i]);
-            hi[i] = rope_exact<TAB>(v, ch[i], u, sh[i]);
+            if constexpr (decltype(exact)::value) {
+              lo[i] = rope_exact(u, cl[i], -v, sl[i]);
+              hi[i] = rope_exact(v, ch[i], u, sh[i]);
+            } else {
+              lo[i] = rope(u, cl[i], -v, sl[i]);
+              hi[i] = rope(v, ch[i], u, sh[i]);
+            }
           }
         }
         use(half, lo, hi);
       }
     };
-    float amax = 0.f;
-    for (int r0 = 0; r0 < BS; r0 += NP * RPP) {
-      load_rows(r0);
+    // the largest finite magnitude of this (KV head, keys / values)
+    auto largest = [&](auto exact) {
+      float amax = 0.f;
+      for (int r0 = 0; r0 < BS; r0 += NP * RPP) {
+        if (!decltype(exact)::value || BS > NP * RPP) load_rows(r0);  // (else they are still at hand)
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        if (at[p] < 0) continue;
-        row(p, [&](int, const float (&lo)[4], const float (&hi)[4]) {
+        for (int p = 0; p < NP; ++p) {
+          if (at[p] < 0) continue;
+          row(p, exact, [&](int, const float (&lo)[4], const float (&hi)[4]) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = fabsf(lo[i]), y = fabsf(hi[i]);
-            amax = fmaxf(amax, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
-          }
-        });
+            for (int i = 0; i < 4; ++i) {
+              const float x = fabsf(lo[i]), y = fabsf(hi[i]);
+              amax = fmaxf(amax, fmaxf(x < INFINITY ? x : 0.f, y < INFINITY ? y : 0.f));
+            }
+          });
+        }
+        if (single) break;
       }
-      if (single) break;
-    }
 #pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!single) {
+      for (int o = 1; o < LPR; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (!single) {
 #pragma unroll
-      for (int o = LPR; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = LPR; o < 32; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      }
+      return amax;
+    };
+    float amax = largest(std::false_type());
+    if constexpr (ROT && sizeof(TAB) == 4) {
+      // mantissa within 4 ulps of 1.75 (448 = 1.75 * 2^8)
+      const bool border = (__float_as_uint(amax) & 0x7fffffu) - (0x600000u - 4u) <= 8u;
+      if (__any_sync(0xffffffffu, border)) amax = largest(std::true_type());
     }
     const float base = old > 0.f && old < INFINITY ? old : 0.f;  // not a scale yet (or never): nothing to keep
     const float s = fmaxf(base, fp8_scale_for(amax));
@@ -316,7 +333,7 @@ __device__ __forceinline__ void write_block(const Fp8WriteArgs& a, const int* ma
       for (int p = 0; p < NP; ++p) {
         if (at[p] < 0) continue;
         uint2 l, h;
-        row(p, [&](int half, const float (&lo)[4], const float (&hi)[4]) {
+        row(p, std::false_type(), [&](int half, const float (&lo)[4], const float (&hi)[4]) {
           (half ? l.y : l.x) = f32x4_to_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv);
           (half ? h.y : h.x) = f32x4_to_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv);
         });

@@ -74,12 +74,12 @@ def write_case(g, tokens, heads, dtype, table_dtype, rows=512):
 
 
 def check_write(heads, bs, dtype, table_dtype, slots, num_blocks, seed=0, calls=1):
-    """`calls` writes into one cache, each of new rows into `slots`; the cache is compared bit for bit.
+    """`calls` writes into one cache, each of new rows into `slots`; scales and value codes are compared bit for bit.
 
-    The model rounds the exact rotation to float32 once, as the kernel does for the keys it codes up to a
-    float32 rounding in about 2^25, and every further step is exact or the same rounding.  Query rows and
-    returned keys are a product and a fused multiply-add in float32 (two roundings, of terms that add up to
-    at most |x c| + |y s|), rounded to 16 bits."""
+    A rotated row is a product and a fused multiply-add in float32: off by at most 2^-24 (|y s| + |r|) from
+    the exact rotation, |r| <= |x c| + |y s|.  Rounded to 16 bits it is half a step more; coded, it can take the
+    other neighbour where the exact value is that near a tie, which of 2^19 float32 values between two ties is
+    about one in 2^18: at most `cells` / 2^18 expected, and 8 more allowed.  Scales are those of exact sums."""
     g = gen(seed)
     H, KH, D = heads
     kc, vc, sc = make_cache(g, num_blocks, KH, bs, D)
@@ -95,8 +95,12 @@ def check_write(heads, bs, dtype, table_dtype, slots, num_blocks, seed=0, calls=
             limit = F.UNIT[dtype] * ref.abs() + 2.0 ** -22 * terms + 2.0 ** -25
             assert ((got.double() - ref).abs() <= limit).all()
         F.write(rk.cpu(), v.float().cpu(), mk, mv, ms, slots.cpu(), bs)
-    assert torch.equal(sc.cpu(), ms)
-    assert torch.equal(bits(kc).cpu(), bits(mk)) and torch.equal(bits(vc).cpu(), bits(mv))
+        assert torch.equal(sc.cpu(), ms) and torch.equal(bits(vc).cpu(), bits(mv))
+        apart = bits(kc).cpu() != bits(mk)
+        assert apart.sum() <= k.numel() / 2 ** 18 + 8
+        a, b = kc.cpu()[apart.view(mk.shape)].float(), mk[apart.view(mk.shape)].float()
+        assert ((a - b).abs() <= torch.maximum(a.abs() / 8, torch.tensor(2.0 ** -9))).all()  # neighbours
+        mk = kc.cpu()
 
 
 @pytest.mark.parametrize("heads", HEADS)
