@@ -35,8 +35,8 @@
 //     slot_mapping[entry] is that slot, so the array needs no initialisation and
 //     keeps nothing from one call to the next.
 // The query rows are rotated by CTAs of their own, behind the others in the same
-// launch or, for many tokens, by a kernel of their own: a thread holds 8 + 8
-// columns of two heads of one token, so the cos and sin rows are read once for two.
+// launch: a thread holds 8 + 8 columns of two heads of one token (four, where there
+// are many tokens), so the cos and sin rows are read once for them.
 // Bound: memory for long chunks; for a decode step the latency of slots ->
 // rows -> maximum -> codes.
 #include <type_traits>
@@ -71,7 +71,7 @@ struct Fp8WriteArgs {
 namespace {
 
 constexpr int kFp8ScanTokens = 2048;
-constexpr int kFp8WriteThreads = 256;
+constexpr int kFp8WriteThreads = 128;
 
 // x c + y s, y the signed partner.  With 16-bit tables the product of two 16-bit
 // floats is exact, and this is the exact rotation rounded once.
@@ -187,13 +187,6 @@ __device__ __forceinline__ void rotate_rows(const Fp8WriteArgs& a, int cta) {
     *reinterpret_cast<uint4*>(dst) = raw[i][0];
     *reinterpret_cast<uint4*>(dst + D / 2) = raw[i][1];
   }
-}
-
-template <typename T, typename TAB, int D>
-__global__ void __launch_bounds__(kFp8WriteThreads, 4) fp8_rotate_kernel(const Fp8WriteArgs a) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  rotate_rows<T, TAB, D, 2>(a, blockIdx.x);
 }
 
 // One block's rows: the call's token at each of its slots is in map (-1: none).
@@ -351,7 +344,7 @@ __device__ __forceinline__ void write_block(const Fp8WriteArgs& a, const int* ma
 // Up to kFp8ScanTokens tokens: CTA t < num_tokens takes token t's block if the token is its leader, the CTAs behind
 // them rotate the query rows.
 template <typename T, typename TAB, int D, bool ROT>
-__global__ void __launch_bounds__(kFp8WriteThreads, 2) fp8_write_kernel(const Fp8WriteArgs a) {
+__global__ void __launch_bounds__(kFp8WriteThreads, 4) fp8_write_kernel(const Fp8WriteArgs a) {
   extern __shared__ int map[];  // [block_size]
   grid_dependency_wait();
   grid_launch_dependents();
@@ -383,14 +376,20 @@ __global__ void __launch_bounds__(kFp8WriteThreads, 2) fp8_write_kernel(const Fp
   write_block<T, TAB, D, ROT>(a, map, b0);
 }
 
-// More tokens, behind fp8_writer_kernel: kFp8Chunk tokens a CTA.
+// More tokens, behind fp8_writer_kernel: kFp8Chunk tokens a CTA, the query rows' CTAs behind them.
 constexpr int kFp8Chunk = 8;
 template <typename T, typename TAB, int D, bool ROT>
-__global__ void __launch_bounds__(kFp8WriteThreads, 2) fp8_write_many_kernel(const Fp8WriteArgs a) {
+__global__ void __launch_bounds__(kFp8WriteThreads, 4) fp8_write_many_kernel(const Fp8WriteArgs a, int kv_ctas) {
   extern __shared__ int map[];  // [block_size]
   __shared__ int64_t slots[kFp8Chunk];  // -1: not a leader
   grid_dependency_wait();
   grid_launch_dependents();
+  if constexpr (ROT) {
+    if ((int)blockIdx.x >= kv_ctas) {
+      rotate_rows<T, TAB, D, 4>(a, (int)blockIdx.x - kv_ctas);
+      return;
+    }
+  }
   const int tid = threadIdx.x, BS = a.block_size;
   const int64_t total_slots = (int64_t)a.num_blocks * BS;
   if (tid < kFp8Chunk) {
@@ -430,13 +429,15 @@ template <typename T, typename TAB, int D, bool ROT>
 int launch_write(const Fp8WriteArgs& a, cudaStream_t stream) {
   const int smem = a.block_size * 4;
   const int rows = a.num_heads + (a.k_out != nullptr ? a.num_kv_heads : 0);
-  const int64_t fill = ((int64_t)a.num_tokens * ((rows + 1) / 2) * (D / 16) + kFp8WriteThreads - 1) / kFp8WriteThreads;
-  const int64_t rotate_ctas = ROT ? fill : 0;
-  if (a.num_tokens + rotate_ctas >= ((int64_t)1 << 31)) return MVB_ERR_INVALID_ARG;
+  auto rotate_ctas = [&](int heads) -> int64_t {
+    const int64_t items = (int64_t)a.num_tokens * ((rows + heads - 1) / heads) * (D / 16);
+    return ROT ? (items + kFp8WriteThreads - 1) / kFp8WriteThreads : 0;
+  };
+  if (a.num_tokens + rotate_ctas(2) >= ((int64_t)1 << 31)) return MVB_ERR_INVALID_ARG;
   if (a.writer == nullptr) {
     auto kern = fp8_write_kernel<T, TAB, D, ROT>;
     if (ensure_kernel_attrs(kern, smem) != cudaSuccess) return MVB_ERR_CUDA;
-    return launch_pdl(kern, dim3((unsigned)(a.num_tokens + rotate_ctas)), dim3(kFp8WriteThreads), smem, stream, a) ==
+    return launch_pdl(kern, dim3((unsigned)(a.num_tokens + rotate_ctas(2))), dim3(kFp8WriteThreads), smem, stream, a) ==
                    cudaSuccess
                ? MVB_OK
                : MVB_ERR_CUDA;
@@ -445,16 +446,11 @@ int launch_write(const Fp8WriteArgs& a, cudaStream_t stream) {
   auto kern = fp8_write_many_kernel<T, TAB, D, ROT>;
   if (ensure_kernel_attrs(first, 0) != cudaSuccess || ensure_kernel_attrs(kern, smem) != cudaSuccess) return MVB_ERR_CUDA;
   if (launch_pdl(first, dim3((a.num_tokens + 255) / 256), dim3(256), 0, stream, a) != cudaSuccess) return MVB_ERR_CUDA;
-  if (launch_pdl(kern, dim3((a.num_tokens + kFp8Chunk - 1) / kFp8Chunk), dim3(kFp8WriteThreads), smem, stream, a) !=
-      cudaSuccess)
-    return MVB_ERR_CUDA;
-  if constexpr (ROT) {
-    auto rotate = fp8_rotate_kernel<T, TAB, D>;
-    if (ensure_kernel_attrs(rotate, 0) != cudaSuccess) return MVB_ERR_CUDA;
-    if (launch_pdl(rotate, dim3((unsigned)rotate_ctas), dim3(kFp8WriteThreads), 0, stream, a) != cudaSuccess)
-      return MVB_ERR_CUDA;
-  }
-  return MVB_OK;
+  const int kv_ctas = (a.num_tokens + kFp8Chunk - 1) / kFp8Chunk;
+  return launch_pdl(kern, dim3((unsigned)(kv_ctas + rotate_ctas(4))), dim3(kFp8WriteThreads), smem, stream, a, kv_ctas) ==
+                 cudaSuccess
+             ? MVB_OK
+             : MVB_ERR_CUDA;
 }
 
 template <typename T>
