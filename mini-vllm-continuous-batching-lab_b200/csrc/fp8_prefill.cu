@@ -5,24 +5,22 @@
 //
 // Rows.  The rows of one KV head are (token, head of its group) pairs,
 // token-major, so the query heads that share keys share a tile.  A CTA holds
-// two tiles of 128 rows and walks the keys 128 at a time up to its last row's
-// limit:   S = Q K_codes^T,   P = exp2(S c_g - m),   O += P V.
+// two tiles of 128 rows and walks the keys 64 at a time up to its last row's limit:
+//   S = Q K_codes^T,   P = exp2(S c_g - m),   O += P V.
 //
-// Roles (5 warpgroups; registers move from the last three to the softmax):
-//   * warps 0-3 and 4-7: the softmax of row tile 0 and 1, one row per thread.
-//     A step takes its exponentials against a maximum of earlier steps and reads
-//     S once.  P may then exceed 1; only when 16 of them add up to more than 2^14
-//     (so that f16 never overflows) is the maximum taken anew, O rescaled in
-//     tensor memory and the step repeated.  A maximum per step cost 128 of its
-//     some 600 instructions.  P goes to tensor memory as f16 (beside S for
-//     head_dim 64; over it for 128, where nothing is left);
-//   * warps 8-11 and 12-15: the loaders of K and of V.  They copy codes through
-//     the block table one step ahead into shared memory (cp.async; block ids and
-//     scales are read four to eight steps ahead), turn them into f16 (exact) and
-//     store tiles in the 128-byte swizzled layout that the tensor core reads, 2
-//     stages each (K 1 for head_dim 128, where shared memory ends);
-//   * warp 16: issues the tensor-core products (tcgen05.mma, 128 x 128 and
-//     128 x D per tile): one row tile's run while the other is in its softmax.
+// Roles (warpgroups; registers move from the last ones to the softmax):
+//   * two of softmax, one per row tile, one row per thread.  A step takes its
+//     exponentials against a maximum of earlier steps and reads S once.  P may then
+//     exceed 1; only when 16 of them add up to more than 2^14 (so that f16 never
+//     overflows) is the maximum taken anew, O rescaled in tensor memory and the
+//     step repeated.  P goes to tensor memory as f16, over S;
+//   * one that loads K and one that loads V.  They copy codes through the block
+//     table one step ahead into shared memory (cp.async; block ids and scales are
+//     read eight to sixteen steps ahead), turn them into f16 (exact) and store tiles
+//     in the 128-byte swizzled layout that the tensor core reads, three stages each;
+//   * one warp per row tile issues its tensor-core products (tcgen05.mma, 128 x 64
+//     and 128 x D per step).  A tile has two buffers of S, so the next step's scores
+//     are there when its softmax comes to them, and the two tiles run independently.
 //
 // Scales.  A block's key scale is one factor of 16 columns of S (a group), so it
 // joins the softmax scale in the exponent's multiply-add at no cost.  A value
@@ -39,8 +37,16 @@
 // the loaders replace NaN codes by 0 and leave a bit per (key, column); a row
 // that attends the key gets NaN in that column at the end.
 //
-// Bound: 16384 exponentials per 128 x 128 tile at 16 per cycle and SM for
-// head_dim 64, the tensor core for head_dim 128.
+// Bound: a step (256 rows, 64 keys) has 1024 cycles of exponentials (16 per cycle
+// and SM) and, for head_dim 128, 1024 of the tensor core.  It takes about 2400: the
+// scores are always there when a softmax warp looks, and its own instructions in
+// turn (two such warps per scheduler) are what the step waits for.  Tried and slower
+// or equal: columns read 32 or 64 at a time; four row tiles of one S buffer each
+// (16 softmax warps, but each then waits for its products: 318 against 287 us for
+// 8192 tokens); 128 keys a step with one buffer of S (278 us there, but 939 against
+// 834 us for head_dim 128, whose P then has to wait in registers for S to be read).
+// Measured: 8192 tokens, 14/2 heads of 64: 287 us, 420 TFLOP/s; 4 x 2048 tokens,
+// 32/8 heads of 128 after 3000 to 6144 cached: 834 us, 760 TFLOP/s.
 //
 // Every wait is bounded (kWaitSpinLimit); one that runs out sets
 // MVB_DEV_TIMEOUT, tells the other roles to leave, and the CTA waits (bounded)
@@ -74,20 +80,18 @@ struct Fp8PrefillArgs {
 namespace {
 
 constexpr int kFp8PrefillMaxChunks = 4096;
-constexpr int kTileRows = 128;               // rows of one row tile (tensor-core M)
-constexpr int kCtaRows = 2 * kTileRows;      // (token, head) rows of one CTA
-constexpr int kKeys = 128;                   // keys per step
-constexpr int kGroups = kKeys / 16;          // 16-key groups: each lies in one block
-constexpr int kThreads = 640;
-// Registers of the warpgroups: 2 softmax, 2 loaders, products; launched with 96 each.
-template <int D> struct Regs { static constexpr int SOFTMAX = 152, LOADER = 64, MMA = 48; };
-template <> struct Regs<64> { static constexpr int SOFTMAX = 128, LOADER = 88, MMA = 48; };
-constexpr int kMinValueExp = -4;
-constexpr int kInfos = 8;                    // steps whose side information is kept (two batches of four)
-constexpr int kMasks = 4;                    // steps whose NaN masks are kept
+constexpr int kTileRows = 128;      // rows of one row tile (tensor-core M)
+constexpr int kKeys = 64;           // keys per step
+constexpr int kGroups = kKeys / 16; // 16-key groups: each lies in one block
+constexpr int kBatch = 32 / kGroups;  // steps whose groups the lanes of a warp hold
+constexpr int kInfos = 2 * kBatch;  // steps whose side information is kept
+constexpr int kStages = 3;          // of K and of V
+constexpr int kNanLag = 3;          // the softmax takes a step's NaN masks this much later
+constexpr int kMasks = kStages + kNanLag;  // steps whose NaN masks are kept
 constexpr int kTmemCols = 512;
+constexpr int kMinValueExp = -4;      // of the part of a value scale that joins the exponent
 
-// Side information of one step, written by the loaders.
+// Side information of one step, written by the loaders (nan by those of V).
 struct alignas(16) StepInfo {
   // per group: the key scale; log2 of the part ve of (value scale / R) that goes into P; 2^-ve
   float4 g[kGroups];
@@ -97,20 +101,39 @@ struct alignas(16) StepInfo {
   int nan[4];         // per loader warp: its keys' values hold NaN, and their masks are written
 };
 
+constexpr int NT = 2;  // row tiles
+constexpr int NB = 2;  // buffers of S (and P) per tile
+constexpr int kThreads = 128 * (NT + 3), kCtaRows = NT * kTileRows;
+constexpr int kLoadWarp = 4 * NT, kMmaWarp = kLoadWarp + 8;  // first warps of the roles behind the softmax
+
 template <int D> struct Geo {
-  static constexpr int QBYTES = kTileRows * D * 2, KBYTES = kKeys * D * 2;
-  static constexpr int NMASK = kMasks * kKeys * (D / 16) * 2;  // a bit per (key, column)
-  static constexpr int KST = D == 64 ? 2 : 1;                  // stages of K
-  static constexpr int Q = 0, K = 2 * QBYTES, V = K + KST * KBYTES, RAW = V + 2 * KBYTES;  // RAW: codes of K, of V
-  static constexpr int MASK = RAW + KBYTES, INFO = MASK + NMASK, BARS = INFO + kInfos * (int)sizeof(StepInfo);
-  static constexpr int BYTES = BARS + 128 + 1024;  // + alignment
-  // tensor-memory columns: S 2 x 128, O 2 x D, P 2 x 64
-  static constexpr bool P_APART = D == 64;
-  static constexpr int S_COL = 0, O_COL = 256, P_COL = P_APART ? 384 : 0, P_STEP = P_APART ? 64 : 128;
+  // registers: launched with LAUNCH, moved to what each role takes
+  static constexpr int LAUNCH = 96, SOFTMAX = D == 64 ? 144 : 152, LOADER = D == 64 ? 72 : 64, MMA = 48;
+  static_assert(NT * SOFTMAX + 2 * LOADER + MMA <= (NT + 3) * LAUNCH, "what the block was launched with");
+  static constexpr int QBYTES = kTileRows * D * 2, KBYTES = kKeys * D * 2, RAWBYTES = kKeys * D;
+  static constexpr int Q = 0, K = NT * QBYTES, V = K + kStages * KBYTES, RAW = V + kStages * KBYTES;  // RAW: K, V codes
+  static constexpr int MASK = RAW + 2 * RAWBYTES, NMASK = kMasks * kKeys * (D / 16) * 2;  // a bit per (key, column)
+  static constexpr int INFO = MASK + NMASK, BARS = INFO + kInfos * (int)sizeof(StepInfo);
+  static constexpr int BYTES = BARS + 256 + 1024;  // + alignment
+  // tensor-memory columns: S (and P over its first half) NT x NB x 64, O NT x D
+  static constexpr int O_COL = NT * NB * kKeys;
+  static_assert(O_COL + NT * D <= kTmemCols, "tensor memory");
 };
 
-// Barriers (indices).
-enum { kQ = 0, kKFull = 1, kKEmpty = 3, kVFull = 5, kVEmpty = 7, kSFull = 9, kPReady = 11, kPvDone = 13, kNumBars = 15 };
+// Barriers (indices): per stage; per tile and buffer of S (so that no one's wait is ever two phases off).
+enum {
+  kQ = 0,
+  kKFull = 1,
+  kKEmpty = kKFull + kStages,
+  kVFull = kKEmpty + kStages,
+  kVEmpty = kVFull + kStages,
+  kSFull = kVEmpty + kStages,
+  kPReady = kSFull + 4,
+  kPvDone = kPReady + 4,
+  kGivenUp = kPvDone + 4,  // per tile, used once
+  kNumBars = kGivenUp + 4
+};
+static_assert(kNumBars * 8 <= 256, "the barriers' place");
 
 // ---- tensor memory and tcgen05 ----------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_dst) {
@@ -248,9 +271,9 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, __half2 f) {
   const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), f);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Byte offset of 16-byte chunk `c` of a row's 64-column panel in a swizzled tile of 128 rows.
-__device__ __forceinline__ uint32_t swz(int row, int panel, int c) {
-  return (uint32_t)(panel * (kKeys * 128) + row * 128 + ((c ^ (row & 7)) << 4));
+// Byte offset of 16-byte chunk `c` of a row's 64-column panel in a swizzled tile of `rows` rows.
+__device__ __forceinline__ uint32_t swz(int rows, int row, int panel, int c) {
+  return (uint32_t)(panel * (rows * 128) + row * 128 + ((c ^ (row & 7)) << 4));
 }
 // Waits of all roles: bounded, and given up when another role has given up.
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* stop, int* err) {
@@ -277,7 +300,6 @@ struct Waiter {
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8PrefillArgs a) {
   using G_ = Geo<D>;
-  static_assert(2 * Regs<D>::SOFTMAX + 2 * Regs<D>::LOADER + Regs<D>::MMA <= 5 * 96, "what the block was launched with");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int s_tot[2][kThreads / 32];
@@ -371,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   }
   const int kv_end = (int)cached + (row0 + nrows - 1) / a.G + 1;  // positions the CTA's last row attends
   const int steps = (kv_end + kKeys - 1) / kKeys;
-  const int tiles = nrows > kTileRows ? 2 : 1;
+  const int tiles = (nrows + kTileRows - 1) / kTileRows;
 
   Waiter wait;
   wait.bars = smem_u32(smem + G_::BARS);
@@ -379,18 +401,21 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   wait.err = a.err;
   StepInfo* infos = reinterpret_cast<StepInfo*>(smem + G_::INFO);
   uint16_t* masks = reinterpret_cast<uint16_t*>(smem + G_::MASK);  // [kMasks][kKeys][D / 16]
-  if (warp == 16) tmem_alloc(smem_u32(&s_tmem));
+  if (warp == kMmaWarp) tmem_alloc(smem_u32(&s_tmem));
   if (tid == 0) {
     s_stop = 0;
     mbar_init(wait.bar(kQ), 4 * tiles);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(wait.bar(kKFull + i), 4);
       mbar_init(wait.bar(kVFull + i), 4);
-      mbar_init(wait.bar(kKEmpty + i), 1);
-      mbar_init(wait.bar(kVEmpty + i), 1);
+      mbar_init(wait.bar(kKEmpty + i), tiles);
+      mbar_init(wait.bar(kVEmpty + i), tiles);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(wait.bar(kSFull + i), 1);
       mbar_init(wait.bar(kPReady + i), 4);
       mbar_init(wait.bar(kPvDone + i), 1);
+      mbar_init(wait.bar(kGivenUp + i), 1);
     }
     fence_mbar_init();
   }
@@ -399,14 +424,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   tc_fence_after();
   const uint32_t tmem = s_tmem;
 
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<D>::SOFTMAX));
+  if (warp < kLoadWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G_::SOFTMAX));
     // ================================ softmax =================================
     const int tile = warp >> 2, r = row0 + tile * kTileRows + (warp & 3) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + lanes + G_::S_COL + tile * kKeys, o_at = tmem + lanes + G_::O_COL + tile * D,
-                     p_at = tmem + lanes + G_::P_COL + tile * G_::P_STEP;
+      const uint32_t o_at = tmem + lanes + G_::O_COL + tile * D;
       const bool live = r < rows;
       const int tok = live ? r / a.G : 0, head = live ? r - tok * a.G : 0;
       const int lim = live ? (int)cached + tok + 1 : kv_end;  // rows past the chunk are zeros that attend all
@@ -440,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
           w.y = pack_h2(to_f32<T>(e[2]) * down, to_f32<T>(e[3]) * down);
           w.z = pack_h2(to_f32<T>(e[4]) * down, to_f32<T>(e[5]) * down);
           w.w = pack_h2(to_f32<T>(e[6]) * down, to_f32<T>(e[7]) * down);
-          *reinterpret_cast<uint4*>(qd + swz(qr, i / 8, i % 8)) = w;
+          *reinterpret_cast<uint4*>(qd + swz(kTileRows, qr, i / 8, i % 8)) = w;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -461,18 +485,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
               nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kMasks) * kKeys + k) * (D / 16))[i];
       };
       // One step of the softmax; EDGE: it holds keys that some row does not attend.
-      auto step = [&](int j, auto edge) {
+      auto step = [&](int j, auto edge, bool anew, float rf) {
         constexpr bool EDGE = decltype(edge)::value;
         const StepInfo& f = infos[j % kInfos];
         const int rem = lim - j * kKeys;
-        // columns read at a time, two reads in flight; P over S waits in registers until the step holds
-        constexpr int CW = G_::P_APART ? 32 : 16, NC = kKeys / CW;
+        const uint32_t s_at = tmem + lanes + (tile * NB + j % NB) * kKeys;  // P goes over it
+        // columns read at a time, two reads in flight; P waits in registers until the step holds
+        constexpr int CW = 16, NC = kKeys / CW;
         uint32_t s[2][CW];
         auto read = [&](int h) {
-          if constexpr (CW == 32)
-            tmem_ld32(s_at + CW * h, s[h & 1]);
-          else
-            tmem_ld16(s_at + CW * h, s[h & 1]);
+          tmem_ld16(s_at + CW * h, s[h & 1]);
         };
         auto mask = [&](int h) {  // -inf where the row does not attend the key
           if constexpr (EDGE) {
@@ -483,17 +505,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
           }
         };
         auto factor = [&](float ks) { return fmaxf(qs * ks, 1.2e-38f); };  // (not 0: -inf stays -inf)
-        bool anew = __any_sync(0xffffffffu, m == -INFINITY);  // a row's first keys
-        const float rf = f.rf;
         float fac = rf;
         bool move = rf != 1.f;
-        // the last step's products read P and added to O
-        if (j > 0) {
-          if (!wait.warp(kPvDone + tile, (j - 1) & 1)) return false;
-          tc_fence_after();
-          take_nan(j - 1);
-        }
-        uint32_t p[G_::P_APART ? 16 : 64];
+        uint32_t p[kKeys / 2];
         for (;;) {
           if (anew) {
             float mx = m;
@@ -547,14 +561,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
                 e.x = fast_exp2(e.x);
                 e.y = fast_exp2(e.y);
                 t[i / 2 & 1] = i < 4 ? e : add2(t[i / 2 & 1], e);
-                p[(G_::P_APART ? 0 : CW / 2 * h) + 8 * gg + i / 2] = pack_h2(e.x, e.y);
+                p[CW / 2 * h + 8 * gg + i / 2] = pack_h2(e.x, e.y);
               }
               t[0] = add2(t[0], t[1]);
               const float u = t[0].x + t[0].y;
               most = fmaxf(most, u);
               sum = fmaf(u, in.z, sum);
             }
-            if constexpr (G_::P_APART) tmem_st16(p_at + CW / 2 * h, p);
           }
           anew = __any_sync(0xffffffffu, most > 16384.f);
           if (!anew) {
@@ -562,11 +575,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
             break;
           }
         }
-        if constexpr (!G_::P_APART) {
-#pragma unroll
-          for (int h = 0; h < 4; ++h) tmem_st16(p_at + 16 * h, p + 16 * h);
-        }
+        tmem_st16(s_at, p);
+        tmem_st16(s_at + 16, p + 16);
         if (move && j > 0) {
+          // the last step's products add to O
+          if (!wait.warp(kPvDone + tile * NB + (j - 1) % NB, ((j - 1) / NB) & 1)) return false;
+          tc_fence_after();
 #pragma unroll
           for (int h = 0; h < D / 32; ++h) {
             uint32_t o[32];
@@ -580,22 +594,28 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(wait.bar(kPReady + tile));
+        if (lane == 0) mbar_arrive(wait.bar(kPReady + tile * NB + j % NB));
         return true;
       };
-      bool ok = true;
+      const int least = __reduce_min_sync(0xffffffffu, lim);
+      bool ok = true, fresh = true;
       for (int j = 0; ok && j < steps; ++j) {
-        ok = wait.warp(kSFull + tile, j & 1);
+        // before the wait: what is known of the step (the scores of the one before it came after the loaders had
+        // written it) and the NaN of values whose products are done (those scores came after them)
+        const bool edge = least - j * kKeys < kKeys;
+        if (fresh) fresh = __any_sync(0xffffffffu, m == -INFINITY);  // a row's first keys
+        if (j >= kNanLag) take_nan(j - kNanLag);
+        if (j == 0 && !wait.warp(kSFull + tile * NB, 0)) break;
+        const float rf = infos[j % kInfos].rf;
+        const int bad = infos[j % kInfos].bad;
+        ok = wait.warp(kSFull + tile * NB + j % NB, (j / NB) & 1);
         if (!ok) break;
         tc_fence_after();
-        if (__any_sync(0xffffffffu, lim - j * kKeys < kKeys) || infos[j % kInfos].bad != 0)
-          ok = step(j, std::true_type());
-        else
-          ok = step(j, std::false_type());
+        ok = edge || bad ? step(j, std::true_type(), fresh, rf) : step(j, std::false_type(), fresh, rf);
       }
-      if (ok && wait.warp(kPvDone + tile, (steps - 1) & 1)) {
+      if (ok && wait.warp(kPvDone + tile * NB + (steps - 1) % NB, ((steps - 1) / NB) & 1)) {
         tc_fence_after();
-        take_nan(steps - 1);
+        for (int j = max(0, steps - kNanLag); j < steps; ++j) take_nan(j);
         const float inv = l == 0.f ? 0.f : infos[(steps - 1) % kInfos].r / l;
         T* op = out + (int64_t)(q0 + tok) * a.o_s0 + (int64_t)(h0 + head) * a.o_s1;
 #pragma unroll
@@ -618,19 +638,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         }
       }
     }
-  } else if (warp < 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<D>::LOADER));
+  } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G_::LOADER));
     // ================================ loaders =================================
     constexpr int CH = D / 16, N = kKeys * CH / 128;  // 16-code chunks per row, chunks per thread and tile
-    constexpr uint32_t NONE = 0xffffffffu;
-    const bool is_v = warp >= 12;
+    constexpr uint32_t NONE = 0xffffffffu, IN_STEP = (1u << kGroups) - 1;
+    const bool is_v = warp >= kLoadWarp + 4;
     const int lw = warp & 3;
     const int64_t* bt = a.bt + srow * a.bt_s0;
     const int BSm = (1 << a.block_shift) - 1, gshift = a.block_shift - 4;
-    // Four steps at a time, one 16-key group per lane: its number among the cache's groups (NONE behind the last
+    // kBatch steps at a time, one 16-key group per lane: its number among the cache's groups (NONE behind the last
     // key or for a bad block id), and its block's scales.
-    auto find = [&](int j4, bool& bad) {
-      const int p = j4 * kKeys + 16 * lane;
+    auto find = [&](int j0, bool& bad) {
+      const int p = j0 * kKeys + 16 * lane;
       bad = false;
       if (p >= kv_end) return NONE;
       const int64_t b = ld_ahead8(bt + (p >> a.block_shift));
@@ -645,224 +665,213 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     // chunks of one panel of two keys, whose swizzled places are in different banks.
     const int ch = CH == 4 ? lane & 3 : (lane & 3) | (lane >> 1 & 4);
     const int key0 = CH == 4 ? lw * 8 + (lane >> 2) : lw * 4 + ((lane >> 2 & 1) | (lane >> 3 & 2));
-    uint8_t* const raw = smem + G_::RAW + (is_v ? G_::KBYTES / 2 : 0) + (lw * 32 + lane) * 16;  // its codes: + 2048 i
-    const uint32_t to0 = swz(key0, ch / 4, 2 * (ch % 4)), to1 = to0 ^ 16;  // its places in a tile: + i * STEP
+    uint8_t* const raw = smem + G_::RAW + (is_v ? G_::RAWBYTES : 0) + (lw * 32 + lane) * 16;  // its codes: + 2048 i
+    const uint32_t to0 = swz(kKeys, key0, ch / 4, 2 * (ch % 4)), to1 = to0 ^ 16;  // its places in a tile: + i * STEP
     constexpr uint32_t STEP = (128 / CH) * 128;
-    const uint8_t* const from = (is_v ? a.vc : a.kc) + ((key0 & 15) * D + ch * 16);
+    const uint8_t* const base = (is_v ? a.vc : a.kc) + (key0 & 15) * D + ch * 16;
     const uint32_t dst = smem_u32(raw);
     auto fetch = [&](int j, uint32_t groups) {
       const bool tail = (j + 1) * kKeys > kv_end;
-#pragma unroll 4
+#pragma unroll
       for (int i = 0; i < N; ++i) {
         const int key = key0 + i * (128 / CH);
-        const uint32_t grp = __shfl_sync(0xffffffffu, groups, (j & 3) * kGroups + (key >> 4));
+        const uint32_t grp = __shfl_sync(0xffffffffu, groups, (j % kBatch) * kGroups + (key >> 4));
         const bool ok = grp != NONE && !(tail && j * kKeys + key >= kv_end);
-        cp_async_16(dst + 2048 * i, from + (ok ? (uint64_t)grp * (16 * D) : 0), ok ? 16 : 0);
+        cp_async_16(dst + 2048 * i, base + (ok ? (uint64_t)grp * (16 * D) : 0), ok ? 16 : 0);
       }
       cp_async_commit();
     };
     bool bad, bad_n;
-    uint32_t grp = find(0, bad), grp_n = find(4, bad_n);
+    uint32_t grp = find(0, bad), grp_n = find(kBatch, bad_n);
     fetch(0, grp);
-    float2 sc = scales(grp), sc_n = make_float2(0.f, 0.f);
-    int RE = 127;                                // exponent field of R
-    uint32_t rests = 0;                          // lanes whose group's value scale goes into the codes in part
+    const float2 sc = scales(grp);
+    float2 sc_n = make_float2(0.f, 0.f);
+    int RE = 127;        // exponent field of R
+    uint32_t rests = 0;  // lanes whose group's value scale goes into the codes in part
     float rest = 1.f;
-    for (int j = 0; j < steps; ++j) {
-      const int st = j & 1, kst = j % G_::KST, q = (j & 3) * kGroups;
-      if (q == 0) {  // side information of four steps
-        const int vexp = (int)(__float_as_uint(sc.y) >> 23) & 0xff;  // 0: a scale of 0 or below 2^-126
-        int top = vexp, mine = 0;  // largest exponent field of the step; R's of this lane's step
-        float rf = 1.f;
+    // The side information of kBatch steps from j on; each lane's part of its group's scale that goes into the codes
+    // of V, and the lanes where that is not 1.
+    auto side_info = [&](int j, float2 sc, uint32_t grp, bool bad, float& rest, uint32_t& rests) {
+      const int vexp = (int)(__float_as_uint(sc.y) >> 23) & 0xff;  // 0: a scale of 0 or below 2^-126
+      int top = vexp, mine = 0;  // largest exponent field of the step; R's of this lane's step
+      float rf = 1.f;
 #pragma unroll
-        for (int o = 1; o < kGroups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = __shfl_sync(0xffffffffu, top, k * kGroups);
-          const int was = RE;
-          if (j + k == 0)
-            RE = t > 0 ? t : 127;
-          else if (t > RE + 7)
-            RE = t;
-          if (lane >> 3 == k) {
-            mine = RE;
-            if (j + k > 0 && RE != was) rf = RE - was < 127 ? __uint_as_float((uint32_t)(127 + was - RE) << 23) : 0.f;
-          }
+      for (int o = 1; o < kGroups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 1
+      for (int k = 0; k < kBatch; ++k) {
+        const int t = __shfl_sync(0xffffffffu, top, k * kGroups);
+        const int was = RE;
+        if (j + k == 0)
+          RE = t > 0 ? t : 127;
+        else if (t > RE + 7)
+          RE = t;
+        if (lane / kGroups == k) {
+          mine = RE;
+          if (j + k > 0 && RE != was) rf = RE - was < 127 ? __uint_as_float((uint32_t)(127 + was - RE) << 23) : 0.f;
         }
-        const int e = vexp > 0 ? vexp - mine : 0, ep = max(e, kMinValueExp);
-        rest = grp != NONE && vexp == 0 ? 0.f
-               : e == ep                ? 1.f
-               : e - ep > -127          ? __uint_as_float((uint32_t)(127 + e - ep) << 23)
-                                        : 0.f;
-        rests = __ballot_sync(0xffffffffu, rest != 1.f);
-        const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-        if (!is_v && lw == 0) {
-          const float vf = vexp > 0 ? __uint_as_float((__float_as_uint(sc.y) & 0x7fffffu) | 0x3f800000u) : 1.f;
-          StepInfo& f = infos[(j + (lane >> 3)) % kInfos];
-          const int g = lane & (kGroups - 1);
-          float ve = (float)ep, vu = __uint_as_float((uint32_t)(127 - ep) << 23);
-          if (vf != 1.f) {
-            ve += log2f(vf);
-            vu /= vf;
-          }
-          f.g[g] = make_float4(sc.x, ve, vu, 0.f);
-          if (g == 0) {
-            f.r = __uint_as_float((uint32_t)mine << 23);
-            f.rf = rf;
-            f.bad = (int)(bads >> (lane & ~7) & ((1u << kGroups) - 1));
-          }
-          if (lane == 0 && bads) atomicOr(a.err, MVB_DEV_BLOCK_ID);
-        }
-        __syncwarp();
       }
-      const uint32_t groups_next = ((j + 1) & 3) == 0 ? grp_n : grp;
+      const int e = vexp > 0 ? vexp - mine : 0, ep = max(e, kMinValueExp);
+      rest = grp != NONE && vexp == 0 ? 0.f
+             : e == ep                ? 1.f
+             : e - ep > -127          ? __uint_as_float((uint32_t)(127 + e - ep) << 23)
+                                      : 0.f;
+      rests = __ballot_sync(0xffffffffu, rest != 1.f);
+      const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+      if (!is_v && lw == 0) {
+        const float vf = vexp > 0 ? __uint_as_float((__float_as_uint(sc.y) & 0x7fffffu) | 0x3f800000u) : 1.f;
+        StepInfo& f = infos[(j + lane / kGroups) % kInfos];
+        const int g = lane % kGroups;
+        float ve = (float)ep, vu = __uint_as_float((uint32_t)(127 - ep) << 23);
+        if (vf != 1.f) {
+          ve += log2f(vf);
+          vu /= vf;
+        }
+        f.g[g] = make_float4(sc.x, ve, vu, 0.f);
+        if (g == 0) {
+          f.r = __uint_as_float((uint32_t)mine << 23);
+          f.rf = rf;
+          f.bad = (int)(bads >> (lane & ~(kGroups - 1)) & IN_STEP);
+        }
+        if (lane == 0 && bads) atomicOr(a.err, MVB_DEV_BLOCK_ID);
+      }
+      __syncwarp();
+    };
+    uint32_t rests_n = 0;
+    float rest_n = 1.f;
+    side_info(0, sc, grp, bad, rest, rests);
+    for (int j = 0; j < steps; ++j) {
+      const int st = j % kStages, q = (j % kBatch) * kGroups;
+      const int again = (j / kStages - 1) & 1;  // parity of the stage's last use
+      if (q == (kBatch - 1) * kGroups) side_info(j + 1, sc_n, grp_n, bad_n, rest_n, rests_n);
+      const uint32_t groups_next = (j + 1) % kBatch == 0 ? grp_n : grp;
       if (!is_v) {
-        if (j >= G_::KST && !wait.warp(kKEmpty + kst, (j / G_::KST - 1) & 1)) break;
+        if (j >= kStages && !wait.warp(kKEmpty + st, again)) break;
         cp_async_wait<0>();
-        {
-          uint8_t* tile = smem + G_::K + kst * G_::KBYTES;
-#pragma unroll 4
-          for (int i = 0; i < N; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
-            uint4 lo4, hi4;
-            e4m3x4_to_f16(x.x, lo4.x, lo4.y);
-            e4m3x4_to_f16(x.y, lo4.z, lo4.w);
-            e4m3x4_to_f16(x.z, hi4.x, hi4.y);
-            e4m3x4_to_f16(x.w, hi4.z, hi4.w);
-            *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
-            *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
-          }
+        uint8_t* tile = smem + G_::K + st * G_::KBYTES;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+          uint4 lo4, hi4;
+          e4m3x4_to_f16(x.x, lo4.x, lo4.y);
+          e4m3x4_to_f16(x.y, lo4.z, lo4.w);
+          e4m3x4_to_f16(x.z, hi4.x, hi4.y);
+          e4m3x4_to_f16(x.w, hi4.z, hi4.w);
+          *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
+          *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(wait.bar(kKFull + kst));
+        if (lane == 0) mbar_arrive(wait.bar(kKFull + st));
       } else {
-        if (j >= 2 && !wait.warp(kVEmpty + st, (j / 2 - 1) & 1)) break;
+        if (j >= kStages && !wait.warp(kVEmpty + st, again)) break;
         cp_async_wait<0>();
-        {
-          uint8_t* tile = smem + G_::V + st * G_::KBYTES;
-                  uint32_t seen = 0;
-          auto store = [&](uint4 x, int i) {
-            uint4 lo4, hi4;
-            e4m3x4_to_f16(x.x, lo4.x, lo4.y);
-            e4m3x4_to_f16(x.y, lo4.z, lo4.w);
-            e4m3x4_to_f16(x.z, hi4.x, hi4.y);
-            e4m3x4_to_f16(x.w, hi4.z, hi4.w);
-            if (rests >> q & ((1u << kGroups) - 1)) {
-              const __half2 r2 =
-                  __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
-              lo4 = make_uint4(mul_h2(lo4.x, r2), mul_h2(lo4.y, r2), mul_h2(lo4.z, r2), mul_h2(lo4.w, r2));
-              hi4 = make_uint4(mul_h2(hi4.x, r2), mul_h2(hi4.y, r2), mul_h2(hi4.z, r2), mul_h2(hi4.w, r2));
-            }
-            *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
-            *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
-          };
-#pragma unroll 4
+        uint8_t* tile = smem + G_::V + st * G_::KBYTES;
+        uint32_t seen = 0;
+        auto store = [&](uint4 x, int i) {
+          uint4 lo4, hi4;
+          e4m3x4_to_f16(x.x, lo4.x, lo4.y);
+          e4m3x4_to_f16(x.y, lo4.z, lo4.w);
+          e4m3x4_to_f16(x.z, hi4.x, hi4.y);
+          e4m3x4_to_f16(x.w, hi4.z, hi4.w);
+          if (rests >> q & IN_STEP) {
+            const __half2 r2 =
+                __float2half2_rn(__shfl_sync(0xffffffffu, rest, q + ((key0 + i * (128 / CH)) >> 4)));
+            lo4 = make_uint4(mul_h2(lo4.x, r2), mul_h2(lo4.y, r2), mul_h2(lo4.z, r2), mul_h2(lo4.w, r2));
+            hi4 = make_uint4(mul_h2(hi4.x, r2), mul_h2(hi4.y, r2), mul_h2(hi4.z, r2), mul_h2(hi4.w, r2));
+          }
+          *reinterpret_cast<uint4*>(tile + to0 + i * STEP) = lo4;
+          *reinterpret_cast<uint4*>(tile + to1 + i * STEP) = hi4;
+        };
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+          // a byte 0x7f or 0xff is NaN: its low seven bits and one more reach the eighth
+          seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
+                  ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+          store(x, i);
+        }
+        const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
+        if (any_nan) {  // once more with zeros in their place, and the masks
+#pragma unroll 1
           for (int i = 0; i < N; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
-            // a byte 0x7f or 0xff is NaN: its low seven bits and one more reach the eighth
-            seen |= ((x.x & 0x7f7f7f7fu) + 0x01010101u) | ((x.y & 0x7f7f7f7fu) + 0x01010101u) |
-                    ((x.z & 0x7f7f7f7fu) + 0x01010101u) | ((x.w & 0x7f7f7f7fu) + 0x01010101u);
+            uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
+            uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+            uint32_t nan16 = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              w[k] &= ~((n >> 7) * 0xffu);
+              nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
+            }
+            masks[((j % kMasks) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
             store(x, i);
           }
-          const bool any_nan = __any_sync(0xffffffffu, (seen & 0x80808080u) != 0);
-          if (any_nan) {  // once more with zeros in their place, and the masks
-#pragma unroll 1
-            for (int i = 0; i < N; ++i) {
-              uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * i);
-              uint32_t* w = reinterpret_cast<uint32_t*>(&x);
-              uint32_t nan16 = 0;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t n = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                w[k] &= ~((n >> 7) * 0xffu);
-                nan16 |= ((n >> 7 & 1) | (n >> 14 & 2) | (n >> 21 & 4) | (n >> 28 & 8)) << (4 * k);
-              }
-              masks[((j % kMasks) * kKeys + key0 + i * (128 / CH)) * CH + ch] = (uint16_t)nan16;
-              store(x, i);
-            }
-          }
-          if (lane == 0) infos[j % kInfos].nan[lw] = any_nan;
         }
+        if (lane == 0) infos[j % kInfos].nan[lw] = any_nan;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(wait.bar(kVFull + st));
       }
       fetch(j + 1, groups_next);  // nothing behind the last key
-      if ((j & 3) == 1) sc_n = scales(grp_n);
-      if ((j & 3) == 3) {
+      if (j % kBatch == kBatch / 2 - 1) sc_n = scales(grp_n);
+      if (j % kBatch == kBatch - 1) {
         grp = grp_n;
-        bad = bad_n;
-        sc = sc_n;
-        grp_n = find(j + 5, bad_n);
+        rest = rest_n;
+        rests = rests_n;
+        grp_n = find(j + 1 + kBatch, bad_n);
       }
     }
     cp_async_wait<0>();  // nothing lands after the CTA has left
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<D>::MMA));
-    if (warp == 16) {
-      // ========================= tensor-core products ===========================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G_::MMA));
+    // ==================== tensor-core products of row tile i ====================
+    const int i = warp - kMmaWarp;
+    if (i < tiles) {
       const uint32_t base = smem_u32(smem);
       const int lead = elect_one();
       constexpr uint32_t SW = mma_word(kKeys, false), PW = mma_word(D, true);
-      auto scores = [&](int i, int kst) {  // S_i = Q_i K^T: 16 columns (32 bytes of a panel's row) a step
+      const uint32_t s_col = tmem + i * NB * kKeys, o_col = tmem + G_::O_COL + i * D;
+      auto scores = [&](int j) {  // S = Q K^T of step j: 16 columns (32 bytes of a panel's row) at a time
         const uint64_t qd = smem_desc(base + G_::Q + i * G_::QBYTES, 16, 1024);
-        const uint64_t kd = smem_desc(base + G_::K + kst * G_::KBYTES, 16, 1024);
+        const uint64_t kd = smem_desc(base + G_::K + (j % kStages) * G_::KBYTES, 16, 1024);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)((k / 4) * (kKeys * 128) + (k % 4) * 32) >> 4;
-          mma_ss(tmem + G_::S_COL + i * kKeys, qd + off, kd + off, SW, k > 0, lead);
-        }
-        tc_commit(wait.bar(kSFull + i), lead);
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(s_col + (j % NB) * kKeys, qd + (((k / 4) * (kTileRows * 128) + (k % 4) * 32) >> 4),
+                 kd + (((k / 4) * (kKeys * 128) + (k % 4) * 32) >> 4), SW, k > 0, lead);
+        tc_commit(wait.bar(kSFull + i * NB + j % NB), lead);
+        tc_commit(wait.bar(kKEmpty + j % kStages), lead);
       };
-      auto values = [&](int i, int st, bool add) {  // O_i += P_i V: 16 keys (2 KB of a panel) a step
-        const uint64_t vd = smem_desc(base + G_::V + st * G_::KBYTES, kKeys * 128, 1024);
+      auto values = [&](int j) {  // O += P V of step j: 16 keys (2 KB of a panel) at a time
+        const uint64_t vd = smem_desc(base + G_::V + (j % kStages) * G_::KBYTES, kKeys * 128, 1024);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
-          mma_ts(tmem + G_::O_COL + i * D, tmem + G_::P_COL + i * G_::P_STEP + 8 * k, vd + (k * 2048 >> 4), PW,
-                 add || k > 0, lead);
-        tc_commit(wait.bar(kPvDone + i), lead);
+          mma_ts(o_col, s_col + (j % NB) * kKeys + 8 * k, vd + (k * 2048 >> 4), PW, j > 0 || k > 0, lead);
+        tc_commit(wait.bar(kPvDone + i * NB + j % NB), lead);
+        tc_commit(wait.bar(kVEmpty + j % kStages), lead);
       };
-      auto ready = [&](int i, int parity) {
-        if (!wait.warp(i, parity)) return false;
+      auto ready = [&](int b, int parity) {
+        if (!wait.warp(b, parity)) return false;
         tc_fence_after();
         return true;
       };
-      bool ok = ready(kQ, 0) && ready(kKFull, 0);
-      if (ok) {
-        for (int i = 0; i < tiles; ++i) scores(i, 0);
-        tc_commit(wait.bar(kKEmpty), lead);
+      auto ready_k = [&](int j) { return ready(kKFull + j % kStages, (j / kStages) & 1); };
+      bool ok = ready(kQ, 0);
+      for (int j = 0; ok && j < min(NB, steps); ++j) {
+        ok = ready_k(j);
+        if (ok) scores(j);
       }
       for (int j = 0; ok && j < steps; ++j) {
-        const int st = j & 1, kn = (j + 1) % G_::KST;
-        const bool next = j + 1 < steps;
-        auto next_scores = [&](int i) {
-          if (i == 0 && !ready(kKFull + kn, ((j + 1) / G_::KST) & 1)) return false;
-          scores(i, kn);
-          if (i == tiles - 1) tc_commit(wait.bar(kKEmpty + kn), lead);
-          return true;
-        };
-        for (int i = 0; ok && i < tiles; ++i) {
-          ok = ready(kPReady + i, j & 1);
-          // P apart: S has been read, and the next step's softmax need not wait for P V
-          if (ok && G_::P_APART && next) ok = next_scores(i);
-          if (ok && i == 0) ok = ready(kVFull + st, (j / 2) & 1);
-          if (!ok) break;
-          values(i, st, j > 0);
-          if (i == tiles - 1) tc_commit(wait.bar(kVEmpty + st), lead);
-          // P over S: the products that read it come before S of the next step
-          if (!G_::P_APART && next) ok = ready(kPvDone + i, j & 1) && next_scores(i);
+        ok = ready(kVFull + j % kStages, (j / kStages) & 1) && ready(kPReady + i * NB + j % NB, (j / NB) & 1);
+        if (!ok) break;
+        values(j);
+        if (j + NB < steps) {  // S overwrites P: the products that read it come first
+          ok = ready_k(j + NB) && ready(kPvDone + i * NB + j % NB, (j / NB) & 1);
+          if (ok) scores(j + NB);
         }
       }
-      if (!ok) {
-        // given up: wait for whatever was issued before the tensor memory goes (on a barrier that nothing else uses)
-        if (lead) {
-          mbar_init(wait.bar(kNumBars), 1);
-          fence_mbar_init();
-        }
-        __syncwarp();
-        tc_commit(wait.bar(kNumBars), lead);
-        mbar_wait_bounded(wait.bar(kNumBars), 0);
+      if (!ok) {  // given up: wait for whatever was issued before the tensor memory goes
+        tc_commit(wait.bar(kGivenUp + i), lead);
+        mbar_wait_bounded(wait.bar(kGivenUp + i), 0);
       }
     }
   }
@@ -870,13 +879,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 16) tmem_free(tmem);
+  if (warp == kMmaWarp) tmem_free(tmem);
 }
 
 template <typename T, int D>
 int launch_prefill_fp8(const Fp8PrefillArgs& a, cudaStream_t stream) {
   auto kern = fp8_prefill_kernel<T, D>;
-  static_assert(2 * (kFp8PrefillMaxChunks + 1) * 4 <= 3 * Geo<D>::KBYTES, "the prefixes fit the stages");
+  static_assert(2 * (kFp8PrefillMaxChunks + 1) * 4 <= 2 * kStages * Geo<D>::KBYTES, "the prefixes fit the stages");
   static_assert(Geo<D>::BYTES <= 227 * 1024 - 512, "shared memory of one CTA");
   if (ensure_kernel_attrs(kern, Geo<D>::BYTES) != cudaSuccess) return MVB_ERR_CUDA;
   const int64_t tiles = ((int64_t)a.total_q * a.G + kCtaRows - 1) / kCtaRows + a.n;
