@@ -445,15 +445,21 @@ int mvb_paged_decode_fp8_workspace(int32_t num_seqs, int32_t num_heads, int32_t 
 /* Causal paged prefill attention over the 8-bit cache: mvb_paged_prefill with
  * every position, the chunk's own among them, read from the cache (written
  * before the call).  A block id outside [0, num_blocks) sets MVB_DEV_BLOCK_ID
- * and its tokens are left out. */
+ * and its tokens are left out.  `workspace` holds mvb_paged_prefill_fp8_workspace
+ * bytes (same arguments; 256-byte aligned, contents arbitrary before and after;
+ * 0 bytes, and then unused, unless there are few rows); calls that may overlap on
+ * the GPU need one each. */
 int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, int64_t q_stride_head, const void* key_cache,
                           const void* value_cache, const float* kv_scale, const int64_t* block_table,
                           int64_t block_table_rows, int64_t block_table_stride, int32_t max_blocks_per_seq,
                           const int64_t* seq_rows, const int64_t* cached_len, const int64_t* query_len,
                           int32_t num_chunks, int32_t total_q, void* out, int64_t out_stride_tok,
                           int64_t out_stride_head, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                          int32_t block_size, int32_t num_blocks, float scale, int32_t dtype, int32_t* error_flags,
-                          void* stream);
+                          int32_t block_size, int32_t num_blocks, float scale, int32_t dtype, void* workspace,
+                          int64_t workspace_bytes, int32_t* error_flags, void* stream);
+int mvb_paged_prefill_fp8_workspace(int32_t num_chunks, int32_t total_q, int32_t num_heads, int32_t num_kv_heads,
+                                    int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq,
+                                    int64_t* bytes_out);
 
 #ifdef __cplusplus
 }

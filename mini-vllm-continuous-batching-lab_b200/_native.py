@@ -127,8 +127,9 @@ SIGNATURES = {
     "mvb_paged_prefill_fp8": (
         _i32,
         [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _i64, _i64,
-         _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp],
+         _i32, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _i64, _vp, _vp],
     ),
+    "mvb_paged_prefill_fp8_workspace": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _p_i64]),
 }
 
 _lib = None

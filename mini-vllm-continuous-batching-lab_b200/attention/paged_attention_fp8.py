@@ -386,13 +386,19 @@ def paged_prefill_attention_fp8(
             return out
         query, block_table = _rows(query), _table(block_table, dev)
         num_blocks, num_kv_heads = key_cache.shape[:2]
+        nbytes = ctypes.c_int64()
+        _host_status(_native.lib().mvb_paged_prefill_fp8_workspace(
+            n, total_q, num_heads, num_kv_heads, head_dim, block_size, block_table.shape[1], ctypes.byref(nbytes)),
+            "fp8 paged prefill")
+        ws = _workspace(nbytes.value, dev)
         state = _state(query.get_device())
         status = _native.lib().mvb_paged_prefill_fp8(
             query.data_ptr(), query.stride(0), query.stride(1), key_cache.data_ptr(), value_cache.data_ptr(),
             kv_scale.data_ptr(), block_table.data_ptr(), block_table.shape[0], block_table.stride(0),
             block_table.shape[1], rows.data_ptr(), cached.data_ptr(), qlen.data_ptr(), n, total_q, target.data_ptr(),
             target.stride(0), target.stride(1), num_heads, num_kv_heads, head_dim, block_size, num_blocks,
-            float(scale), _DTYPE_CODES[query.dtype], state.err_ptr, _stream_handle(query.get_device()))
+            float(scale), _DTYPE_CODES[query.dtype], ws.data_ptr() if ws is not None else 0, nbytes.value,
+            state.err_ptr, _stream_handle(query.get_device()))
         _host_status(status, "fp8 paged prefill")
         if target is not out:
             out.copy_(target)

@@ -30,6 +30,10 @@
 // down to 2^-4, where P's f16 still has 10 bits for p >= 2^-10; the rest of a
 // smaller scale goes into the f16 codes (exact to 2^-15 R).
 //
+// Few rows (fewer CTAs than SMs): several CTAs share a row tile's keys, each leaves its
+// result and the log2 of its sum of exponentials in the workspace, and
+// fp8_prefill_merge_kernel joins them.
+//
 // The query enters as f16, each row times a power of two that brings its
 // largest element into [1, 2) (as in the decode kernel, fp8_decode.cu).
 //
@@ -51,6 +55,7 @@
 // Every wait is bounded (kWaitSpinLimit); one that runs out sets
 // MVB_DEV_TIMEOUT, tells the other roles to leave, and the CTA waits (bounded)
 // for its products in flight before it frees its tensor memory.
+#include <algorithm>
 #include <type_traits>
 
 #include "fp8_common.cuh"
@@ -74,6 +79,8 @@ struct Fp8PrefillArgs {
   int64_t o_s0, o_s1;
   int num_heads, num_kv_heads, G, block_shift, num_blocks;
   float scale_log2;
+  int splits;  // CTAs that share the keys of a row tile
+  float* part; // splits > 1: [splits][total_q][num_heads][D] results, then [splits][total_q][num_heads] log2 of sums
   int* err;
 };
 
@@ -89,6 +96,8 @@ constexpr int kStages = 3;          // of K and of V
 constexpr int kNanLag = 3;          // the softmax takes a step's NaN masks this much later
 constexpr int kMasks = kStages + kNanLag;  // steps whose NaN masks are kept
 constexpr int kTmemCols = 512;
+constexpr int kMinSteps = 2;        // of one of the CTAs that share a row tile's keys
+constexpr int kMaxSplits = 16;
 constexpr int kMinValueExp = -4;      // of the part of a value scale that joins the exponent
 
 // Side information of one step, written by the loaders (nan by those of V).
@@ -379,20 +388,38 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   const int q0 = qpre[lo], ql = qpre[lo + 1] - q0, rows = ql * a.G;
   const int row0 = (x - pre[lo]) * kCtaRows;  // the CTA's first row in the chunk
   const int nrows = min(kCtaRows, rows - row0);
+  float* const sums = a.part + (int64_t)a.splits * a.total_q * a.num_heads * D;
+  auto part_row = [&](int r) {  // of the chunk's row r in this CTA's partial results
+    return ((int64_t)blockIdx.z * a.total_q + q0 + r / a.G) * a.num_heads + h0 + r % a.G;
+  };
+  auto nothing = [&]() {  // this CTA adds nothing to its rows
+    for (int r = tid; r < nrows; r += kThreads) sums[part_row(row0 + r)] = -INFINITY;
+  };
   const int64_t srow = __ldg(a.seq_rows + lo), cached = __ldg(a.cached + lo);
   T* const out = static_cast<T*>(a.out);
   if (cached < 0 || srow < 0 || srow >= a.bt_rows ||
       (cached + ql + (1 << a.block_shift) - 1) >> a.block_shift > a.max_blocks) {
     // a table too short for the chunk (or a bad row): zeros, and the flag
     if (tid == 0) atomicOr(a.err, MVB_DEV_TABLE_SHORT);
-    for (int e = tid; e < nrows * D; e += kThreads) {
+    if (a.splits > 1) nothing();
+    for (int e = tid; e < nrows * D && a.splits == 1; e += kThreads) {
       const int r = row0 + e / D;
       out[(int64_t)(q0 + r / a.G) * a.o_s0 + (int64_t)(h0 + r % a.G) * a.o_s1 + e % D] = from_f32<T>(0.f);
     }
     return;
   }
-  const int kv_end = (int)cached + (row0 + nrows - 1) / a.G + 1;  // positions the CTA's last row attends
-  const int steps = (kv_end + kKeys - 1) / kKeys;
+  int kv_end = (int)cached + (row0 + nrows - 1) / a.G + 1;  // positions the CTA's last row attends
+  int steps = (kv_end + kKeys - 1) / kKeys, first = 0;      // this CTA's steps, and its first position
+  if (a.splits > 1) {
+    const int share = max(kMinSteps, (steps + a.splits - 1) / a.splits), from = (int)blockIdx.z * share;
+    if (from >= steps) {
+      nothing();
+      return;
+    }
+    steps = min(share, steps - from);
+    first = from * kKeys;
+    kv_end = min(kv_end - first, steps * kKeys);  // relative to first, as all positions below
+  }
   const int tiles = (nrows + kTileRows - 1) / kTileRows;
 
   Waiter wait;
@@ -433,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       const uint32_t o_at = tmem + lanes + G_::O_COL + tile * D;
       const bool live = r < rows;
       const int tok = live ? r / a.G : 0, head = live ? r - tok * a.G : 0;
-      const int lim = live ? (int)cached + tok + 1 : kv_end;  // rows past the chunk are zeros that attend all
+      const int lim = live ? (int)cached + tok + 1 - first : kv_end;  // rows past the chunk are zeros that attend all
       float qs;
       {
         const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(q0 + tok) * a.q_s0 +
@@ -617,6 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         tc_fence_after();
         for (int j = max(0, steps - kNanLag); j < steps; ++j) take_nan(j);
         const float inv = l == 0.f ? 0.f : infos[(steps - 1) % kInfos].r / l;
+        float4* const pp = reinterpret_cast<float4*>(a.part + (a.splits > 1 ? part_row(live ? r : 0) * D : 0));
+        if (a.splits > 1 && live) sums[part_row(r)] = l == 0.f ? -INFINITY : m + log2f(l);
         T* op = out + (int64_t)(q0 + tok) * a.o_s0 + (int64_t)(h0 + head) * a.o_s1;
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
@@ -624,6 +653,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
           tmem_ld32(o_at + 32 * h, o);
           tc_wait_ld();
           if (!live) continue;
+          if (a.splits > 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = (nanbits[h] >> i) & 1 ? 0x7fffffffu : __float_as_uint(__uint_as_float(o[i]) * inv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pp[8 * h + i] = reinterpret_cast<const float4*>(o)[i];
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint4 w;
@@ -650,9 +687,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     // kBatch steps at a time, one 16-key group per lane: its number among the cache's groups (NONE behind the last
     // key or for a bad block id), and its block's scales.
     auto find = [&](int j0, bool& bad) {
-      const int p = j0 * kKeys + 16 * lane;
+      int p = j0 * kKeys + 16 * lane;
       bad = false;
       if (p >= kv_end) return NONE;
+      p += first;
       const int64_t b = ld_ahead8(bt + (p >> a.block_shift));
       bad = b < 0 || b >= a.num_blocks;
       return bad ? NONE : ((uint32_t)(b * a.num_kv_heads + kvh) << gshift) + ((uint32_t)(p & BSm) >> 4);
@@ -882,15 +920,81 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   if (warp == kMmaWarp) tmem_free(tmem);
 }
 
+// Joins the CTAs' results of a row: out = sum of w_z O_z / sum of w_z, w_z = 2^(sums_z - their maximum).  D / 4
+// threads per row; a few MB that are still in L2.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) fp8_prefill_merge_kernel(const Fp8PrefillArgs a) {
+  __shared__ int s_n[4];
+  const int tid = threadIdx.x;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  int have = 0;  // tokens of all chunks: rows behind them stay
+  for (int i = tid; i < a.n; i += 128)
+    have = min(have + (int)min((int64_t)a.total_q + 1, max((int64_t)0, __ldg(a.qlen + i))), a.total_q + 1);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) have = min(have + __shfl_xor_sync(0xffffffffu, have, o), a.total_q + 1);
+  if (tid % 32 == 0) s_n[tid / 32] = have;
+  __syncthreads();
+  have = min(min(s_n[0] + s_n[1], a.total_q + 1) + min(s_n[2] + s_n[3], a.total_q + 1), a.total_q + 1);
+  if (have > a.total_q) return;  // refused by the kernel before
+  constexpr int TPR = D / 4;
+  const int64_t rows = (int64_t)a.total_q * a.num_heads, row = (int64_t)blockIdx.x * (128 / TPR) + tid / TPR;
+  if (row >= (int64_t)have * a.num_heads) return;
+  const int c = tid % TPR;
+  const float* sums = a.part + a.splits * rows * D;
+  float top = -INFINITY;
+  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, sums[z * rows + row]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int z = 0; z < a.splits; ++z) {
+    const float s = sums[z * rows + row];
+    if (s == -INFINITY) continue;  // nothing was written there
+    const float w = fast_exp2(s - top);
+    const float4 o = reinterpret_cast<const float4*>(a.part + (z * rows + row) * D)[c];
+    acc = make_float4(fmaf(w, o.x, acc.x), fmaf(w, o.y, acc.y), fmaf(w, o.z, acc.z), fmaf(w, o.w, acc.w));
+    l += w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint2 w;
+  T* e = reinterpret_cast<T*>(&w);
+  e[0] = from_f32<T>(acc.x * inv);
+  e[1] = from_f32<T>(acc.y * inv);
+  e[2] = from_f32<T>(acc.z * inv);
+  e[3] = from_f32<T>(acc.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row / a.num_heads) * a.o_s0 + (row % a.num_heads) * a.o_s1 +
+                            4 * c) = w;
+}
+
+int64_t row_tiles(int total_q, int G, int num_chunks) {  // at most
+  return ((int64_t)total_q * G + kCtaRows - 1) / kCtaRows + num_chunks;
+}
+
+// How many CTAs share a row tile's keys: as many as there are SMs for, each with kMinSteps steps or more.  With one
+// CTA and shared (14/2 heads of 64): 20 tokens after 300: 13.7 and 14.4 us, 20 after 600: 20.1 and 14.6, 37 after
+// 1003: 30.1 and 17.5, 512 after 32768: 646 and 175; with four steps or more, 13.8, 17.3, 19.3 and 175.
+int num_splits(int64_t ctas, int64_t max_keys) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t steps = (max_keys + kKeys - 1) / kKeys;
+  const int64_t most = std::min(sms / ctas, std::min<int64_t>(steps / kMinSteps, kMaxSplits));
+  return most > 1 ? (int)most : 1;
+}
+
 template <typename T, int D>
 int launch_prefill_fp8(const Fp8PrefillArgs& a, cudaStream_t stream) {
-  auto kern = fp8_prefill_kernel<T, D>;
   static_assert(2 * (kFp8PrefillMaxChunks + 1) * 4 <= 2 * kStages * Geo<D>::KBYTES, "the prefixes fit the stages");
   static_assert(Geo<D>::BYTES <= 227 * 1024 - 512, "shared memory of one CTA");
+  const int64_t tiles = row_tiles(a.total_q, a.G, a.n);
+  auto kern = fp8_prefill_kernel<T, D>;
   if (ensure_kernel_attrs(kern, Geo<D>::BYTES) != cudaSuccess) return MVB_ERR_CUDA;
-  const int64_t tiles = ((int64_t)a.total_q * a.G + kCtaRows - 1) / kCtaRows + a.n;
-  return launch_pdl(kern, dim3((unsigned)tiles, a.num_kv_heads), dim3(kThreads), Geo<D>::BYTES, stream, a) ==
-                 cudaSuccess
+  if (launch_pdl(kern, dim3((unsigned)tiles, a.num_kv_heads, a.splits), dim3(kThreads), Geo<D>::BYTES, stream, a) !=
+      cudaSuccess)
+    return MVB_ERR_CUDA;
+  if (a.splits == 1) return MVB_OK;
+  auto merge = fp8_prefill_merge_kernel<T, D>;
+  if (ensure_kernel_attrs(merge, 0) != cudaSuccess) return MVB_ERR_CUDA;
+  const int64_t rows = (int64_t)a.total_q * a.num_heads, per = 128 / (D / 4);
+  return launch_pdl(merge, dim3((unsigned)((rows + per - 1) / per)), dim3(128), 0, stream, a) == cudaSuccess
              ? MVB_OK
              : MVB_ERR_CUDA;
 }
@@ -900,6 +1004,40 @@ int launch_prefill_fp8(const Fp8PrefillArgs& a, cudaStream_t stream) {
 
 using namespace mvb;
 
+namespace {
+int plan_prefill(int num_chunks, int total_q, int num_heads, int num_kv_heads, int head_dim, int block_size,
+                 int max_blocks, int* splits, int64_t* bytes) {
+  if (head_dim != 64 && head_dim != 128) return MVB_ERR_HEAD_DIM;
+  if (block_size < kFp8MinBlock || block_size > kFp8MaxBlock || (block_size & (block_size - 1)) != 0)
+    return MVB_ERR_BLOCK_SIZE;
+  if (num_chunks < 0 || num_chunks > kFp8PrefillMaxChunks || total_q < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_kv_heads > 65535 || max_blocks < 0)
+    return MVB_ERR_INVALID_ARG;
+  if (num_heads % num_kv_heads != 0) return MVB_ERR_HEADS;
+  const int G = num_heads / num_kv_heads;
+  // rows of a KV head and positions of a sequence are 32-bit
+  if ((int64_t)total_q * G >= ((int64_t)1 << 30) || (int64_t)max_blocks * block_size >= ((int64_t)1 << 30))
+    return MVB_ERR_INVALID_ARG;
+  *splits = 1;
+  *bytes = 0;
+  if (num_chunks == 0 || total_q == 0) return MVB_OK;
+  *splits = num_splits(row_tiles(total_q, G, num_chunks) * num_kv_heads, (int64_t)max_blocks * block_size);
+  if (*splits > 1) *bytes = (int64_t)*splits * total_q * num_heads * (head_dim + 1) * 4;
+  return MVB_OK;
+}
+}  // namespace
+
+extern "C" int mvb_paged_prefill_fp8_workspace(int32_t num_chunks, int32_t total_q, int32_t num_heads,
+                                               int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                               int32_t max_blocks_per_seq, int64_t* bytes_out) {
+  int splits = 1;
+  int64_t bytes = 0;
+  const int st = plan_prefill(num_chunks, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                              &splits, &bytes);
+  if (st == MVB_OK && bytes_out) *bytes_out = bytes;
+  return st;
+}
+
 extern "C" int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, int64_t q_stride_head,
                                      const void* key_cache, const void* value_cache, const float* kv_scale,
                                      const int64_t* block_table, int64_t block_table_rows,
@@ -907,21 +1045,18 @@ extern "C" int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, in
                                      const int64_t* cached_len, const int64_t* query_len, int32_t num_chunks,
                                      int32_t total_q, void* out, int64_t out_stride_tok, int64_t out_stride_head,
                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-                                     int32_t num_blocks, float scale, int32_t dtype, int32_t* error_flags,
-                                     void* stream) {
+                                     int32_t num_blocks, float scale, int32_t dtype, void* workspace,
+                                     int64_t workspace_bytes, int32_t* error_flags, void* stream) {
   mvb::NvtxRange nvtx_range("mvb_paged_prefill_fp8");
   if (dtype != MVB_DTYPE_F16 && dtype != MVB_DTYPE_BF16) return MVB_ERR_DTYPE;
-  if (head_dim != 64 && head_dim != 128) return MVB_ERR_HEAD_DIM;
-  if (block_size < kFp8MinBlock || block_size > kFp8MaxBlock || (block_size & (block_size - 1)) != 0)
-    return MVB_ERR_BLOCK_SIZE;
-  if (num_chunks < 0 || num_chunks > kFp8PrefillMaxChunks || total_q < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_kv_heads > 65535 || num_blocks <= 0 || max_blocks_per_seq < 0 || block_table_rows < 0)
-    return MVB_ERR_INVALID_ARG;
-  if (num_heads % num_kv_heads != 0) return MVB_ERR_HEADS;
-  const int G = num_heads / num_kv_heads;
-  // rows of a KV head, positions of a sequence, (block, KV head) and 16-token group numbers are 32-bit
-  if ((int64_t)total_q * G >= ((int64_t)1 << 30) || (int64_t)max_blocks_per_seq * block_size >= ((int64_t)1 << 30) ||
-      (int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31) ||
+  int splits = 1;
+  int64_t bytes = 0;
+  const int st = plan_prefill(num_chunks, total_q, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                              &splits, &bytes);
+  if (st != MVB_OK) return st;
+  if (num_blocks <= 0 || block_table_rows < 0) return MVB_ERR_INVALID_ARG;
+  // (block, KV head) and 16-token group numbers are 32-bit
+  if ((int64_t)num_blocks * num_kv_heads >= ((int64_t)1 << 31) ||
       (int64_t)num_blocks * num_kv_heads * (block_size / 16) >= 0xffffffffll)
     return MVB_ERR_INVALID_ARG;
   if (num_chunks == 0 || total_q == 0) return MVB_OK;
@@ -933,6 +1068,7 @@ extern "C" int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, in
   if (!al(query, 16) || q_stride_tok % 8 || q_stride_head % 8 || !al(out, 16) || out_stride_tok % 8 ||
       out_stride_head % 8 || !al(key_cache, 16) || !al(value_cache, 16) || !al(kv_scale, 8))
     return MVB_ERR_ALIGNMENT;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes || !al(workspace, 256))) return MVB_ERR_WORKSPACE;
   Fp8PrefillArgs a;
   a.q = query;
   a.q_s0 = q_stride_tok;
@@ -954,10 +1090,12 @@ extern "C" int mvb_paged_prefill_fp8(const void* query, int64_t q_stride_tok, in
   a.o_s1 = out_stride_head;
   a.num_heads = num_heads;
   a.num_kv_heads = num_kv_heads;
-  a.G = G;
+  a.G = num_heads / num_kv_heads;
   a.block_shift = 31 - __builtin_clz(block_size);
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.splits = splits;
+  a.part = static_cast<float*>(workspace);
   a.err = error_flags;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MVB_DTYPE_BF16)

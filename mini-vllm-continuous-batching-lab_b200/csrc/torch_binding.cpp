@@ -353,18 +353,25 @@ std::tuple<int64_t, at::Tensor> prefill_fp8(const at::Tensor& query, const at::T
     if (!(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type() && out.get_device() == dev &&
           rows16(out)))
       return {kSlowPath, none};
-  } else {
-    out = at::empty(query.sizes(), query.options());
   }
   c10::cuda::CUDAGuard guard(dev);
+  int64_t ws_bytes = 0;
+  int st = mvb_paged_prefill_fp8_workspace((int32_t)seq_rows.size(0), (int32_t)query.size(0), (int32_t)query.size(1),
+                                           (int32_t)kc.size(1), (int32_t)query.size(2), (int32_t)block_size,
+                                           (int32_t)block_table.size(1), &ws_bytes);
+  if (st != MVB_OK) return {st, none};
+  if (!out.defined()) out = at::empty(query.sizes(), query.options());
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = scratch(ws_bytes, dev);
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
-  const int st = mvb_paged_prefill_fp8(
+  st = mvb_paged_prefill_fp8(
       query.data_ptr(), query.stride(0), query.stride(1), kc.data_ptr(), vc.data_ptr(), scale.data_ptr<float>(),
       block_table.data_ptr<int64_t>(), block_table.size(0), block_table.stride(0), (int32_t)block_table.size(1),
       seq_rows.data_ptr<int64_t>(), cached_len.data_ptr<int64_t>(), query_len.data_ptr<int64_t>(),
       (int32_t)seq_rows.size(0), (int32_t)query.size(0), out.data_ptr(), out.stride(0), out.stride(1),
       (int32_t)query.size(1), (int32_t)kc.size(1), (int32_t)query.size(2), (int32_t)block_size, (int32_t)kc.size(0),
-      (float)softmax_scale, dt, reinterpret_cast<int32_t*>(err_ptr), stream);
+      (float)softmax_scale, dt, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, reinterpret_cast<int32_t*>(err_ptr),
+      stream);
   return {st, out};
 }
 

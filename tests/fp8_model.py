@@ -100,7 +100,7 @@ def attend(q, k, v, first, scale):
     A = torch.matmul(p, v.abs()) / total
     prod = torch.matmul(q.abs(), k.abs().transpose(1, 2)).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
     lost = (q.abs().amax(-1, keepdim=True) * 2.0 ** -25) * k.abs().sum(-1).amax(-1)[:, None, None]
-    E = scale * ((D + 4) * 2.0 ** -23 * prod + lost)
+    E = abs(scale) * ((D + 4) * 2.0 ** -23 * prod + lost)
     tol = (2.0 ** -11 + 2 * E + (N + 16) * 2.0 ** -23) * A + N * 2.0 ** -25 * v.abs().amax((1, 2))[:, None, None]
     return out.transpose(0, 1), tol.transpose(0, 1)
 

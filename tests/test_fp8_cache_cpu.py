@@ -102,14 +102,22 @@ def test_library_checks_without_a_gpu():
     assert lib.mvb_paged_decode_fp8_workspace(256, 14, 2, 64, 16, 100, 128, BF16, ctypes.byref(n)) == _native.OK
     assert n.value >= 148 * 2 * (16 + 8 * 66 * 4)
 
-    def p(chunks, total, heads=14, kv=2, dim=64, bs=16, dtype=BF16, ptr=None):
-        return lib.mvb_paged_prefill_fp8(ptr, 64, 64, ptr, ptr, ptr, ptr, 4, 8, 8, ptr, ptr, ptr, chunks, total, ptr, 64,
-                                         64, heads, kv, dim, bs, 100, 0.1, dtype, ptr, None)
+    def p(chunks, total, heads=14, kv=2, dim=64, bs=16, dtype=BF16, ptr=None, maxb=8, ws=None, size=0):
+        return lib.mvb_paged_prefill_fp8(ptr, 64, 64, ptr, ptr, ptr, ptr, 4, 1000, maxb, ptr, ptr, ptr, chunks, total,
+                                         ptr, 64, 64, heads, kv, dim, bs, 100, 0.1, dtype, ws, size, ptr, None)
 
     assert p(0, 5) == _native.OK and p(1, 0) == _native.OK and p(1, 1) == _native.ERR_INVALID_ARG
     assert p(4097, 5000) == _native.ERR_INVALID_ARG and p(1, 1, heads=15) == _native.ERR_HEADS
     assert p(1, 1, dim=32) == _native.ERR_HEAD_DIM and p(1, 1, bs=8) == _native.ERR_BLOCK_SIZE
     assert p(1, 1, dtype=_native.DTYPE_F32) == _native.ERR_DTYPE and p(1, 1, ptr=8) == _native.ERR_ALIGNMENT
+    # few rows after many keys: a workspace
+    assert p(1, 5, ptr=4096, maxb=100) == p(1, 5, ptr=4096, maxb=100, ws=4096, size=64) == _native.ERR_WORKSPACE
+    assert p(1, 5, ptr=4096, maxb=100, ws=4096 + 16, size=1 << 30) == _native.ERR_WORKSPACE
+    w = lambda *c: (lib.mvb_paged_prefill_fp8_workspace(*c, ctypes.byref(n)), n.value)  # noqa: E731
+    assert w(1, 5, 14, 2, 64, 16, 100) == (_native.OK, 12 * 5 * 14 * 65 * 4)  # 25 steps of 64 keys: twelve shares of two or more
+    assert w(1, 5, 14, 2, 64, 16, 12) == w(30, 8192, 14, 2, 64, 16, 1000) == w(0, 0, 14, 2, 64, 16, 0) == (_native.OK, 0)
+    assert w(1, 5, 15, 2, 64, 16, 1)[0] == _native.ERR_HEADS and w(1, 5, 14, 2, 96, 16, 1)[0] == _native.ERR_HEAD_DIM
+    assert w(1, 1 << 28, 14, 2, 64, 16, 1)[0] == w(1, 1, 14, 2, 64, 1024, 1 << 20)[0] == _native.ERR_INVALID_ARG
 
 
 def test_pool_of_8_bits():

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -10,6 +11,7 @@ import torch
 
 import fp8_model as F
 import mini_vllm_b200 as M
+from mini_vllm_b200 import _native
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -680,3 +682,104 @@ def test_decode_one_head_of_nan_leaves_the_others():
     q[0, 3] = 0
     ref, tol = F.attend(q, k, v, 600, 0.125)
     F.check(out[:, keep], ref[:, keep], tol[:, keep])
+
+
+# ---------------------------------------------------------------------------
+# prefill of few rows: CTAs share a row tile's keys
+# ---------------------------------------------------------------------------
+FEW = {"one row": ([5000], [1]), "ragged": ([3000, 0, 255, 1000], [3, 1, 1, 20]), "no short share": ([4095], [1]),
+       "empty shares": ([10, 5000], [3, 1]), "rows end in other shares": ([200], [300]),
+       "with empty": ([2000, 70, 300], [9, 0, 30])}
+
+
+@pytest.mark.parametrize("chunks", list(FEW))
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 8, 128), (16, 1, 128), (5, 5, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prefill_of_few_rows(chunks, heads, dtype):
+    cached, query = FEW[chunks]
+    q, kc, vc, sc, table = prefill_case(40, cached, query, heads, 16, dtype, spare=2)
+    n, rows = len(cached), sum(query)
+    table = torch.cat([table, torch.full((n, 400), -1, dtype=table.dtype, device=DEV)], 1)  # wider than any needs
+    size = _workspace_bytes(n, rows + 2, heads, 16, table.shape[1])
+    assert size >= 2 * (rows + 2) * heads[0] * (heads[2] + 1) * 4  # two shares or more
+    out = torch.full_like(q, 5.0)
+    M.paged_prefill_attention_fp8(q, kc, vc, sc, table, list(range(n)), cached, query, 16, out=out)
+    check_prefill(out[:rows], q, kc, vc, sc, table, cached, query, 16)
+    assert (out[rows:] == 5.0).all()
+
+
+def _workspace_bytes(chunks, total_q, heads, bs, max_blocks):
+    size = ctypes.c_int64()
+    assert _native.lib().mvb_paged_prefill_fp8_workspace(chunks, total_q, *heads, bs, max_blocks,
+                                                         ctypes.byref(size)) == _native.OK
+    return size.value
+
+
+@pytest.mark.parametrize("bs", [128, 1024])
+def test_prefill_of_few_rows_with_wide_scales(bs):
+    """Scales that differ from share to share, and a query that makes one key win."""
+    cached, query, heads = [2900], [40], (14, 2, 64)
+    q, kc, vc, sc, table = prefill_case(41, cached, query, heads, bs, torch.bfloat16)
+    sc *= torch.exp2(torch.randint(-6, 6, sc.shape, generator=gen(42), device=DEV).float())
+    assert _workspace_bytes(1, 40, heads, bs, table.shape[1]) > 0
+    for scale in (0.125, 2.0, -0.3):
+        out = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, [0], cached, query, bs, scale=scale)
+        check_prefill(out, q, kc, vc, sc, table, cached, query, bs, scale=scale)
+
+
+def test_prefill_of_few_rows_nan_and_errors():
+    cached, query, (H, KH, D), bs = [1000], [30], (14, 2, 64), 16
+    q, kc, vc, sc, table = prefill_case(43, cached, query, (H, KH, D), bs, torch.float16)
+    assert _workspace_bytes(1, 30, (H, KH, D), bs, table.shape[1]) > 0
+    call = lambda t, c=cached, n=query, **kw: M.paged_prefill_attention_fp8(q, kc, vc, sc, t, [0], c, n, bs, **kw)  # noqa: E731
+    plain = call(table)
+    for p, h, d in ((300, 0, 3), (1015, 1, 17)):  # in the first shares, and in the last one from row 15 on
+        bits(vc)[table[0, p // bs], h, p % bs, d] = 0xFF
+    out = call(table)
+    want = torch.zeros_like(out, dtype=torch.bool)
+    want[:, :7, 3] = True
+    want[15:, 7:, 17] = True
+    assert torch.equal(torch.isnan(out), want)
+    assert torch.equal(torch.where(want, 0, out), torch.where(want, 0, plain))
+    q[4, 2, 5] = float("nan")
+    out = call(table)
+    want[4, 2] = True
+    assert torch.equal(torch.isnan(out), want)
+    with pytest.raises(IndexError, match="insufficient"):
+        call(table, [1011], [30])  # 1041 positions, a table of 65 blocks
+    out = call(table, [1100], [30], strict=False)
+    assert (out == 0).all()
+    with pytest.raises(IndexError):
+        M.check_device_errors(DEV)
+    out = torch.full_like(q, 5.0)
+    with pytest.raises(IndexError):
+        call(table, [900], [31], out=out)  # more tokens than query has rows
+    assert (out == 5.0).all()
+    t = table.clone()
+    t[0, 10] = -1
+    with pytest.raises(IndexError, match="block_table entry"):
+        call(t)
+    M.check_device_errors(DEV)
+
+
+def test_prefill_of_few_rows_captured_on_two_streams():
+    """Each call has results of its own between its kernels: two graphs at once, with an eager call between."""
+    cases = [prefill_case(s, [3000, 500], [20, 7], (14, 2, 64), 16, torch.bfloat16) for s in (44, 45)]
+    idx = [torch.tensor(x, device=DEV) for x in ([0, 1], [3000, 500], [20, 7])]
+    want = [M.paged_prefill_attention_fp8(*c, *idx, 16) for c in cases]
+    graphs, outs = [], []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            outs.append(M.paged_prefill_attention_fp8(*c, *idx, 16, strict=False))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = M.paged_prefill_attention_fp8(*cases[0], *idx, 16, strict=False)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(eager, want[0])
