@@ -377,6 +377,8 @@ int mvb_paged_decode_noalloc(const void* query, int64_t q_stride_seq, int64_t q_
  * [num_blocks][num_kv_heads][block_size][head_dim]; kv_scale, float32
  * [num_blocks][num_kv_heads][2], holds the scale of the keys and the scale of
  * the values of each (block, KV head).  An element stands for code * scale.
+ * The writes below make powers of two; the attention takes any positive finite
+ * scales (a block whose scale is 0, as in a new pool, holds zeros).
  * Caches are 16-byte, kv_scale 8-byte aligned; block_size is a power of two
  * from 16 to 1024, head_dim 64 or 128, dtype (of query, key, value and output)
  * f16 or bf16.  Rows of query, key, value and outputs are 16-byte aligned
@@ -393,10 +395,10 @@ int mvb_paged_decode_noalloc(const void* query, int64_t q_stride_seq, int64_t q_
  * round is to the nearest e4m3 value, ties to even; max runs over the finite
  * elements, infinities are stored as +-448 s, NaN as NaN.  A block is to be
  * filled from slot 0 on.  Two tokens with one slot set MVB_DEV_DUP_SLOT (one of
- * the two is written).  The call needs
- * the bytes of workspace that mvb_kv_cache_write_fp8_workspace reports (0 for few tokens; 4-byte aligned, contents arbitrary before and
- * after); calls that may overlap on the GPU need one each.  Calls that write
- * to one block must be ordered. */
+ * the two is written).  The call needs the bytes of workspace that
+ * mvb_kv_cache_write_fp8_workspace reports (0 up to 2048 tokens; 4-byte aligned,
+ * contents arbitrary before and after); calls that may overlap on the GPU need
+ * one each.  Calls that write to one block must be ordered. */
 int mvb_kv_cache_write_fp8(const void* key, int64_t k_stride_token, int64_t k_stride_head, const void* value,
                            int64_t v_stride_token, int64_t v_stride_head, void* key_cache, void* value_cache,
                            float* kv_scale, const int64_t* slot_mapping, int32_t num_tokens, int32_t num_kv_heads,
@@ -407,11 +409,13 @@ int mvb_kv_cache_write_fp8_workspace(int32_t num_tokens, int32_t num_blocks, int
 /* Rotary embedding of the step's query and key rows fused with
  * mvb_kv_cache_write_fp8 of the rotated keys and the values:
  *   out = x * cos[pos] + rotate_half(x) * sin[pos]
- * (mini_vllm/model/rotary.py:47-85) computed in float32 and rounded once: to
- * dtype for query_out and key_out, to the cache's codes for the keys (the
- * exact rotation rounded to float32 is what is coded).  The tables are
- * contiguous [table_rows, head_dim] of `table_dtype`, which is dtype or
- * MVB_DTYPE_F32.  query_out may equal query; key_out (optional) is contiguous
+ * (mini_vllm/model/rotary.py:47-85) computed in float32 as one product, rounded,
+ * and one fused multiply-add, and rounded once more: to dtype for query_out and
+ * key_out, to the cache's codes for the keys.  A scale is that of the exact
+ * rotation rounded to float32; a code can differ from the exact rotation's only
+ * where that lies within 2^-23 of sum |products| of a tie.  The tables are
+ * contiguous [table_rows, head_dim] (fewer than 2^31 rows) of `table_dtype`,
+ * which is dtype or MVB_DTYPE_F32.  query_out may equal query; key_out (optional) is contiguous
  * [T, KH, D].  A position outside [0, table_rows) sets MVB_DEV_POSITION and
  * leaves all of that token's rows unwritten; slot -1 rotates the query and
  * writes nothing. */
@@ -428,7 +432,8 @@ int mvb_rope_kv_cache_write_fp8(const void* query, int64_t q_stride_token, int64
 
 /* Paged decode attention over the 8-bit cache, one query token per sequence;
  * arguments, zero rows and device errors as in mvb_paged_decode (at most 6144
- * sequences).  `workspace` holds mvb_paged_decode_fp8_workspace bytes (same
+ * sequences, num_blocks * num_kv_heads * block_size below 2^31), and
+ * MVB_DEV_TIMEOUT when a bounded wait on the device runs out.  `workspace` holds mvb_paged_decode_fp8_workspace bytes (same
  * arguments; 256-byte aligned, contents arbitrary before and after); calls
  * that may overlap on the GPU need one each. */
 int mvb_paged_decode_fp8(const void* query, int64_t q_stride_seq, int64_t q_stride_head, const void* key_cache,
@@ -444,8 +449,8 @@ int mvb_paged_decode_fp8_workspace(int32_t num_seqs, int32_t num_heads, int32_t 
 
 /* Causal paged prefill attention over the 8-bit cache: mvb_paged_prefill with
  * every position, the chunk's own among them, read from the cache (written
- * before the call).  A block id outside [0, num_blocks) sets MVB_DEV_BLOCK_ID
- * and its tokens are left out.  `workspace` holds mvb_paged_prefill_fp8_workspace
+ * before the call; at most 4096 chunks).  A block id outside [0, num_blocks) sets
+ * MVB_DEV_BLOCK_ID and its tokens are left out; MVB_DEV_TIMEOUT as above.  `workspace` holds mvb_paged_prefill_fp8_workspace
  * bytes (same arguments; 256-byte aligned, contents arbitrary before and after;
  * 0 bytes, and then unused, unless there are few rows); calls that may overlap on
  * the GPU need one each. */

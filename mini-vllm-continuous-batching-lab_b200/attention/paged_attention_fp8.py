@@ -17,8 +17,9 @@ The cache of one layer is three tensors:
 ``head_dim`` 64 or 128, bf16 or f16 queries, keys and values, and a ``block_size``
 that is a power of two from 16 to 1024.
 
-Scales are powers of two and belong to whole blocks: ``paged_cache_write_fp8`` says
-how they follow the rows that come in.
+Scales belong to whole blocks: ``paged_cache_write_fp8`` says how they follow the rows
+that come in.  The writes make powers of two; the attention takes any positive finite
+scales, such as a calibration's (a block whose scale is 0, as in a new pool, holds zeros).
 """
 
 from __future__ import annotations
@@ -200,9 +201,9 @@ def rope_cache_write_fp8(
     the values (``mvb_rope_kv_cache_write_fp8``).
 
     ``cos`` / ``sin`` are tables ``[rows, head_dim]`` (see ``rope_tables``) in the rows' dtype or in float32.
-    The rotation is computed in float32 and rounded once, to the rows' dtype for the query and the returned
-    keys, to the cache's codes for the written ones (``rope_cache_write`` rounds after each operation, as the
-    reference does).  Returns the rotated query (into ``query_out`` when given, which may be ``query`` itself
+    The rotation is computed in float32 (a product and a fused multiply-add) and rounded once more, to the
+    rows' dtype for the query and the returned keys, to the cache's codes for the written ones
+    (``rope_cache_write`` rounds after each operation, as the reference does).  Returns the rotated query (into ``query_out`` when given, which may be ``query`` itself
     and overlaps no other argument) and, with ``return_key``, the rotated keys.  A position outside the tables
     raises ``IndexError`` and leaves that token's rows unwritten; a token with slot -1 has its query rotated and
     writes nothing.
@@ -293,7 +294,8 @@ def paged_decode_attention_fp8(
     Arguments, result and errors are ``paged_decode_attention``'s, with ``kv_scale`` beside the caches.  The
     query enters the tensor cores as f16 (a bf16 row by a power of two, exact but for elements below 2**-14 of
     its largest), probabilities as f16; logits, sums and the output are accumulated in float32.  The result does
-    not depend on timing.  At most 6144 sequences.  The call keeps no state between calls and may be captured.
+    not depend on timing.  At most 6144 sequences, and fewer than 2**31 cache rows (blocks * KV heads * block
+    size).  The call keeps no state between calls and may be captured.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5
@@ -357,8 +359,10 @@ def paged_prefill_attention_fp8(
 
     Arguments and result are ``paged_prefill_attention``'s, with ``kv_scale`` beside the caches and without
     ``key`` / ``value``: every position is read from the cache, where the chunk has been written before.
-    Token ``t`` of chunk ``i`` attends positions ``[0, cached_len[i] + t]``.  Precision is
-    ``paged_decode_attention_fp8``'s.
+    Token ``t`` of chunk ``i`` attends positions ``[0, cached_len[i] + t]``.  At most 4096 chunks; rows behind
+    the last chunk's stay as they are.  Precision is ``paged_decode_attention_fp8``'s, but that a value whose
+    block's scale is below ``2**-4`` of the sequence's largest keeps it as f16 in units of that one: exact down
+    to ``2**-15`` of it.
     """
     _require(query.dim() == 3, lambda: f"query must be [total_q, num_heads, head_dim], got {tuple(query.shape)}")
     if scale is None:

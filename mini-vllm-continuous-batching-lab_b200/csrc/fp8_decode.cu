@@ -32,14 +32,19 @@
 //
 // Work split: the tiles of all (sequence, KV head, head group) units in order
 // are one stream, cut into equal ranges, one per warp of a grid of at most one
-// CTA per SM.  A unit inside a warp's range is written at once.  The pieces of
+// CTA per SM (or each unit is a CTA's own: see kFp8WholeTiles).  A unit inside a warp's range is written at once.  The pieces of
 // units cut between the warps of a CTA are merged in shared memory; only a unit
 // cut between two CTAs leaves partial states in global memory, which
 // fp8_decode_merge_kernel joins in CTA order.  The workspace holds nothing from
 // one call to the next and needs no initialisation.
-// Bound: memory (1 byte per element; 28 operations per byte at 7 heads).
+// Bound: memory (1 byte per element; 28 operations per byte at 7 heads), short
+// sequences by the launches and the first loads.  Measured: 256 sequences of 32/8
+// heads of 128, 817 MB: 146 us, 5.6 TB/s; 32 x 32768 tokens of 14/2 heads of 64,
+// 270 MB: 59 us, 4.6 TB/s; 256 x 2048: 29 us, 16 of them the stream (4.7 TB/s), the
+// rest prologue and merges.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fp8_common.cuh"
@@ -62,6 +67,7 @@ struct Fp8DecodeArgs {
   int64_t o_s0, o_s1;
   int num_seqs, num_heads, num_kv_heads, G, head_groups, block_shift, num_blocks;
   float scale_log2;
+  int whole;    // a CTA per unit, each with all of its tiles
   float* part;  // [grid][2][16 * (D + 2)] partial states of units cut between CTAs: O, then (m, l)
   int4* desc;   // [grid][2] {unit (-1: none), sequence, first head, heads}; slot 0: the unit began earlier
   int* err;
@@ -75,6 +81,14 @@ constexpr int kFp8DecodeMaxSeqs = 6144;  // the tile prefix lies in shared memor
 constexpr float kMinValueExp = -4.f, kMaxValueExp = 7.f;
 // A warp gets at least this many tiles where the batch has few.
 constexpr int kFp8MinTiles = 2;
+// A CTA takes a unit of its own, and nothing is left to merge in a second launch, where
+// there are SMs for all units, a unit has at most kFp8WholeTiles tiles per warp, and
+// that is at most kFp8WholeMore more than an equal share of the stream would be: a
+// tile costs a warp about 0.7 us, the merge 3 to 4.  Shared and whole (us): 1 x 1000,
+// 14/2 heads of 64: 10.6 and 9.4; 64 x 1000: 14.7 and 10.7; 64 x 2000: 18.1 and 13.7;
+// 16 x 1500, 32/8 of 128: 19.0 and 15.4; but 1 x 2000: 10.8 and 12.3, 1 x 4000: 11.6
+// and 18.5.  The first limit is for tables wider than most sequences need.
+constexpr int kFp8WholeTiles = 8, kFp8WholeMore = 4;
 
 // Geometry by head_dim and column blocks: warps per CTA and tiles in a warp's
 // ring.  The rings, a piece per warp and the prefix of the largest batch fill
@@ -178,7 +192,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
       const int bad = c < 1 ? MVB_DEV_KV_LEN
                       : ((int64_t)c + (1 << a.block_shift) - 1) >> a.block_shift > a.max_blocks ? MVB_DEV_TABLE_SHORT
                                                                                                : 0;
-      const int n = bad ? 0 : ((c + kFp8Tile - 1) / kFp8Tile) * KHG;
+      const int n = bad ? 0 : ((c - 1) / kFp8Tile + 1) * KHG;
       pre[i] = n;
       mine += n;
       if (bad && blockIdx.x == 0) atomicOr(a.err, bad);
@@ -212,12 +226,19 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
       out[(int64_t)i * a.o_s0 + (int64_t)(e / D) * a.o_s1 + e % D] = from_f32<T>(0.f);
   }
 
-  const int T_all = pre[Nd];
-  const int ctas = min((int)gridDim.x, max(1, (T_all + NW * kFp8MinTiles - 1) / (NW * kFp8MinTiles)));
-  const int W = min(ctas * NW, max(T_all, 1)), wid = blockIdx.x * NW + warp;
-  auto bound = [&](int w) { return (int)((int64_t)min(w, W) * T_all / W); };
-  const int r0 = bound(wid), r1 = bound(wid + 1);
-  const int c0 = bound(blockIdx.x * NW), c1 = bound(blockIdx.x * NW + NW);
+  // this CTA's share of the stream, [base, base + T), or with others' all of it, and the first of its W warps there
+  int base = 0, T_all = pre[Nd], ctas = gridDim.x, first = blockIdx.x * NW;
+  if (a.whole) {
+    const int seq = blockIdx.x / KHG;
+    T_all = (pre[seq + 1] - pre[seq]) / KHG;
+    base = pre[seq] + (blockIdx.x - seq * KHG) * T_all;
+    ctas = 1;
+    first = 0;
+  }
+  const int W = min(min(ctas, max(1, (T_all + NW * kFp8MinTiles - 1) / (NW * kFp8MinTiles))) * NW, max(T_all, 1));
+  auto bound = [&](int w) { return base + (int)((int64_t)min(w, W) * T_all / W); };
+  const int r0 = bound(first + warp), r1 = bound(first + warp + 1);
+  const int c0 = bound(first), c1 = bound(first + NW);
 
   auto unit_at = [&](int tile) {
     int lo = 0, hi = Nd;  // pre[lo] <= tile < pre[hi]
@@ -777,18 +798,22 @@ __global__ void __launch_bounds__(256) fp8_decode_merge_kernel(const Fp8DecodeAr
   }
 }
 
-// CTAs of the stream kernel: one per SM, fewer where the tables bound the work.
-int decode_grid(int num_seqs, int units_per_seq, int max_blocks, int block_size, int nw) {
+// CTAs of the stream kernel: one per SM, fewer where the tables bound the work; or one per unit.
+int decode_grid(int num_seqs, int units_per_seq, int max_blocks, int block_size, int nw, int* whole) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t tiles = (int64_t)num_seqs * units_per_seq * ((int64_t)max_blocks * block_size / kFp8Tile);
+  const int64_t units = (int64_t)num_seqs * units_per_seq, unit_tiles = (int64_t)max_blocks * block_size / kFp8Tile;
+  const int64_t mine = (unit_tiles + nw - 1) / nw, share = std::max<int64_t>(kFp8MinTiles, units * unit_tiles / (sms * nw));
+  *whole = units <= sms && mine <= kFp8WholeTiles && mine - share <= kFp8WholeMore;
+  if (*whole) return (int)std::max<int64_t>(units, 1);
+  const int64_t tiles = units * unit_tiles;
   const int64_t per = (int64_t)nw * kFp8MinTiles;
   const int64_t want = (tiles + per - 1) / per;
   return (int)(want < 1 ? 1 : want < sms ? want : sms);
 }
 
 struct Fp8DecodePlan {
-  int head_groups, ng, nw, grid;
+  int head_groups, ng, nw, grid, whole;
   int64_t off_part, bytes;
 };
 
@@ -812,7 +837,7 @@ int plan_decode(int num_seqs, int num_heads, int num_kv_heads, int head_dim, int
   if ((int64_t)num_seqs * units * ((int64_t)max_blocks * block_size / kFp8Tile + 1) >= ((int64_t)1 << 31) ||
       (int64_t)num_blocks * num_kv_heads * block_size >= ((int64_t)1 << 31))
     return MVB_ERR_INVALID_ARG;
-  pl->grid = decode_grid(num_seqs, units, max_blocks, block_size, pl->nw);
+  pl->grid = decode_grid(num_seqs, units, max_blocks, block_size, pl->nw, &pl->whole);
   pl->off_part = ((int64_t)pl->grid * 32 + 255) / 256 * 256;
   pl->bytes = pl->off_part + (int64_t)pl->grid * 2 * 16 * (head_dim + 2) * 4;
   return MVB_OK;
@@ -841,7 +866,7 @@ int launch_decode(const Fp8DecodeArgs& a, int grid, cudaStream_t stream) {
   // the largest batch's size at once: the attribute is set on the first call only
   if (ensure_kernel_attrs(kern, Fp8Smem<D, NG>::bytes(kFp8DecodeMaxSeqs)) != cudaSuccess) return MVB_ERR_CUDA;
   if (launch_pdl(kern, dim3(grid), dim3(Fp8Geo<D, NG>::NW * 32), smem, stream, tmk, tmv, a) != cudaSuccess) return MVB_ERR_CUDA;
-  if (grid == 1) return MVB_OK;  // no unit is cut between CTAs
+  if (grid == 1 || a.whole) return MVB_OK;  // no unit is cut between CTAs
   auto merge = fp8_decode_merge_kernel<T, D, 8 * NG>;
   if (ensure_kernel_attrs(merge, 0) != cudaSuccess) return MVB_ERR_CUDA;
   return launch_pdl(merge, dim3(grid), dim3(256), 0, stream, a, grid) == cudaSuccess ? MVB_OK : MVB_ERR_CUDA;
@@ -910,6 +935,7 @@ extern "C" int mvb_paged_decode_fp8(const void* query, int64_t q_stride_seq, int
   a.num_kv_heads = num_kv_heads;
   a.G = num_heads / num_kv_heads;
   a.head_groups = pl.head_groups;
+  a.whole = pl.whole;
   a.block_shift = 31 - __builtin_clz(block_size);
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * 1.4426950408889634f;

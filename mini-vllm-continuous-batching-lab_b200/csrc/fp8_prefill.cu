@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   };
   const int64_t srow = __ldg(a.seq_rows + lo), cached = __ldg(a.cached + lo);
   T* const out = static_cast<T*>(a.out);
-  if (cached < 0 || srow < 0 || srow >= a.bt_rows ||
+  if (cached < 0 || cached > (int64_t)a.max_blocks << a.block_shift || srow < 0 || srow >= a.bt_rows ||
       (cached + ql + (1 << a.block_shift) - 1) >> a.block_shift > a.max_blocks) {
     // a table too short for the chunk (or a bad row): zeros, and the flag
     if (tid == 0) atomicOr(a.err, MVB_DEV_TABLE_SHORT);

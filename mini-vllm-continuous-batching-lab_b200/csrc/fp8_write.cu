@@ -38,7 +38,9 @@
 // launch: a thread holds 8 + 8 columns of two heads of one token (four, where there
 // are many tokens), so the cos and sin rows are read once for them.
 // Bound: memory for long chunks; for a decode step the latency of slots ->
-// rows -> maximum -> codes.
+// rows -> maximum -> codes.  Measured: 9721 tokens of 32/8 heads of 128, 229 MB:
+// 61 us, 3.7 TB/s (instructions: each row is rotated twice, for the maximum and
+// for the codes); 1048 tokens 11.7 us; 256 tokens of a decode step 3 to 4 us.
 #include <type_traits>
 
 #include "fp8_common.cuh"

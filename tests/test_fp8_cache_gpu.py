@@ -783,3 +783,44 @@ def test_prefill_of_few_rows_captured_on_two_streams():
         eager = M.paged_prefill_attention_fp8(*cases[0], *idx, 16, strict=False)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(eager, want[0])
+
+
+@pytest.mark.parametrize("lens,width", [([1000], 0), ([2048], 0), ([1, 16, 17, 700, 1000, 33], 0), ([0, 900, 0], 0),
+                                        ([100] * 74, 0), ([100] * 75, 0), ([300, 40], 200), ([1, 5], 0)])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 2, 64), (16, 2, 128), (24, 2, 128)])
+def test_decode_of_few_short_sequences(lens, width, heads):
+    """Units that a CTA takes whole, and lengths and tables beside the limits of that."""
+    q, kc, vc, sc, table, kvl = decode_case(50, lens, heads, 16, torch.bfloat16)
+    if width:
+        table = torch.cat([table, torch.full((len(lens), width), -1, dtype=table.dtype, device=DEV)], 1)
+    out = M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16, strict=False)
+    kept = [i for i, n in enumerate(lens) if n > 0]
+    check_decode(out[kept], q[kept], kc, vc, sc, table[kept], [lens[i] for i in kept], 16)
+    assert all((out[i] == 0).all() for i, n in enumerate(lens) if n == 0)
+    again = M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16, strict=False)
+    assert torch.equal(out, again)
+    if 0 in lens:
+        with pytest.raises(ValueError):
+            M.check_device_errors(DEV)
+    M.check_device_errors(DEV)
+
+
+def test_scales_of_zero_and_lengths_past_any_table():
+    """A block whose scale is 0 holds zeros; lengths near the integers' ends are refused, not followed."""
+    lens, heads = [200, 90], (14, 2, 64)
+    q, kc, vc, sc, table, kvl = decode_case(51, lens, heads, 16, torch.bfloat16)
+    sc[table[0, 3]] = 0.0
+    sc[table[0, 0], :, 1] = 0.0
+    out = M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16)
+    check_decode(out, q, kc, vc, sc, table, lens, 16)
+    rows, cached, one = (torch.tensor(x, device=DEV) for x in ([0, 1], [199, 89], [1, 1]))
+    got = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, rows, cached, one, 16)
+    check_prefill(got, q, kc, vc, sc, table, [199, 89], [1, 1], 16)
+    for far in (2 ** 31 - 1, 2 ** 62, 2 ** 63 - 1):
+        cached[0] = far
+        with pytest.raises(IndexError):
+            M.paged_prefill_attention_fp8(q, kc, vc, sc, table, rows, cached, one, 16)
+    kvl[0] = 2 ** 31 - 1
+    with pytest.raises(IndexError):
+        M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16)
+    M.check_device_errors(DEV)
