@@ -824,3 +824,58 @@ def test_scales_of_zero_and_lengths_past_any_table():
     with pytest.raises(IndexError):
         M.paged_decode_attention_fp8(q, kc, vc, sc, table, kvl, 16)
     M.check_device_errors(DEV)
+
+
+@pytest.mark.parametrize("n", [3, 100])
+def test_captured_step_writes_then_attends(n):
+    """A decode step in one graph (rotation and write, then attention), replayed as the sequences grow, against
+    the same calls made one by one; the sequences share their first block."""
+    H, KH, D, bs, width = 14, 2, 64, 16, 20
+    g = gen(60)
+    start = torch.randint(16, 290, (n,), generator=g, device=DEV)
+    table = 1 + torch.arange(n * width, device=DEV).reshape(n, width)
+    table[:, 0] = 0
+    a = make_cache(g, n * width + 1, KH, bs, D)
+    b = tuple(x.clone() for x in a)
+    cos, sin = M.rope_tables(D, 10000.0, 512, torch.float32, DEV)
+    rows = lambda h: torch.randn(n, h, D, generator=g, device=DEV).bfloat16()  # noqa: E731
+    q, k, v, pos, slots = rows(H), rows(KH), rows(KH), start.clone(), torch.zeros_like(start)
+    kvl = torch.zeros(n, dtype=torch.int32, device=DEV)
+
+    def step(q, k, v, cache):
+        qr, _ = M.rope_cache_write_fp8(q, k, v, pos, cos, sin, *cache, slots, bs, strict=False)
+        return M.paged_decode_attention_fp8(qr, *cache, table, kvl, bs, strict=False)
+
+    def at(p):  # the step of position p
+        pos.copy_(p)
+        slots.copy_(table.gather(1, (p // bs)[:, None])[:, 0] * bs + p % bs)
+        kvl.copy_(p + 1)
+
+    at(start)
+    step(q, k, v, b)
+    b = tuple(x.clone() for x in a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(q, k, v, a)
+    for i in range(20):
+        at(start + i)
+        for x, h in ((q, H), (k, KH), (v, KH)):
+            x.copy_(rows(h))
+        graph.replay()
+        want = step(q, k, v, b)
+        assert torch.equal(out, want) and all(torch.equal(bits(x), bits(y)) for x, y in zip(a, b))
+    check_decode(out, M.rope_cache_write_fp8(q, k, v, pos, cos, sin, *b, torch.full_like(slots, -1), bs)[0], *a, table,
+                 kvl.tolist(), bs)
+    M.check_device_errors(DEV)
+
+
+def test_prefill_chunks_of_one_sequence():
+    """The same row of the table twice, in any order of its chunks."""
+    q, kc, vc, sc, table = prefill_case(61, [400], [100], (14, 2, 64), 16, torch.bfloat16)
+    whole = M.paged_prefill_attention_fp8(q, kc, vc, sc, table, [0], [400], [100], 16)
+    parts = torch.cat([q[60:], q[:60]])
+    out = M.paged_prefill_attention_fp8(parts, kc, vc, sc, table, [0, 0], [460, 400], [40, 60], 16)
+    check_prefill(out[:40], parts[:40], kc, vc, sc, table, [460], [40], 16)
+    check_prefill(out[40:], parts[40:], kc, vc, sc, table, [400], [60], 16)
+    check_prefill(whole, q, kc, vc, sc, table, [400], [100], 16)
