@@ -44,11 +44,14 @@
 // Bound: a step (256 rows, 64 keys) has 1024 cycles of exponentials (16 per cycle
 // and SM) and, for head_dim 128, 1024 of the tensor core.  It takes about 2400: the
 // scores are always there when a softmax warp looks, and its own instructions in
-// turn (two such warps per scheduler) are what the step waits for.  Tried and slower
-// or equal: columns read 32 or 64 at a time; four row tiles of one S buffer each
-// (16 softmax warps, but each then waits for its products: 318 against 287 us for
-// 8192 tokens); 128 keys a step with one buffer of S (278 us there, but 939 against
-// 834 us for head_dim 128, whose P then has to wait in registers for S to be read).
+// turn (two such warps per scheduler) are what the step waits for; no unit is busy
+// for half of the time.  Tried (8192 tokens, against 287 us): columns read 32 or 64
+// at a time: 308, 298; four row tiles of one S buffer each (16 softmax warps, each
+// of which then waits for its products): 318; two warps per row, each with half of a
+// step's keys and an O of its own: 284 to 290, and 20 against 17.5 us for 37 tokens;
+// loaders that bring two steps at once: 296; 128 keys a step with one buffer of S:
+// 278, but 939 against 834 us for head_dim 128, whose P then has to wait in registers
+// for S to be read.
 // Measured: 8192 tokens, 14/2 heads of 64: 287 us, 420 TFLOP/s; 4 x 2048 tokens,
 // 32/8 heads of 128 after 3000 to 6144 cached: 834 us, 760 TFLOP/s.
 //
