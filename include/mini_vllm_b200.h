@@ -409,11 +409,10 @@ int mvb_kv_cache_write_fp8_workspace(int32_t num_tokens, int32_t num_blocks, int
 /* Rotary embedding of the step's query and key rows fused with
  * mvb_kv_cache_write_fp8 of the rotated keys and the values:
  *   out = x * cos[pos] + rotate_half(x) * sin[pos]
- * (mini_vllm/model/rotary.py:47-85) computed in float32 as one product, rounded,
- * and one fused multiply-add, and rounded once more: to dtype for query_out and
- * key_out, to the cache's codes for the keys.  A scale is that of the exact
- * rotation rounded to float32; a code can differ from the exact rotation's only
- * where that lies within 2^-23 of sum |products| of a tie.  The tables are
+ * (mini_vllm/model/rotary.py:47-85).  Scales and codes of the keys are those of
+ * the exact rotation rounded to float32; query_out and key_out are computed in
+ * float32 as one product, rounded, and one fused multiply-add, and rounded to
+ * dtype.  The tables are
  * contiguous [table_rows, head_dim] (fewer than 2^31 rows) of `table_dtype`,
  * which is dtype or MVB_DTYPE_F32.  query_out may equal query; key_out (optional) is contiguous
  * [T, KH, D].  A position outside [0, table_rows) sets MVB_DEV_POSITION and

@@ -201,8 +201,8 @@ def rope_cache_write_fp8(
     the values (``mvb_rope_kv_cache_write_fp8``).
 
     ``cos`` / ``sin`` are tables ``[rows, head_dim]`` (see ``rope_tables``) in the rows' dtype or in float32.
-    The rotation is computed in float32 (a product and a fused multiply-add) and rounded once more, to the
-    rows' dtype for the query and the returned keys, to the cache's codes for the written ones
+    The written keys' scales and codes are those of the exact rotation rounded to float32; the query and the
+    returned keys are computed in float32 (a product and a fused multiply-add) and rounded to the rows' dtype
     (``rope_cache_write`` rounds after each operation, as the reference does).  Returns the rotated query (into ``query_out`` when given, which may be ``query`` itself
     and overlaps no other argument) and, with ``return_key``, the rotated keys.  A position outside the tables
     raises ``IndexError`` and leaves that token's rows unwritten; a token with slot -1 has its query rotated and

@@ -15,12 +15,12 @@
 // holds does not depend on how its tokens were split into calls but for those.
 // The maximum runs over the finite elements; an infinity is stored as +-448 s.
 //
-// A rotated row is a product and a fused multiply-add in float32: the exact
-// rotation rounded once but for the product's rounding, which matters only beside
-// a tie (about one code in 2^20 differs from the exact rotation's).  A maximum
-// within 4 ulps of 448 * 2^k decides about a scale, so there it is taken again
-// from exact sums (rope_exact); sums exact everywhere were half of the kernel's
-// instructions.
+// Queries and returned keys are a product and a fused multiply-add in float32.
+// With float32 tables the product is rounded, so beside a tie one code in 2^20
+// would differ from the exact rotation's: the keys are coded from sums with their
+// rounding errors added back (rope_exact; 63.7 against 60.8 us for the chunks
+// below).  Their maximum is taken without; only one within 4 ulps of 448 * 2^k
+// decides about a scale, and there it is taken again.
 //
 // Work split.  A block's scale needs the maximum over all the call's rows of the
 // block, so its rows belong together, with the CTA of the block's leader: the
@@ -39,7 +39,7 @@
 // are many tokens), so the cos and sin rows are read once for them.
 // Bound: memory for long chunks; for a decode step the latency of slots ->
 // rows -> maximum -> codes.  Measured: 9721 tokens of 32/8 heads of 128, 229 MB:
-// 61 us, 3.7 TB/s (instructions: each row is rotated twice, for the maximum and
+// 64 us, 3.6 TB/s (instructions: each row is rotated twice, for the maximum and
 // for the codes); 1048 tokens 11.7 us; 256 tokens of a decode step 3 to 4 us.
 #include <type_traits>
 
@@ -82,10 +82,11 @@ __device__ __forceinline__ float rope(float x, float c, float y, float s) {
 }
 // The same rounded once for float32 tables: the products and the sum with their
 // rounding errors (exact by fma and by Knuth's two-sum), added back at the end.
-__device__ __noinline__ float rope_exact(float x, float c, float y, float s) {
+__device__ __forceinline__ float rope_exact(float x, float c, float y, float s) {
   const float p1 = __fmul_rn(x, c), e1 = __fmaf_rn(x, c, -p1);
   const float p2 = __fmul_rn(y, s), e2 = __fmaf_rn(y, s, -p2);
   const float t = __fadd_rn(p1, p2);
+  if (!(fabsf(t) < INFINITY)) return t;  // (the errors of infinities are NaN)
   const float b = __fsub_rn(t, p1);
   const float e3 = __fadd_rn(__fsub_rn(p1, __fsub_rn(t, b)), __fsub_rn(p2, b));
   return __fadd_rn(t, __fadd_rn(e3, __fadd_rn(e1, e2)));
@@ -328,7 +329,7 @@ __device__ __forceinline__ void write_block(const Fp8WriteArgs& a, const int* ma
       for (int p = 0; p < NP; ++p) {
         if (at[p] < 0) continue;
         uint2 l, h;
-        row(p, std::false_type(), [&](int half, const float (&lo)[4], const float (&hi)[4]) {
+        row(p, std::bool_constant<ROT && sizeof(TAB) == 4>(), [&](int half, const float (&lo)[4], const float (&hi)[4]) {
           (half ? l.y : l.x) = f32x4_to_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv);
           (half ? h.y : h.x) = f32x4_to_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv);
         });

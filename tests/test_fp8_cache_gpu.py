@@ -879,3 +879,25 @@ def test_prefill_chunks_of_one_sequence():
     check_prefill(out[:40], parts[:40], kc, vc, sc, table, [460], [40], 16)
     check_prefill(out[40:], parts[40:], kc, vc, sc, table, [400], [60], 16)
     check_prefill(whole, q, kc, vc, sc, table, [400], [100], 16)
+
+
+@pytest.mark.parametrize("tokens", [1500, 4000])
+def test_write_codes_are_those_of_the_exact_rotation(tokens):
+    """Float32 tables: every key's code is that of the exact rotation rounded to float32, ties among 4 million too
+    (a rotation by a rounded product and a fused multiply-add has another code about once in 2^20); infinities
+    and NaN as ever."""
+    g = gen(70)
+    H, KH, D, bs = 8, 8, 128, 16
+    kc, vc, sc = make_cache(g, tokens // bs + 1, KH, bs, D)
+    mk, mv, ms = kc.cpu(), vc.cpu(), sc.cpu()
+    q, k, v, pos, cos, sin = write_case(g, tokens, (H, KH, D), torch.bfloat16, torch.float32)
+    slots = torch.arange(tokens, device=DEV)
+    M.rope_cache_write_fp8(q, k, v, pos, cos, sin, kc, vc, sc, slots, bs)
+    F.write(F.rotate(k, cos, sin, pos).cpu(), v.float().cpu(), mk, mv, ms, slots.cpu(), bs)
+    for a, b in ((kc, mk), (vc, mv), (sc, ms)):
+        assert torch.equal(bits(a).cpu(), bits(b))
+    k = k.clone()
+    k[3, 0, 5], k[4, 1, 70], pos[3:5] = float("inf"), float("nan"), 0  # (position 0: by cos 1 and sin 0)
+    M.rope_cache_write_fp8(q, k, v, pos, cos, sin, kc, vc, sc, slots, bs)
+    codes = kc[0].float()
+    assert codes[0, 3, 5] == 448 and torch.isnan(codes[1, 4, 70]) and torch.isnan(codes[0]).sum() <= 1
