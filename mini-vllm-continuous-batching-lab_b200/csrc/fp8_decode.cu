@@ -543,34 +543,13 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
             v[b][4 * i] = x.x, v[b][4 * i + 1] = x.y, v[b][4 * i + 2] = x.z, v[b][4 * i + 3] = x.w;
           }
         }
-      // P against the maximum of earlier tiles; taken anew where a lane's P add up to more than 2^14
+      // P against the maximum of earlier tiles, which is taken anew, once, where a lane's P add up to more than 2^14.
+      // An exponent is a fused multiply-add: its product is not rounded, so it can lie half an ulp of m above the
+      // maximum of the rounded ones (2^4 from |m| = 2^28 on).  Against a maximum just taken it is therefore the
+      // difference of the rounded ones: 0 at the largest, nowhere above the tile's ve, whatever the logits' size.
       uint32_t pb[NT][NG][2];
-      for (bool anew = fresh;;) {
-        if (anew) {
-#pragma unroll
-          for (int n = 0; n < NG; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float mx = m[n][c];
-#pragma unroll
-              for (int b = 0; b < NT; ++b) {
-                if (tok_g < valid[b]) mx = fmaxf(mx, s[b][n][c] * (qs[n][c] * ks[b]));
-                if (tok_g + 8 < valid[b]) mx = fmaxf(mx, s[b][n][c + 2] * (qs[n][c] * ks[b]));
-              }
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float al = m[n][c] == mx ? 1.f : fast_exp2(m[n][c] - mx);
-              m[n][c] = mx;
-              l[n][c] *= al;
-#pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                o[n][i][c] *= al;
-                o[n][i][c + 2] *= al;
-              }
-            }
-        }
-        float t[NT][NG][2];
+      float t[NT][NG][2];
+      auto weights = [&](auto anew) {
         bool over = false;
 #pragma unroll
         for (int b = 0; b < NT; ++b)
@@ -578,7 +557,13 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
           for (int n = 0; n < NG; ++n) {
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = fmaf(s[b][n][i], qs[n][i & 1] * ks[b], ve[b] - m[n][i & 1]);
+            for (int i = 0; i < 4; ++i) {
+              const float f = __fmul_rn(qs[n][i & 1], ks[b]), top = m[n][i & 1];
+              if constexpr (decltype(anew)::value)  // (all of them -inf: P is 0)
+                y[i] = __fadd_rn(__fsub_rn(__fmul_rn(s[b][n][i], f), top == -INFINITY ? 0.f : top), ve[b]);
+              else
+                y[i] = fmaf(s[b][n][i], f, ve[b] - top);
+            }
             if (edge) {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
@@ -592,22 +577,49 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant
             pb[b][n][0] = pack_h2(y[0], y[1]);
             pb[b][n][1] = pack_h2(y[2], y[3]);
           }
-        anew = __any_sync(0xffffffffu, over);
-        if (anew) continue;
+        return over;
+      };
+      // (fresh: some maximum is -inf still)
+      if (fresh || __any_sync(0xffffffffu, weights(std::false_type()))) {
+        bool none = false;
 #pragma unroll
-        for (int b = 0; b < NT; ++b) {
-          const float vu = fast_exp2(-ve[b]);
+        for (int n = 0; n < NG; ++n)
 #pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            l[n][0] = fmaf(t[b][n][0], vu, l[n][0]);
-            l[n][1] = fmaf(t[b][n][1], vu, l[n][1]);
-            pb[b][n][0] = movmatrix(pb[b][n][0]);
-            pb[b][n][1] = movmatrix(pb[b][n][1]);
+          for (int c = 0; c < 2; ++c) {
+            float mx = m[n][c];
+#pragma unroll
+            for (int b = 0; b < NT; ++b) {
+              const float f = __fmul_rn(qs[n][c], ks[b]);
+              if (tok_g < valid[b]) mx = fmaxf(mx, __fmul_rn(s[b][n][c], f));
+              if (tok_g + 8 < valid[b]) mx = fmaxf(mx, __fmul_rn(s[b][n][c + 2], f));
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float al = m[n][c] == mx ? 1.f : fast_exp2(m[n][c] - mx);
+            m[n][c] = mx;
+            none |= mx == -INFINITY;
+            l[n][c] *= al;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              o[n][i][c] *= al;
+              o[n][i][c + 2] *= al;
+            }
           }
-        }
-        break;
+        fresh = __any_sync(0xffffffffu, none);
+        weights(std::true_type());
       }
-      if (fresh) fresh = __any_sync(0xffffffffu, m[0][0] == -INFINITY);  // (nothing but bad blocks so far)
+#pragma unroll
+      for (int b = 0; b < NT; ++b) {
+        const float vu = fast_exp2(-ve[b]);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          l[n][0] = fmaf(t[b][n][0], vu, l[n][0]);
+          l[n][1] = fmaf(t[b][n][1], vu, l[n][1]);
+          pb[b][n][0] = movmatrix(pb[b][n][0]);
+          pb[b][n][1] = movmatrix(pb[b][n][1]);
+        }
+      }
       // O^T += V^T P^T; rows past the last token may hold any bits
       if (edge) {
 #pragma unroll

@@ -1,0 +1,63 @@
+"""Attention over the 8-bit cache where logits are finite and very large: it ends, and the largest key's value comes
+out (tests/test_fp8_large_logits_cpu.py has the arithmetic)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import fp8_model as F
+import mini_vllm_b200 as M
+from fp8_large_logits import CASES, HEADS, case, winners
+
+DEV = torch.device("cuda", 0)
+
+
+def check(out, q, kc, vc, sc, table, spans, bs, scale):
+    """Rows with a winner hold its value: off by P's rounding to f16 (2^-11), which numerator and denominator do not
+    share, float32 sums (2^-20 is ample) and the output's own.  The others lie between the values."""
+    at = 0
+    for i, (length, rows) in enumerate(spans):
+        ref, sure, most = winners(q[at:at + rows], kc, vc, sc, table[i], length, bs, scale)
+        got = out[at:at + rows].double().cpu()
+        assert torch.isfinite(got).all()
+        unit = F.UNIT[out.dtype]
+        off = (2.0 ** -11 + 2.0 ** -20) * ref.abs()
+        limit = torch.where(sure[..., None], off + unit * (ref.abs() + off) + 2.0 ** -25, math.inf)
+        assert ((got - ref).abs() <= limit).all()
+        assert (got.abs() <= most * (1 + 2.0 ** -7) + 2.0 ** -25).all()
+        at += rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("name", list(CASES))
+def test_decode(name, heads):
+    lens = [700, 1, 40, 17, 333]
+    q, kc, vc, sc, table, scale = case(name, [(n, 1) for n in lens], heads, 16)
+    kvl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    dev = [x.to(DEV) for x in (q, kc, vc, sc, table)]
+    wide = torch.cat([dev[4], torch.full((5, 400), -1, dtype=torch.int64, device=DEV)], 1)
+    # units cut between CTAs (as a wide table may need), and (a narrow table, short sequences) whole ones
+    for keep in (slice(0, 5), slice(1, 4)):
+        sub = wide if keep.start == 0 else dev[4][keep, :3].contiguous()
+        out = M.paged_decode_attention_fp8(dev[0][keep], *dev[1:4], sub, kvl[keep], 16, scale=scale)
+        check(out, q[keep], kc, vc, sc, table[keep], [(n, 1) for n in lens[keep]], 16, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+def test_decode_logits_that_overflow(heads):
+    """Logits below float32's range count for nothing; other sequences of the batch are as ever."""
+    lens = [300, 45]
+    q, kc, vc, sc, table, _ = case("negative", [(n, 1) for n in lens], heads, 16)
+    scale = 2e37
+    q[1] *= 1e-33
+    kvl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    out = M.paged_decode_attention_fp8(*(x.to(DEV) for x in (q, kc, vc, sc, table)), kvl, 16, scale=scale)
+    assert (out[0] == 0).all()
+    check(out[1:], q[1:], kc, vc, sc, table[1:], [(45, 1)], 16, scale)
+    out = M.paged_decode_attention_fp8(*(x.to(DEV) for x in (-q, kc, vc, sc, table)), kvl, 16, scale=scale)
+    assert torch.isnan(out[0]).all()  # above it: as infinities are
