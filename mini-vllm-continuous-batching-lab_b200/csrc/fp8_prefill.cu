@@ -13,7 +13,7 @@
 //     exponentials against a maximum of earlier steps and reads S once.  P may then
 //     exceed 1; only when 16 of them add up to more than 2^14 (so that f16 never
 //     overflows) is the maximum taken anew, O rescaled in tensor memory and the
-//     step repeated.  P goes to tensor memory as f16, over S;
+//     step repeated, once.  P goes to tensor memory as f16, over S;
 //   * one that loads K and one that loads V.  They copy codes through the block
 //     table one step ahead into shared memory (cp.async; block ids and scales are
 //     read eight to sixteen steps ahead), turn them into f16 (exact) and store tiles
@@ -52,10 +52,10 @@
 // loaders that bring two steps at once: 296; 128 keys a step with one buffer of S:
 // 278, but 939 against 834 us for head_dim 128, whose P then has to wait in registers
 // for S to be read.
-// Measured: 8192 tokens, 14/2 heads of 64: 287 us, 420 TFLOP/s; 4 x 2048 tokens,
-// 32/8 heads of 128 after 3000 to 6144 cached: 834 us, 760 TFLOP/s.
+// Measured: 8192 tokens, 14/2 heads of 64: 275 us, 437 TFLOP/s; 4 x 2048 tokens,
+// 32/8 heads of 128 after 3000 to 6144 cached: 820 us, 770 TFLOP/s.
 //
-// Every wait is bounded (kWaitSpinLimit); one that runs out sets
+// Every wait is bounded (kWaitSpinLimit), as every loop is; one that runs out sets
 // MVB_DEV_TIMEOUT, tells the other roles to leave, and the CTA waits (bounded)
 // for its products in flight before it frees its tensor memory.
 #include <algorithm>
@@ -206,6 +206,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // Shared-memory operand in the 128-byte swizzle: `lead` and `stride` in bytes.
@@ -457,12 +463,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
   if (warp < kLoadWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G_::SOFTMAX));
     // ================================ softmax =================================
-    const int tile = warp >> 2, r = row0 + tile * kTileRows + (warp & 3) * 32 + lane;
+    const int tile = warp >> 2, r0 = row0 + tile * kTileRows + (warp & 3) * 32 + lane;
     if (tile < tiles) {
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t o_at = tmem + lanes + G_::O_COL + tile * D;
-      const bool live = r < rows;
-      const int tok = live ? r / a.G : 0, head = live ? r - tok * a.G : 0;
+      const bool live = r0 < rows;
+      const int tok = live ? r0 / a.G : 0, head = live ? r0 - tok * a.G : 0;
       const int lim = live ? (int)cached + tok + 1 - first : kv_end;  // rows past the chunk are zeros that attend all
       float qs;
       {
@@ -514,8 +520,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
             for (int i = 0; i < D / 32; ++i)
               nanbits[i] |= reinterpret_cast<const uint32_t*>(masks + ((j % kMasks) * kKeys + k) * (D / 16))[i];
       };
-      // One step of the softmax; EDGE: it holds keys that some row does not attend.
-      auto step = [&](int j, auto edge, bool anew, float rf) {
+      enum { kLeave, kDone, kAnew };  // a wait ran out; the step is done; it wants its maximum taken anew
+      // One step of the softmax.  EDGE: it takes its maximum anew, or holds keys that some row does not attend
+      // (`masked`); one form for both: with the second pass in each form, 8192 tokens took 293 us for 275.
+      auto step = [&](int j, auto edge, bool anew, bool masked, float rf) {
         constexpr bool EDGE = decltype(edge)::value;
         const StepInfo& f = infos[j % kInfos];
         const int rem = lim - j * kKeys;
@@ -527,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
           tmem_ld16(s_at + CW * h, s[h & 1]);
         };
         auto mask = [&](int h) {  // -inf where the row does not attend the key
-          if constexpr (EDGE) {
+          if (EDGE && masked) {
             const int bad = f.bad >> (CW / 16 * h), n = rem - CW * h;
 #pragma unroll
             for (int i = 0; i < CW; ++i)
@@ -537,38 +545,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         auto factor = [&](float ks) { return fmaxf(qs * ks, 1.2e-38f); };  // (not 0: -inf stays -inf)
         float fac = rf;
         bool move = rf != 1.f;
+        // P against the maximum at hand; whether 16 of them add up to more than 2^14
         uint32_t p[kKeys / 2];
-        for (;;) {
-          if (anew) {
-            float mx = m;
-#pragma unroll
-            for (int h = 0; h < NC; ++h) {
-              read(h);
-              tc_wait_ld();
-              mask(h);
-#pragma unroll
-              for (int g = 0; g < CW / 16; ++g) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 16; i += 2)
-                  top = fmaxf(fmaxf(top, __uint_as_float(s[h & 1][16 * g + i])),
-                              __uint_as_float(s[h & 1][16 * g + i + 1]));
-                mx = fmaxf(mx, top * factor(f.g[CW / 16 * h + g].x));
-              }
-            }
-            const float al = mx == m ? 1.f : fast_exp2(m - mx);  // (0 for a row's first keys, where l and O are 0)
-            m = mx;
-            l *= al;
-            fac *= al;
-            move = true;
-          }
+        float sum = 0.f;
+        auto weights = [&]() {
           read(NC - 1);
           float4 info[2][CW / 16];  // of the columns at hand and of the next ones
 #pragma unroll
           for (int g = 0; g < CW / 16; ++g) info[(NC - 1) & 1][g] = f.g[CW / 16 * (NC - 1) + g];
-          // a row that has attended nothing yet: m and all of s are -inf, and P is 0
-          const float base = EDGE && m == -INFINITY ? 0.f : -m;
-          float sum = 0.f, most = 0.f;
+          float most = 0.f;
 #pragma unroll
           for (int h = NC - 1; h >= 0; --h) {
             const uint32_t(&x)[CW] = s[h & 1];
@@ -582,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
 #pragma unroll
             for (int gg = 0; gg < CW / 16; ++gg) {
               const float4 in = info[h & 1][gg];
-              const float c = factor(in.x), b = base + in.y;
+              const float c = factor(in.x), b = in.y - m;
               const float2 cc = make_float2(c, c), mm = make_float2(b, b);
               float2 t[2];
 #pragma unroll
@@ -599,17 +584,70 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
               sum = fmaf(u, in.z, sum);
             }
           }
-          anew = __any_sync(0xffffffffu, most > 16384.f);
-          if (!anew) {
-            l += sum;
-            break;
+          return most > 16384.f;
+        };
+        const bool holds = !anew && !__any_sync(0xffffffffu, weights());
+        if (!EDGE && !holds) return kAnew;
+        if (!EDGE || holds) {
+          tmem_st16(s_at, p);
+          tmem_st16(s_at + 16, p + 16);
+        } else {
+          float mx = m;
+#pragma unroll
+          for (int h = 0; h < NC; ++h) {
+            if (h == 0) read(0);
+            tc_wait_ld();
+            if (h + 1 < NC) read(h + 1);
+            mask(h);
+#pragma unroll
+            for (int g = 0; g < CW / 16; ++g) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; i += 2)
+                top = fmaxf(fmaxf(top, __uint_as_float(s[h & 1][16 * g + i])), __uint_as_float(s[h & 1][16 * g + i + 1]));
+              mx = fmaxf(mx, __fmul_rn(top, factor(f.g[CW / 16 * h + g].x)));
+            }
+          }
+          const float al = mx == m ? 1.f : fast_exp2(m - mx);  // (0 for a row's first keys, where l and O are 0)
+          m = mx;
+          l *= al;
+          fac *= al;
+          move = true;
+          // The exponents above are fused multiply-adds: their products are not rounded, so they can lie half an ulp of
+          // m above the maximum of the rounded ones (2^4 from |m| = 2^28 on).  Against this maximum they are therefore
+          // differences of the rounded ones: 0 at the largest, nowhere above the group's part of the value scale (2^7),
+          // whatever the logits' size.  (A row that has attended nothing yet: m and all of s are -inf, and P is 0.)
+          const float base = m == -INFINITY ? 0.f : -m;
+          sum = 0.f;
+          static_assert(CW == 16, "a group's P covers scores that have been read");
+#pragma unroll
+          for (int h = 0; h < NC; ++h) {
+            if (h == 0) read(0);
+            const float4 in = f.g[h];
+            const float c = factor(in.x);
+            const float2 mm = make_float2(base, base), vv = make_float2(in.y, in.y);
+            tc_wait_ld();
+            if (h + 1 < NC) read(h + 1);
+            mask(h);
+            float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              // (packed products are joined with the sum behind them, for all their rounding modes)
+              float2 e = make_float2(__fmul_rn(__uint_as_float(s[h & 1][i]), c), __fmul_rn(__uint_as_float(s[h & 1][i + 1]), c));
+              e = add2(add2(e, mm), vv);
+              e.x = fast_exp2(e.x);
+              e.y = fast_exp2(e.y);
+              t = add2(t, e);
+              p[i / 2] = pack_h2(e.x, e.y);
+            }
+            sum = fmaf(t.x + t.y, in.z, sum);
+            tmem_st8(s_at + 8 * h, p);
           }
         }
-        tmem_st16(s_at, p);
-        tmem_st16(s_at + 16, p + 16);
+        l += sum;
         if (move && j > 0) {
           // the last step's products add to O
-          if (!wait.warp(kPvDone + tile * NB + (j - 1) % NB, ((j - 1) / NB) & 1)) return false;
+          if (!wait.warp(kPvDone + tile * NB + (j - 1) % NB, ((j - 1) / NB) & 1)) return kLeave;
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < D / 32; ++h) {
@@ -625,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(wait.bar(kPReady + tile * NB + j % NB));
-        return true;
+        return kDone;
       };
       const int least = __reduce_min_sync(0xffffffffu, lim);
       bool ok = true, fresh = true;
@@ -641,12 +679,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
         ok = wait.warp(kSFull + tile * NB + j % NB, (j / NB) & 1);
         if (!ok) break;
         tc_fence_after();
-        ok = edge || bad ? step(j, std::true_type(), fresh, rf) : step(j, std::false_type(), fresh, rf);
+        const bool masked = edge || bad;
+        int did = masked || fresh ? kAnew : step(j, std::false_type(), false, false, rf);
+        if (did == kAnew) did = step(j, std::true_type(), fresh || !masked, masked, rf);
+        ok = did == kDone;
       }
       if (ok && wait.warp(kPvDone + tile * NB + (steps - 1) % NB, ((steps - 1) / NB) & 1)) {
         tc_fence_after();
         for (int j = max(0, steps - kNanLag); j < steps; ++j) take_nan(j);
         const float inv = l == 0.f ? 0.f : infos[(steps - 1) % kInfos].r / l;
+        int r = r0;
+        asm("" : "+r"(r));  // (the row's place, worked out again and not kept in registers through the steps)
+        const bool live = r < rows;
+        const int tok = live ? r / a.G : 0, head = live ? r - tok * a.G : 0;
         float4* const pp = reinterpret_cast<float4*>(a.part + (a.splits > 1 ? part_row(live ? r : 0) * D : 0));
         if (a.splits > 1 && live) sums[part_row(r)] = l == 0.f ? -INFINITY : m + log2f(l);
         T* op = out + (int64_t)(q0 + tok) * a.o_s0 + (int64_t)(h0 + head) * a.o_s1;

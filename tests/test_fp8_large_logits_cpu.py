@@ -71,7 +71,7 @@ def test_products_that_overflow():
     assert m == 4.0 and p[3] == 1.0 and p.sum() == 1.0
 
 
-@pytest.mark.parametrize("source", ["fp8_decode.cu"])
+@pytest.mark.parametrize("source", ["fp8_decode.cu", "fp8_prefill.cu"])
 def test_every_loop_has_a_bound_in_its_head(source):
     text = open(os.path.join(CSRC, source)).read()
     assert not re.search(r"for \([^;]*;\s*;|while \((true|1)\)", text)
@@ -96,3 +96,17 @@ def test_the_inputs_have_winners_and_the_logits_they_say():
                 top = x.amax(-1)
                 assert (top.abs() >= 2.0 ** 23).all() and (top.abs() <= 2.0 ** 43).all()
                 assert (torch.sign(top) == (1 if sign * scale > 0 else -1)).all()
+
+
+def test_most_rows_of_chunks_have_winners():
+    import fp8_large_logits as L
+
+    for name in L.CASES:
+        for spans in ([(700, 700), (1, 1), (300, 200)], [(2100, 20), (50, 3), (17, 1)]):
+            for heads in L.HEADS[:2]:
+                q, kc, vc, sc, table, scale = L.case(name, spans, heads, 16)
+                at = 0
+                for i, (n, rows) in enumerate(spans):
+                    _, sure, _ = L.winners(q[at:at + rows], kc, vc, sc, table[i], n, 16, scale)
+                    assert sure.double().mean() > 0.9
+                    at += rows

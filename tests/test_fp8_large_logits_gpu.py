@@ -61,3 +61,38 @@ def test_decode_logits_that_overflow(heads):
     check(out[1:], q[1:], kc, vc, sc, table[1:], [(45, 1)], 16, scale)
     out = M.paged_decode_attention_fp8(*(x.to(DEV) for x in (-q, kc, vc, sc, table)), kvl, 16, scale=scale)
     assert torch.isnan(out[0]).all()  # above it: as infinities are
+
+
+# chunks whose rows fill the card's CTAs, and few rows, whose keys several CTAs share
+SPANS = {"many rows": [(700, 700), (1, 1), (300, 200)], "few rows": [(2100, 20), (50, 3), (17, 1)]}
+
+
+def prefill(q, kc, vc, sc, table, spans, bs, scale):
+    rows, cached, qlen = (torch.tensor(x, device=DEV) for x in
+                          (range(len(spans)), [n - r for n, r in spans], [r for _, r in spans]))
+    return M.paged_prefill_attention_fp8(*(x.to(DEV) for x in (q, kc, vc, sc, table)), rows, cached, qlen, bs,
+                                         scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("name", list(CASES))
+@pytest.mark.parametrize("spans", list(SPANS))
+def test_prefill(spans, name, heads):
+    spans = SPANS[spans]
+    q, kc, vc, sc, table, scale = case(name, spans, heads, 16)
+    check(prefill(q, kc, vc, sc, table, spans, 16, scale), q, kc, vc, sc, table, spans, 16, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+def test_prefill_logits_that_overflow(heads):
+    for spans in SPANS.values():
+        q, kc, vc, sc, table, _ = case("negative", spans, heads, 16)
+        scale, first = 2e37, spans[0][1]
+        q[first:] *= 1e-33
+        out = prefill(q, kc, vc, sc, table, spans, 16, scale)
+        assert (out[:first] == 0).all()
+        check(out[first:], q[first:], kc, vc, sc, table[1:], spans[1:], 16, scale)
+        out = prefill(-q, kc, vc, sc, table, spans, 16, scale)
+        assert torch.isnan(out[:first]).all()
