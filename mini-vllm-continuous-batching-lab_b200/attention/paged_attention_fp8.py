@@ -80,14 +80,15 @@ def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
 
 
 def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(tensor to return, tensor the kernel writes): the second is a copy where the rows are not aligned."""
+    """(tensor to return, tensor the kernel writes): the second is a copy where the rows are not aligned, which the
+    caller copies back whole: rows that the kernel leaves alone keep what they held."""
     if out is None:
         out = torch.empty(like.shape, dtype=like.dtype, device=like.device)
         return out, out
     _require(out.shape == like.shape and out.dtype == like.dtype and out.device == like.device,
              lambda: f"{name} must match query's shape, dtype and device")
     _require(out.stride(2) == 1, lambda: f"{name}'s last dimension must be contiguous")
-    return out, out if _aligned(out) else torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    return out, _rows(out)
 
 
 def _raise_write(state, slot_mapping, key_cache, block_size, table_rows=None) -> None:
