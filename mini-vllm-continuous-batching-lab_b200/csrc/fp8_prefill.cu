@@ -25,10 +25,11 @@
 // Scales.  A block's key scale is one factor of 16 columns of S (a group), so it
 // joins the softmax scale in the exponent's multiply-add at no cost.  A value
 // scale v joins the exponent too: P = p v / R, with the sum of p undone per
-// group, and O is in units of R, a power of two.  R is the first step's largest
-// scale and moves (O with it) when a scale passes 2^7 R.  The exponent takes v / R
-// down to 2^-4, where P's f16 still has 10 bits for p >= 2^-10; the rest of a
-// smaller scale goes into the f16 codes (exact to 2^-15 R).
+// group, and O is in units of R, a power of two.  R is the largest scale of the
+// first step that has one above 0, and moves (O with it) when a scale passes
+// 2^7 R.  The exponent takes v / R down to 2^-4, where P's f16 still has 10 bits
+// for p >= 2^-10; the rest of a smaller scale goes into the f16 codes (exact to
+// 2^-15 R).
 //
 // Few rows (fewer CTAs than SMs): several CTAs share a row tile's keys, each leaves its
 // result and the log2 of its sum of exponentials in the workspace, and
@@ -772,14 +773,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
     fetch(0, grp);
     const float2 sc = scales(grp);
     float2 sc_n = make_float2(0.f, 0.f);
-    int RE = 127;        // exponent field of R
+    int RE = 0;          // exponent field of R (0: no value scale has given it yet)
     uint32_t rests = 0;  // lanes whose group's value scale goes into the codes in part
     float rest = 1.f;
     // The side information of kBatch steps from j on; each lane's part of its group's scale that goes into the codes
     // of V, and the lanes where that is not 1.
     auto side_info = [&](int j, float2 sc, uint32_t grp, bool bad, float& rest, uint32_t& rests) {
       const int vexp = (int)(__float_as_uint(sc.y) >> 23) & 0xff;  // 0: a scale of 0 or below 2^-126
-      int top = vexp, mine = 0;  // largest exponent field of the step; R's of this lane's step
+      int top = vexp, mine = 127;  // largest exponent field of the step; R's of this lane's step
       float rf = 1.f;
 #pragma unroll
       for (int o = 1; o < kGroups; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -787,13 +788,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_prefill_kernel(const Fp8Prefi
       for (int k = 0; k < kBatch; ++k) {
         const int t = __shfl_sync(0xffffffffu, top, k * kGroups);
         const int was = RE;
-        if (j + k == 0)
-          RE = t > 0 ? t : 127;
-        else if (t > RE + 7)
-          RE = t;
-        if (lane / kGroups == k) {
+        if (RE == 0 || t > RE + 7) RE = t;
+        if (lane / kGroups == k && RE > 0) {  // (before that O is 0, in any unit)
           mine = RE;
-          if (j + k > 0 && RE != was) rf = RE - was < 127 ? __uint_as_float((uint32_t)(127 + was - RE) << 23) : 0.f;
+          if (was > 0 && RE != was) rf = RE - was < 127 ? __uint_as_float((uint32_t)(127 + was - RE) << 23) : 0.f;
         }
       }
       const int e = vexp > 0 ? vexp - mine : 0, ep = max(e, kMinValueExp);
