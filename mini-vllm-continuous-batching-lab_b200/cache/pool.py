@@ -83,7 +83,7 @@ class KVCachePool:
         values = [torch.empty(shape, dtype=dtype, device=dev) for _ in range(num_layers)]
         scales = None
         if dtype == torch.float8_e4m3fn:
-            scales = [torch.zeros((num_blocks, num_kv_heads, 2), device=dev) for _ in range(num_layers)]
+            scales = [torch.zeros((num_blocks, num_kv_heads, 2), dtype=torch.float32, device=dev) for _ in range(num_layers)]
         return KVCachePool(keys, values, num_blocks, block_size, num_layers, num_kv_heads,
                            head_dim, dev, dtype, scales)
 
