@@ -153,7 +153,9 @@ def paged_cache_write_fp8(
 
     So a block is filled from its slot 0 on, over any number of calls.  Two tokens with one slot raise
     ``AssertionError``, a slot outside the cache ``IndexError`` (with ``strict=False``: at
-    ``check_device_errors``).  The call may be captured in a graph.
+    ``check_device_errors``).  The call may be captured in a graph.  More than 2048 tokens take 4 bytes of
+    scratch per slot of the cache from torch's allocator (a captured graph keeps its own), which
+    ``compute_num_gpu_blocks`` leaves room for once.
     """
     fast = _native.fast()
     if fast is not None and key.is_cuda:

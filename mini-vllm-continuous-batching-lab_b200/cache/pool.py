@@ -134,8 +134,9 @@ def compute_num_gpu_blocks(
     """Blocks that fit in free device memory (budget rule of reference pool.py:174-278).
 
     ``budget = (free - peak_runtime_estimate - workspace_reserve) * utilization``
-    divided by the bytes one block takes across all layers (K and V), never
-    below ``MIN_BLOCKS``.  An override is returned as-is after the minimum check.
+    divided by the bytes one block takes across all layers (K and V; for an 8-bit
+    pool its scales and the scratch of one long write too), never below
+    ``MIN_BLOCKS``.  An override is returned as-is after the minimum check.
     """
     if not (0 < gpu_memory_utilization <= 1.0):
         raise ValueError(f"gpu_memory_utilization must be in (0, 1], got {gpu_memory_utilization}")
@@ -161,4 +162,6 @@ def compute_num_gpu_blocks(
         )
     budget = int(post * gpu_memory_utilization)
     per_block = num_layers * _block_bytes(num_kv_heads, block_size, head_dim, dtype)
+    if dtype == torch.float8_e4m3fn:
+        per_block += 4 * block_size  # scratch of a write of more than 2048 tokens: an int32 per slot, for all layers
     return max(MIN_BLOCKS, budget // per_block)
