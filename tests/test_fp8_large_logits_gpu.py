@@ -96,3 +96,25 @@ def test_prefill_logits_that_overflow(heads):
         check(out[first:], q[first:], kc, vc, sc, table[1:], spans[1:], 16, scale)
         out = prefill(-q, kc, vc, sc, table, spans, 16, scale)
         assert torch.isnan(out[:first]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("last", [False, True])
+def test_some_keys_overflow(last, heads):
+    """160 positions whose logits are below float32's range, before or behind 140 that count."""
+    n, rows = 300, 4
+    q, kc, vc, sc, table, _ = case("negative", [(n, rows)], heads, 16)
+    scale = 2e37
+    kept = table[:, :9] if last else table[:, 10:]
+    length = 144 if last else 140
+    sc[kept[0], :, 0] *= 1e-33
+    out = prefill(q, kc, vc, sc, table, [(n, rows)], 16, scale)
+    one = M.paged_decode_attention_fp8(*(x.to(DEV) for x in (q[-1:], kc, vc, sc, table)),
+                                       torch.tensor([n], dtype=torch.int32, device=DEV), 16, scale=scale)
+    if last:  # every row attends all of what counts
+        for r in range(rows):
+            check(out[r:r + 1], q[r:r + 1], kc, vc, sc, kept, [(length, 1)], 16, scale)
+    else:
+        check(out, q, kc, vc, sc, kept, [(length, rows)], 16, scale)
+    check(one, q[-1:], kc, vc, sc, kept, [(length, 1)], 16, scale)
