@@ -377,8 +377,8 @@ int mvb_paged_decode_noalloc(const void* query, int64_t q_stride_seq, int64_t q_
  * [num_blocks][num_kv_heads][block_size][head_dim]; kv_scale, float32
  * [num_blocks][num_kv_heads][2], holds the scale of the keys and the scale of
  * the values of each (block, KV head).  An element stands for code * scale.
- * The writes below make powers of two; the attention takes any positive finite
- * scales (a block whose scale is 0, as in a new pool, holds zeros).
+ * The writes below make powers of two; the attention takes any positive normal
+ * float32 scales (a block whose scale is 0 holds zeros).
  * Caches are 16-byte, kv_scale 8-byte aligned; block_size is a power of two
  * from 16 to 1024, head_dim 64 or 128, dtype (of query, key, value and output)
  * f16 or bf16.  Rows of query, key, value and outputs are 16-byte aligned
@@ -414,8 +414,8 @@ int mvb_kv_cache_write_fp8_workspace(int32_t num_tokens, int32_t num_blocks, int
  * float32 as one product, rounded, and one fused multiply-add, and rounded to
  * dtype.  The tables are
  * contiguous [table_rows, head_dim] (fewer than 2^31 rows) of `table_dtype`,
- * which is dtype or MVB_DTYPE_F32.  query_out may equal query; key_out (optional) is contiguous
- * [T, KH, D].  A position outside [0, table_rows) sets MVB_DEV_POSITION and
+ * which is dtype or MVB_DTYPE_F32.  query_out may equal query; key_out (optional)
+ * is contiguous [T, KH, D].  A position outside [0, table_rows) sets MVB_DEV_POSITION and
  * leaves all of that token's rows unwritten; slot -1 rotates the query and
  * writes nothing. */
 int mvb_rope_kv_cache_write_fp8(const void* query, int64_t q_stride_token, int64_t q_stride_head, void* query_out,
@@ -432,7 +432,9 @@ int mvb_rope_kv_cache_write_fp8(const void* query, int64_t q_stride_token, int64
 /* Paged decode attention over the 8-bit cache, one query token per sequence;
  * arguments, zero rows and device errors as in mvb_paged_decode (at most 6144
  * sequences, num_blocks * num_kv_heads * block_size below 2^31), and
- * MVB_DEV_TIMEOUT when a bounded wait on the device runs out.  `workspace` holds mvb_paged_decode_fp8_workspace bytes (same
+ * MVB_DEV_TIMEOUT when a bounded wait on the device runs out.  Logits below
+ * float32's range count for nothing (a row with no others is zeros).
+ * `workspace` holds mvb_paged_decode_fp8_workspace bytes (same
  * arguments; 256-byte aligned, contents arbitrary before and after); calls
  * that may overlap on the GPU need one each. */
 int mvb_paged_decode_fp8(const void* query, int64_t q_stride_seq, int64_t q_stride_head, const void* key_cache,
@@ -449,7 +451,8 @@ int mvb_paged_decode_fp8_workspace(int32_t num_seqs, int32_t num_heads, int32_t 
 /* Causal paged prefill attention over the 8-bit cache: mvb_paged_prefill with
  * every position, the chunk's own among them, read from the cache (written
  * before the call; at most 4096 chunks).  A block id outside [0, num_blocks) sets
- * MVB_DEV_BLOCK_ID and its tokens are left out; MVB_DEV_TIMEOUT as above.  `workspace` holds mvb_paged_prefill_fp8_workspace
+ * MVB_DEV_BLOCK_ID and its tokens are left out; MVB_DEV_TIMEOUT and logits
+ * below float32's range as above.  `workspace` holds mvb_paged_prefill_fp8_workspace
  * bytes (same arguments; 256-byte aligned, contents arbitrary before and after;
  * 0 bytes, and then unused, unless there are few rows); calls that may overlap on
  * the GPU need one each. */

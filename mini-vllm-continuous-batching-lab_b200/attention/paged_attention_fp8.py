@@ -1,9 +1,12 @@
 """The attention path over a KV cache held in 8 bits.
 
-Half the bytes of a bf16 pool: twice the tokens in the same memory, and a decode,
-which is bound by reading the cache, in about half the time.  The reference has no
-counterpart (its pool is 16 or 32 bits wide); names, arguments and errors follow
-``paged_attention_b200.py``.
+Half the bytes of a bf16 pool: twice the tokens in the same memory.  A decode takes
+0.56 of the 16-bit one's time (with its per-step schedule, both in a graph) where reading
+the cache is all of it (256 sequences of 32/8 heads of 128: 141 against 252 us), 0.65 for
+32 sequences of 32768 tokens (59 against 91 us), 0.72 for one of 1000, but 0.87 for 256
+sequences of up to 2048 (28.8 against 33.1 us), where half of it is set-up and merges.
+The reference has no counterpart (its pool is 16 or 32 bits wide); names, arguments and
+errors follow ``paged_attention_b200.py``.
 
 The cache of one layer is three tensors:
 
@@ -18,8 +21,8 @@ The cache of one layer is three tensors:
 that is a power of two from 16 to 1024.
 
 Scales belong to whole blocks: ``paged_cache_write_fp8`` says how they follow the rows
-that come in.  The writes make powers of two; the attention takes any positive finite
-scales, such as a calibration's (a block whose scale is 0, as in a new pool, holds zeros).
+that come in.  The writes make powers of two; the attention takes any positive normal
+float32 scales, such as a calibration's (a block whose scale is 0 holds zeros).
 """
 
 from __future__ import annotations
@@ -206,10 +209,10 @@ def rope_cache_write_fp8(
     ``cos`` / ``sin`` are tables ``[rows, head_dim]`` (see ``rope_tables``) in the rows' dtype or in float32.
     The written keys' scales and codes are those of the exact rotation rounded to float32; the query and the
     returned keys are computed in float32 (a product and a fused multiply-add) and rounded to the rows' dtype
-    (``rope_cache_write`` rounds after each operation, as the reference does).  Returns the rotated query (into ``query_out`` when given, which may be ``query`` itself
-    and overlaps no other argument) and, with ``return_key``, the rotated keys.  A position outside the tables
-    raises ``IndexError`` and leaves that token's rows unwritten; a token with slot -1 has its query rotated and
-    writes nothing.
+    (``rope_cache_write`` rounds after each operation, as the reference does).  Returns the rotated query (into
+    ``query_out`` when given, which may be ``query`` itself and overlaps no other argument) and, with
+    ``return_key``, the rotated keys.  A position outside the tables raises ``IndexError`` and leaves that token's
+    rows unwritten; a token with slot -1 has its query rotated and writes nothing.
     """
     fast = _native.fast()
     if fast is not None and key.is_cuda:
@@ -296,8 +299,9 @@ def paged_decode_attention_fp8(
 
     Arguments, result and errors are ``paged_decode_attention``'s, with ``kv_scale`` beside the caches.  The
     query enters the tensor cores as f16 (a bf16 row by a power of two, exact but for elements below 2**-14 of
-    its largest), probabilities as f16; logits, sums and the output are accumulated in float32.  The result does
-    not depend on timing.  At most 6144 sequences, and fewer than 2**31 cache rows (blocks * KV heads * block
+    its largest), probabilities as f16; logits, sums and the output are accumulated in float32.  Logits may be of any
+    size in float32; those below its range count for nothing (a row with no others is zeros).  The result does not
+    depend on timing.  At most 6144 sequences, and fewer than 2**31 cache rows (blocks * KV heads * block
     size).  The call keeps no state between calls and may be captured.
     """
     if scale is None:

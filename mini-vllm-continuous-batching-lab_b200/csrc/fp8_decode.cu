@@ -25,8 +25,8 @@
 //   down to 2^-4, where P's f16 still has 10 bits for p >= 2^-10; the rest of a
 //   smaller scale goes into the f16 codes (exact to 2^-15 R).
 // * P enters as f16 (11 bits; the output has 8 or 11), against a maximum m of
-//   earlier tiles; m is taken anew only when a lane's P add up to more than 2^14,
-//   so a tile needs no reduction across lanes, only a vote.
+//   earlier tiles; m is taken anew only when a lane's P add up to more than 2^14
+//   (once a tile), so a tile needs no reduction across lanes, only a vote.
 // * With a factor on every output of a tile and a maximum per tile, one tile at a
 //   time, it took 204 instructions per tile of head_dim 64 and was bound by them.
 //
@@ -39,9 +39,9 @@
 // one call to the next and needs no initialisation.
 // Bound: memory (1 byte per element; 28 operations per byte at 7 heads), short
 // sequences by the launches and the first loads.  Measured: 256 sequences of 32/8
-// heads of 128, 817 MB: 146 us, 5.6 TB/s; 32 x 32768 tokens of 14/2 heads of 64,
-// 270 MB: 59 us, 4.6 TB/s; 256 x 2048: 29 us, 16 of them the stream (4.7 TB/s), the
-// rest prologue and merges.
+// heads of 128, 817 MB: 157 us, 5.2 TB/s (141 us, 5.8 TB/s in a graph); 32 x 32768
+// tokens of 14/2 heads of 64, 270 MB: 60 us, 4.5 TB/s; 256 x 2048: 29 us, 16 of them the
+// stream (4.7 TB/s), the rest prologue and merges.
 #include <cudaTypedefs.h>
 
 #include <algorithm>

@@ -43,10 +43,10 @@
 // that attends the key gets NaN in that column at the end.
 //
 // Bound: a step (256 rows, 64 keys) has 1024 cycles of exponentials (16 per cycle
-// and SM) and, for head_dim 128, 1024 of the tensor core.  It takes about 2400: the
+// and SM) and, for head_dim 128, 1024 of the tensor core.  It takes about 2300: the
 // scores are always there when a softmax warp looks, and its own instructions in
 // turn (two such warps per scheduler) are what the step waits for; no unit is busy
-// for half of the time.  Tried (8192 tokens, against 287 us): columns read 32 or 64
+// for half of the time.  Tried (8192 tokens, against 287 us then): columns read 32 or 64
 // at a time: 308, 298; four row tiles of one S buffer each (16 softmax warps, each
 // of which then waits for its products): 318; two warps per row, each with half of a
 // step's keys and an O of its own: 284 to 290, and 20 against 17.5 us for 37 tokens;
